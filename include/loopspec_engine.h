@@ -15,6 +15,7 @@
 #ifndef LOOPSPEC_ENGINE_H
 #define LOOPSPEC_ENGINE_H
 
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -327,6 +328,132 @@ int ls_decode_attention_noalloc(const float* q, const void* k_pool, const void* 
                                 int head_dim, int n_slots, int n_rows, int max_context, float* out,
                                 void* stream);
 size_t ls_decode_attention_noalloc_limit(void);
+
+/* ---- One step of a batch whose requests share a long prefix --------------
+ *
+ * Three handle-less operators over paged K/V (blocks of page_size slots, a
+ * power of two up to 1024; page_size 1 is the engine's own layout): slot maps
+ * from request lengths, the per-head norm with the position rotation and the
+ * K/V write, and the attention over a shared prefix and each request's own
+ * positions. They have no counterpart in the reference, which serves one
+ * request at a time (server/cli.py:88-89).
+ *
+ * Pointers are device memory unless said otherwise; each call enqueues its
+ * kernels on `stream` (cudaStream_t, NULL = legacy default) of the current
+ * device and returns without waiting, so it can be captured in a CUDA graph.
+ * What the host can check is refused with LS_EINVAL (ls_last_error(NULL)).
+ * What only the GPU sees -- a length, position, slot or block out of range --
+ * is skipped and recorded in *status, an int32 the caller clears to 0 and
+ * reads with ls_check_status. Types: LS_BF16, LS_F16, LS_F32. */
+#define LS_BF16 0
+#define LS_F16 1
+#define LS_F32 2
+
+/* Wait for `stream`, read and clear *status (device memory). LS_OK, or
+ * LS_ECAPACITY (free blocks or token buffers exhausted) or LS_EDEVICE (an
+ * index or length out of range). */
+int ls_check_status(int32_t* status, void* stream);
+
+/* Block tables and slot maps from request lengths. Request i holds lens[i]
+ * tokens and changes by delta[i]: new tokens if positive, cut back if negative
+ * (rejected drafts; -lens[i] releases the request). Blocks it no longer needs
+ * are pushed on the stack free_blocks[0 .. free_count), in request order and
+ * ascending block index; then new blocks are popped, one after the other in
+ * request order, and entered in its table row. Entry k < token_start[R] of the
+ * token buffers describes new token k: its slot, its position (base + index in
+ * the request) and its request; entries past it get -1, 0, -1. All or nothing:
+ * when a length is out of range, the blocks do not suffice or the tokens do
+ * not fit, lens and the count keep their values, table and stack are left
+ * alone, token_start is all 0 and *status tells why. lens_out / free_count_out
+ * may be lens / free_count. */
+typedef struct ls_slots_args {
+  const int32_t* lens;        /* [R]                                          */
+  const int32_t* delta;       /* [R]                                          */
+  int32_t* block_table;       /* [R][table_width], rows table_stride apart    */
+  int64_t table_stride;
+  int32_t* free_blocks;       /* [free_capacity]                              */
+  const int32_t* free_count;  /* [1]                                          */
+  int32_t* slots;             /* [max_tokens]                                 */
+  int32_t* positions;         /* [max_tokens]                                 */
+  int32_t* requests;          /* [max_tokens]                                 */
+  int32_t* token_start;       /* [R + 1]                                      */
+  int32_t* lens_out;          /* [R]                                          */
+  int32_t* free_count_out;    /* [1]                                          */
+  int32_t* status;
+  int32_t n_requests;         /* R, 1 .. 16384                                */
+  int32_t table_width, free_capacity, n_blocks, page_size, base, max_tokens;
+} ls_slots_args;
+int ls_build_slots(const ls_slots_args* args, void* stream);
+
+/* Per-head RMS norm of q and k, position rotation, K/V to their slots. qkv:
+ * [T] rows of (n_heads + 2 n_kv_heads) * head_dim values, q heads then k then
+ * v (the packed projection). Each q and k head x becomes
+ * x * rsqrt(mean(x^2) + eps) * weight, its first `rot` dimensions rotated by
+ * the angles of positions[t]: rope [max_positions][2][rot/2] holds fp32
+ * cosines, then sines; pairs are (i, i + rot/2), or (2i, 2i + 1) with
+ * interleaved. q_out gets q in qkv's type (it may be qkv's own q part); k and
+ * v go to rows slots[t] of the pools (row t when slots is null, nowhere where
+ * it is -1). fp32 arithmetic, one rounding. head_dim 64 or 128; rot a multiple
+ * of 16; rows and pool rows 16-byte aligned. */
+typedef struct ls_qk_norm_args {
+  const void* qkv;
+  int64_t qkv_stride;         /* elements between rows                        */
+  const void* q_weight;       /* [head_dim]                                   */
+  const void* k_weight;
+  const float* rope;
+  const int32_t* positions;   /* [T]                                          */
+  const int32_t* slots;       /* [T] or null                                  */
+  void* k_pool;               /* [n_slots][n_kv_heads * head_dim]             */
+  void* v_pool;
+  int64_t slot_stride;        /* elements between pool rows                   */
+  void* q_out;
+  int64_t q_out_stride;
+  int32_t* status;
+  int32_t qkv_type, weight_type, cache_type;
+  int32_t n_tokens, n_heads, n_kv_heads, head_dim;
+  int32_t max_positions, rot, interleaved, n_slots;
+  float eps;
+} ls_qk_norm_args;
+int ls_qk_norm_rope(const ls_qk_norm_args* args, void* stream);
+
+/* Attention of a batch over one shared prefix and each request's own
+ * positions. Tokens token_start[i] .. token_start[i+1] are the newest of
+ * request i's lens[i] own positions (K/V already in the pools); token t
+ * attends to all prefix_len prefix positions and to own positions
+ * 0 .. lens[i] - n_i + (t - token_start[i]). Position p of the prefix is in
+ * slot prefix_table[p / page_size] * page_size + p % page_size, those of
+ * request i likewise through row i of block_table. The prefix is read once for
+ * the whole batch. q, out: [T][n_heads][head_dim], of the cache's type (bf16
+ * or f16) or fp32, which keeps fp32-like precision (|q| < 65504 with an f16
+ * cache). A token that sees nothing, or past token_start[R], gets zeros.
+ * max_new and max_len bound the requests' new tokens and lengths (they size
+ * the launch). workspace: ls_prefix_attention_workspace_bytes() bytes,
+ * 256-byte aligned; calls that share one must not overlap. head_dim 64 or
+ * 128; any n_heads / n_kv_heads. */
+typedef struct ls_prefix_attention_args {
+  const void* q;
+  int64_t q_stride;           /* elements between tokens                      */
+  const void* k_pool;         /* [n_slots][n_kv_heads * head_dim]             */
+  const void* v_pool;
+  int64_t slot_stride;        /* elements between pool rows                   */
+  const int32_t* prefix_table;
+  const int32_t* block_table; /* [R], rows table_stride apart                 */
+  int64_t table_stride;
+  const int32_t* lens;        /* [R]                                          */
+  const int32_t* token_start; /* [R + 1]                                      */
+  void* out;
+  int64_t out_stride;
+  void* workspace;
+  uint64_t workspace_bytes;
+  int32_t* status;
+  int32_t q_type, cache_type;
+  int32_t n_tokens, n_requests, n_heads, n_kv_heads, head_dim;
+  int32_t prefix_len, max_new, max_len, page_size, n_slots;
+  float scale;
+} ls_prefix_attention_args;
+size_t ls_prefix_attention_workspace_bytes(int n_tokens, int n_requests, int n_heads, int n_kv_heads,
+                                           int head_dim, int prefix_len, int max_new, int max_len);
+int ls_prefix_attention(const ls_prefix_attention_args* args, void* stream);
 
 int ls_destroy(ls_engine* eng);
 const char* ls_last_error(ls_engine* eng);

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libloopspec_engine.so")
@@ -57,6 +58,54 @@ class Stats(ctypes.Structure):
 
     def as_dict(self):
         return {name: getattr(self, name) for name, _ in self._fields_}
+
+
+_VP = ctypes.c_void_p
+
+
+class SlotsArgs(ctypes.Structure):
+    _fields_ = [
+        ("lens", _VP), ("delta", _VP), ("block_table", _VP), ("table_stride", _i64), ("free_blocks", _VP),
+        ("free_count", _VP), ("slots", _VP), ("positions", _VP), ("requests", _VP), ("token_start", _VP),
+        ("lens_out", _VP), ("free_count_out", _VP), ("status", _VP),
+        ("n_requests", _i32), ("table_width", _i32), ("free_capacity", _i32), ("n_blocks", _i32),
+        ("page_size", _i32), ("base", _i32), ("max_tokens", _i32),
+    ]
+
+
+class QkNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("qkv", _VP), ("qkv_stride", _i64), ("q_weight", _VP), ("k_weight", _VP), ("rope", _VP),
+        ("positions", _VP), ("slots", _VP), ("k_pool", _VP), ("v_pool", _VP), ("slot_stride", _i64),
+        ("q_out", _VP), ("q_out_stride", _i64), ("status", _VP),
+        ("qkv_type", _i32), ("weight_type", _i32), ("cache_type", _i32), ("n_tokens", _i32),
+        ("n_heads", _i32), ("n_kv_heads", _i32), ("head_dim", _i32), ("max_positions", _i32), ("rot", _i32),
+        ("interleaved", _i32), ("n_slots", _i32), ("eps", _f32),
+    ]
+
+
+class PrefixAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _VP), ("q_stride", _i64), ("k_pool", _VP), ("v_pool", _VP), ("slot_stride", _i64),
+        ("prefix_table", _VP), ("block_table", _VP), ("table_stride", _i64), ("lens", _VP),
+        ("token_start", _VP), ("out", _VP), ("out_stride", _i64), ("workspace", _VP),
+        ("workspace_bytes", _u64), ("status", _VP),
+        ("q_type", _i32), ("cache_type", _i32), ("n_tokens", _i32), ("n_requests", _i32),
+        ("n_heads", _i32), ("n_kv_heads", _i32), ("head_dim", _i32), ("prefix_len", _i32),
+        ("max_new", _i32), ("max_len", _i32), ("page_size", _i32), ("n_slots", _i32), ("scale", _f32),
+    ]
+
+
+_CODES = {_VP: "P", _i64: "q", _u64: "Q", _i32: "i", _f32: "f"}
+
+
+def packer(args):
+    """pack(*fields) -> the bytes of the argument struct `args`, in field order.
+    A call of one of these operators takes a few microseconds; packing costs a
+    third of one, filling a ctypes Structure several."""
+    form = struct.Struct("@" + "".join(_CODES[kind] for _, kind in args._fields_) + "0P")
+    assert form.size == ctypes.sizeof(args)
+    return form.pack
 
 
 DECIDE_FN = ctypes.CFUNCTYPE(ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int32)
@@ -114,6 +163,11 @@ SIGNATURES = [
     ("ls_decode_attention_noalloc", _i32, [_P, _P, _P, _P, _P, _P, _i32, _i32, _i32, _i32, _i32,
                                            _i32, _i32, _P, _P]),
     ("ls_decode_attention_noalloc_limit", ctypes.c_size_t, []),
+    ("ls_check_status", _i32, [_P, _P]),
+    ("ls_build_slots", _i32, [ctypes.c_char_p, _P]),
+    ("ls_qk_norm_rope", _i32, [ctypes.c_char_p, _P]),
+    ("ls_prefix_attention_workspace_bytes", ctypes.c_size_t, [_i32] * 8),
+    ("ls_prefix_attention", _i32, [ctypes.c_char_p, _P]),
     ("ls_destroy", _i32, [_P]),
     ("ls_last_error", ctypes.c_char_p, [_P]),
     ("ls_version", ctypes.c_char_p, []),

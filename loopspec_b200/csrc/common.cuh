@@ -20,6 +20,9 @@ enum DeviceError : int {
   kDevBadIndex = 4,       // a metadata index was out of range (access skipped)
   // 5 and 6 are unused
   kDevTimeoutPeer = 7,    // a tensor-parallel peer did not publish its partials in time
+  kDevBadLength = 8,      // a length, count or token range is out of its bounds (work skipped)
+  kDevNoBlocks = 9,       // the free blocks do not cover the growth (nothing changed)
+  kDevTooManyTokens = 10, // more new tokens than the token buffers hold (nothing changed)
 };
 
 // Lane metadata: int32 [cap][kMetaFields], lane-major (one record per lane,
@@ -306,6 +309,28 @@ __device__ __forceinline__ void store_pair4(__nv_bfloat16* x, long K, int b, lon
   }
   *reinterpret_cast<uint2*>(x + (2L * b) * K + i) = *reinterpret_cast<uint2*>(hi);
   *reinterpret_cast<uint2*>(x + (2L * b + 1) * K + i) = *reinterpret_cast<uint2*>(lo);
+}
+
+// -------------------------------------------------- mma.sync / ldmatrix fragments
+__device__ __forceinline__ uint32_t pack_bf16(float lo_elem, float hi_elem) {
+  // element 0 (lower column) in the low half, as mma fragments expect
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo_elem, hi_elem);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void* p) {
+  const uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
 }
 
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw, SC'11), counter = (i/4, pos, 0, 0).

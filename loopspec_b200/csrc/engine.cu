@@ -15,6 +15,7 @@
 #include "common.cuh"
 #include "dev_sched.cuh"
 #include "gemm_tc.cuh"
+#include "host.cuh"
 #include "kernels.cuh"
 #include "prefill_attn.cuh"
 #include "sampler.cuh"
@@ -41,25 +42,8 @@ typedef __nv_bfloat16 bf16;
 
 namespace {
 
-struct EngineError : std::runtime_error {
-  int code;
-  EngineError(int c, const std::string& m) : std::runtime_error(m), code(c) {}
-};
-
 // Error text of the last failed call that has no engine handle.
 thread_local std::string g_last_error;
-
-#define CK(x)                                                                            \
-  do {                                                                                   \
-    cudaError_t e_ = (x);                                                                \
-    if (e_ != cudaSuccess)                                                               \
-      throw EngineError(LS_ECUDA, std::string(#x) + ": " + cudaGetErrorString(e_));      \
-  } while (0)
-
-#define REQUIRE(cond, code, msg)                  \
-  do {                                                \
-    if (!(cond)) throw EngineError((code), (msg));    \
-  } while (0)
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -139,23 +123,6 @@ struct StackEnd {
   bool want_x = false;               // produce x for a following GEMM
   const bf16* x_norm = nullptr;      // ... normalised by this weight (Raven ln_f)
 };
-
-// Launch with optional programmatic-dependent-launch attribute.
-template <typename... KArgs, typename... Args>
-void launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool pdl,
-            Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = pdl ? attr : nullptr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  CK(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
-}
 
 double now_s() {
   return std::chrono::duration<double>(std::chrono::steady_clock::now().time_since_epoch()).count();
@@ -2282,13 +2249,13 @@ int fail(ls_engine* e, const std::exception& ex) {
 }  // namespace
 
 // ================================================ standalone decode attention
-namespace {
-
-int fail_global(const std::exception& ex) {
+int ls::fail_global(const std::exception& ex) {
   const EngineError* ee = dynamic_cast<const EngineError*>(&ex);
   g_last_error = ex.what();
   return ee ? ee->code : LS_EINVAL;
 }
+
+namespace {
 
 // Scratch of one decode-attention call, carved from a byte buffer: an error
 // word, the per-chunk partials (acc, then max/sum) and the arrival tickets.

@@ -39,32 +39,11 @@ constexpr size_t pattn_smem_bytes() {
   return (size_t)2 * 2 * kPAttnKeys * pattn_row_bytes<HD>();   // 2 buffers x (K, V)
 }
 
-__device__ __forceinline__ uint32_t pack_bf16(float lo_elem, float hi_elem) {
-  // element 0 (lower column) in the low half, as mma fragments expect
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo_elem, hi_elem);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
 // (hi, lo) bf16 split of a pair of fp32 values, packed for a fragment register.
 __device__ __forceinline__ void split_pair(float x0, float x1, uint32_t& hi, uint32_t& lo) {
   const __nv_bfloat16 h0 = __float2bfloat16_rn(x0), h1 = __float2bfloat16_rn(x1);
   hi = pack_bf16(__bfloat162float(h0), __bfloat162float(h1));
   lo = pack_bf16(x0 - __bfloat162float(h0), x1 - __bfloat162float(h1));
-}
-
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], const void* p) {
-  const uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(a));
 }
 
 

@@ -1,0 +1,342 @@
+// C entry points of the shared-prefix serving step: slot maps, per-head norm
+// with rotation and K/V write, prefix attention. Each checks its arguments,
+// picks the kernel variant and enqueues; none waits or allocates.
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "host.cuh"
+#include "prefix_attn.cuh"
+#include "qk_norm.cuh"
+#include "slots.cuh"
+
+using namespace ls;
+typedef __nv_bfloat16 bf16;
+
+namespace {
+
+int sm_count() {
+  int dev = 0, sms = 0;
+  CK(cudaGetDevice(&dev));
+  CK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  return sms;
+}
+
+int cdiv(long a, long b) { return (int)((a + b - 1) / b); }
+
+int page_shift_of(int page_size, const char* who) {
+  int s = 0;
+  while (s < 10 && (1 << s) < page_size) ++s;
+  REQUIRE(page_size >= 1 && (1 << s) == page_size, LS_EINVAL,
+          std::string(who) + ": page_size must be a power of two in [1, 1024]");
+  return s;
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+long type_bytes(int type) { return type == LS_F32 ? 4 : 2; }
+
+// Dynamic shared memory above the default limit is granted once a kernel and device.
+template <typename K>
+void allow_smem(K kernel, size_t bytes) {
+  if (bytes > 48 * 1024)
+    CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+}
+
+template <typename F>
+int guarded(F f) {
+  try {
+    f();
+  } catch (const std::exception& ex) {
+    return fail_global(ex);
+  } catch (...) {
+    return fail_global(EngineError(LS_EINVAL, "unknown failure"));
+  }
+  return LS_OK;
+}
+
+// ------------------------------------------------------------------- slot maps
+void run_build_slots(const ls_slots_args& p, cudaStream_t stream) {
+  const char* who = "slot maps";
+  REQUIRE(p.lens && p.delta && p.block_table && p.free_blocks && p.free_count && p.token_start &&
+              p.lens_out && p.free_count_out && p.status,
+          LS_EINVAL, "slot maps: null pointer argument");
+  REQUIRE(p.max_tokens >= 0 && (p.max_tokens == 0 || (p.slots && p.positions && p.requests)), LS_EINVAL,
+          "slot maps: max_tokens must not be negative and its buffers not null");
+  REQUIRE(p.n_requests >= 1 && p.n_requests <= kSlotMaxRequests, LS_EINVAL,
+          "slot maps: n_requests must be in [1, " + std::to_string(kSlotMaxRequests) + "]");
+  REQUIRE(p.table_width >= 1 && p.table_stride >= p.table_width && p.free_capacity >= 0 && p.n_blocks >= 1,
+          LS_EINVAL, "slot maps: table_width, table_stride, free_capacity or n_blocks out of range");
+  const int shift = page_shift_of(p.page_size, who);
+  const int64_t kTop = INT32_MAX;
+  REQUIRE((int64_t)p.n_blocks << shift <= kTop && (int64_t)p.table_width << shift <= kTop &&
+              (int64_t)p.n_requests * p.table_width <= kTop && p.base >= 0 &&
+              (int64_t)p.base + ((int64_t)p.table_width << shift) <= kTop,
+          LS_EINVAL, "slot maps: slots, positions and table entries must stay below 2^31");
+  SlotArgs a{p.lens, p.delta, p.n_requests, p.block_table, (long)p.table_stride, p.table_width,
+             p.free_blocks, p.free_capacity, p.free_count, p.n_blocks, shift, p.base, p.max_tokens,
+             p.slots, p.positions, p.requests, p.token_start, p.lens_out, p.free_count_out, p.status};
+  const size_t smem = slot_smem_bytes(p.n_requests);
+  allow_smem(build_slots_kernel, smem);
+  // one CTA while every thread has at most 4 tokens; more CTAs share the
+  // stores of a prompt batch but each repeats the sums
+  int ctas = 1;
+  while (ctas < kSlotMaxCluster && (long)ctas * kSlotThreads * 4 < std::max(p.max_tokens, p.n_requests)) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kSlotThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  CK(cudaLaunchKernelEx(&cfg, build_slots_kernel, a));
+}
+
+// ----------------------------------------------------------- norm and rotation
+template <typename T, typename C, int HD>
+void launch_qk(const QkNormArgs& a, bool interleaved, cudaStream_t stream) {
+  constexpr int kHeads = kQkThreads * 16 / HD;
+  const dim3 grid(a.n_tokens, cdiv(a.nh + 2 * a.nkv, kHeads));
+  if (interleaved) launch(qk_norm_rope_kernel<T, C, HD, true>, grid, dim3(kQkThreads), 0, stream, false, a);
+  else launch(qk_norm_rope_kernel<T, C, HD, false>, grid, dim3(kQkThreads), 0, stream, false, a);
+}
+
+template <typename T, typename C>
+void launch_qk(const QkNormArgs& a, int hd, bool interleaved, cudaStream_t stream) {
+  if (hd == 64) launch_qk<T, C, 64>(a, interleaved, stream);
+  else launch_qk<T, C, 128>(a, interleaved, stream);
+}
+
+void run_qk_norm_rope(const ls_qk_norm_args& p, cudaStream_t stream) {
+  REQUIRE(p.n_tokens >= 0, LS_EINVAL, "qk norm: n_tokens must not be negative");
+  REQUIRE(p.n_heads >= 1 && p.n_kv_heads >= 1 && (p.head_dim == 64 || p.head_dim == 128), LS_EINVAL,
+          "qk norm: head counts must be positive and head_dim 64 or 128");
+  REQUIRE(p.qkv_type >= LS_BF16 && p.qkv_type <= LS_F32 && p.weight_type >= LS_BF16 && p.weight_type <= LS_F32 &&
+              (p.cache_type == LS_BF16 || p.cache_type == LS_F16) &&
+              (p.qkv_type == LS_F32 || p.qkv_type == p.cache_type),
+          LS_EINVAL, "qk norm: the cache must be bf16 or f16, and qkv of its type or fp32");
+  REQUIRE(p.rot >= 16 && p.rot % 16 == 0 && p.rot <= p.head_dim, LS_EINVAL,
+          "qk norm: rot must be a multiple of 16 up to head_dim");
+  REQUIRE(p.max_positions >= 1 && p.n_slots >= 1, LS_EINVAL, "qk norm: max_positions and n_slots must be positive");
+  const int64_t qd = (int64_t)p.n_heads * p.head_dim, kd = (int64_t)p.n_kv_heads * p.head_dim;
+  REQUIRE(p.qkv_stride >= qd + 2 * kd && p.q_out_stride >= qd && p.slot_stride >= kd, LS_EINVAL,
+          "qk norm: a stride is smaller than its row");
+  if (p.n_tokens == 0) return;
+  REQUIRE(p.qkv && p.q_weight && p.k_weight && p.rope && p.positions && p.k_pool && p.v_pool && p.q_out && p.status,
+          LS_EINVAL, "qk norm: null pointer argument");
+  const long eb = type_bytes(p.qkv_type), cb = type_bytes(p.cache_type);
+  REQUIRE(aligned16(p.qkv) && aligned16(p.q_weight) && aligned16(p.k_weight) && aligned16(p.rope) &&
+              aligned16(p.k_pool) && aligned16(p.v_pool) && aligned16(p.q_out) && p.qkv_stride * eb % 16 == 0 &&
+              p.q_out_stride * eb % 16 == 0 && p.slot_stride * cb % 16 == 0,
+          LS_EINVAL, "qk norm: pointers and row strides must be 16-byte aligned");
+  QkNormArgs a{p.qkv, (long)p.qkv_stride, p.n_tokens, p.n_heads, p.n_kv_heads, p.q_weight, p.k_weight,
+               p.weight_type, p.eps, p.rope, p.max_positions, p.rot, p.positions, p.slots, p.k_pool, p.v_pool,
+               (long)p.slot_stride, p.n_slots, p.q_out, (long)p.q_out_stride, p.status};
+  const bool il = p.interleaved != 0;
+  if (p.qkv_type == LS_BF16) launch_qk<bf16, bf16>(a, p.head_dim, il, stream);
+  else if (p.qkv_type == LS_F16) launch_qk<__half, __half>(a, p.head_dim, il, stream);
+  else if (p.cache_type == LS_BF16) launch_qk<float, bf16>(a, p.head_dim, il, stream);
+  else launch_qk<float, __half>(a, p.head_dim, il, stream);
+}
+
+// ------------------------------------------------------------ prefix attention
+// How a call is cut into units: a function of its sizes alone.
+struct PrefixPlan {
+  int prefix_parts, prefix_chunk, suffix_parts, suffix_chunk, prefix_tiles, suffix_tiles;
+  size_t o_bytes, ml_bytes, total;
+};
+
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Key ranges for `len` positions of `units` row tiles: enough that the SMs
+// hold about two units each, none under 256 positions.
+void cut(long units, int len, int sms, int& parts, int& chunk) {
+  parts = chunk = 0;
+  if (len == 0) return;
+  const long want = std::max(1L, (2L * sms) / std::max(1L, units));
+  const int most = std::max(1, len / 256);
+  parts = (int)std::min<long>(want, most);
+  chunk = cdiv(cdiv(len, parts), 64) * 64;
+  parts = cdiv(len, chunk);
+}
+
+PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int prefix_len, int max_new,
+                     int max_len, int sms) {
+  PrefixPlan p{};
+  const int G = nh / nkv;
+  p.prefix_tiles = cdiv((long)n_tokens * G, 16);
+  p.suffix_tiles = cdiv((long)std::min(max_new, n_tokens) * G, 16);
+  cut((long)p.prefix_tiles * nkv, prefix_len, sms, p.prefix_parts, p.prefix_chunk);
+  cut((long)p.suffix_tiles * nkv * n_requests, max_len, sms, p.suffix_parts, p.suffix_chunk);
+  const size_t rows = (size_t)(p.prefix_parts + p.suffix_parts) * n_tokens * nh;
+  p.o_bytes = round256(rows * hd * sizeof(float));
+  p.ml_bytes = round256(rows * sizeof(float2));
+  p.total = p.o_bytes + p.ml_bytes;
+  return p;
+}
+
+template <int HD, typename Q, typename C, int TERMS>
+void launch_prefix(const PrefixAttnArgs& a, cudaStream_t stream) {
+  const long units = (long)a.prefix_parts * a.prefix_tiles * a.nkv +
+                     (long)a.suffix_parts * a.suffix_tiles * a.nkv * a.n_requests;
+  REQUIRE(units <= INT32_MAX, LS_EINVAL, "prefix attention: too many units for one launch");
+  if (units > 0) {
+    const size_t smem = unit_smem_bytes<HD>();
+    allow_smem(prefix_unit_kernel<HD, Q, C, TERMS>, smem);
+    launch(prefix_unit_kernel<HD, Q, C, TERMS>, dim3((unsigned)units), dim3(kUnitThreads), smem, stream, false, a);
+  }
+  const int per = kJoinThreads / (HD / 4);
+  launch(prefix_join_kernel<HD, Q>, dim3((unsigned)cdiv((long)a.n_tokens * a.nh, per)), dim3(kJoinThreads), 0,
+         stream, false, a);
+}
+
+template <typename Q, typename C, int TERMS>
+void launch_prefix(const PrefixAttnArgs& a, int hd, cudaStream_t stream) {
+  if (hd == 64) launch_prefix<64, Q, C, TERMS>(a, stream);
+  else launch_prefix<128, Q, C, TERMS>(a, stream);
+}
+
+void check_prefix_sizes(int n_tokens, int n_requests, int nh, int nkv, int hd, int prefix_len, int max_new,
+                        int max_len) {
+  REQUIRE(n_tokens >= 0 && n_requests >= 1 && nh >= 1 && nkv >= 1 && prefix_len >= 0 && max_new >= 0 && max_len >= 0,
+          LS_EINVAL, "prefix attention: sizes must not be negative, requests and heads positive");
+  REQUIRE(nh % nkv == 0, LS_EINVAL, "prefix attention: n_heads must be a multiple of n_kv_heads");
+  REQUIRE(hd == 64 || hd == 128, LS_EINVAL, "prefix attention: head_dim must be 64 or 128");
+  REQUIRE((int64_t)n_tokens * nh <= INT32_MAX, LS_EINVAL, "prefix attention: too many query rows");
+}
+
+void run_prefix_attention(const ls_prefix_attention_args& p, cudaStream_t stream) {
+  check_prefix_sizes(p.n_tokens, p.n_requests, p.n_heads, p.n_kv_heads, p.head_dim, p.prefix_len, p.max_new,
+                     p.max_len);
+  REQUIRE((p.cache_type == LS_BF16 || p.cache_type == LS_F16) &&
+              (p.q_type == LS_F32 || p.q_type == p.cache_type),
+          LS_EINVAL, "prefix attention: the cache must be bf16 or f16, and q of its type or fp32");
+  REQUIRE(p.n_slots >= 1 && std::isfinite(p.scale), LS_EINVAL,
+          "prefix attention: n_slots must be positive and the scale finite");
+  const int shift = page_shift_of(p.page_size, "prefix attention");
+  const int64_t qd = (int64_t)p.n_heads * p.head_dim, kd = (int64_t)p.n_kv_heads * p.head_dim;
+  REQUIRE(p.q_stride >= qd && p.out_stride >= qd && p.slot_stride >= kd &&
+              p.table_stride >= cdiv(p.max_len, p.page_size),
+          LS_EINVAL, "prefix attention: a stride is smaller than its row");
+  if (p.n_tokens == 0) return;
+  REQUIRE(p.q && p.k_pool && p.v_pool && p.lens && p.token_start && p.out && p.workspace && p.status &&
+              (p.prefix_table || p.prefix_len == 0) && (p.block_table || p.max_len == 0),
+          LS_EINVAL, "prefix attention: null pointer argument");
+  const long eb = type_bytes(p.q_type);
+  REQUIRE(aligned16(p.q) && aligned16(p.k_pool) && aligned16(p.v_pool) && aligned16(p.out) &&
+              p.q_stride * eb % 16 == 0 && p.out_stride * eb % 16 == 0 && p.slot_stride * 2 % 16 == 0,
+          LS_EINVAL, "prefix attention: pointers and row strides must be 16-byte aligned");
+  const PrefixPlan plan = make_plan(p.n_tokens, p.n_requests, p.n_heads, p.n_kv_heads, p.head_dim, p.prefix_len,
+                                    p.max_new, p.max_len, sm_count());
+  REQUIRE((reinterpret_cast<uintptr_t>(p.workspace) & 255) == 0, LS_EINVAL,
+          "prefix attention: workspace must be 256-byte aligned");
+  REQUIRE(p.workspace_bytes >= plan.total, LS_EINVAL,
+          "prefix attention: workspace smaller than ls_prefix_attention_workspace_bytes()");
+  char* w = static_cast<char*>(p.workspace);
+  PrefixAttnArgs a{};
+  a.q = p.q;
+  a.q_stride = (long)p.q_stride;
+  a.k_pool = p.k_pool;
+  a.v_pool = p.v_pool;
+  a.slot_stride = (long)p.slot_stride;
+  a.n_slots = p.n_slots;
+  a.prefix_table = p.prefix_table;
+  a.prefix_len = p.prefix_len;
+  a.block_table = p.block_table;
+  a.table_stride = (long)p.table_stride;
+  a.lens = p.lens;
+  a.token_start = p.token_start;
+  a.n_requests = p.n_requests;
+  a.n_tokens = p.n_tokens;
+  a.max_new = p.max_new;
+  a.max_len = p.max_len;
+  a.page_shift = shift;
+  a.nh = p.n_heads;
+  a.nkv = p.n_kv_heads;
+  a.scale_log2 = (float)((double)p.scale * 1.4426950408889634);
+  a.out = p.out;
+  a.out_stride = (long)p.out_stride;
+  a.part_o = reinterpret_cast<float*>(w);
+  a.part_ml = reinterpret_cast<float2*>(w + plan.o_bytes);
+  a.prefix_parts = plan.prefix_parts;
+  a.prefix_chunk = plan.prefix_chunk;
+  a.suffix_parts = plan.suffix_parts;
+  a.suffix_chunk = plan.suffix_chunk;
+  a.prefix_tiles = plan.prefix_tiles;
+  a.suffix_tiles = plan.suffix_tiles;
+  a.status = p.status;
+  if (p.q_type == LS_BF16) launch_prefix<bf16, bf16, 1>(a, p.head_dim, stream);
+  else if (p.q_type == LS_F16) launch_prefix<__half, __half, 1>(a, p.head_dim, stream);
+  else if (p.cache_type == LS_BF16) launch_prefix<float, bf16, 3>(a, p.head_dim, stream);
+  else launch_prefix<float, __half, 2>(a, p.head_dim, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ls_check_status(int32_t* status, void* stream) {
+  return guarded([&] {
+    REQUIRE(status, LS_EINVAL, "status: null pointer argument");
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int32_t code = 0;
+    CK(cudaMemcpyAsync(&code, status, sizeof(code), cudaMemcpyDeviceToHost, s));
+    CK(cudaStreamSynchronize(s));
+    if (code == kDevOk) return;
+    CK(cudaMemsetAsync(status, 0, sizeof(code), s));
+    CK(cudaStreamSynchronize(s));
+    switch (code) {
+      case kDevNoBlocks:
+        throw EngineError(LS_ECAPACITY, "device reported: the free blocks do not cover the requests' growth");
+      case kDevTooManyTokens:
+        throw EngineError(LS_ECAPACITY, "device reported: more new tokens than max_tokens");
+      case kDevBadLength:
+        throw EngineError(LS_EDEVICE, "device reported: a length, count or token range is out of its bounds");
+      case kDevBadIndex:
+        throw EngineError(LS_EDEVICE, "device reported: a position, block or slot is out of range");
+      case kDevTimeoutFull:
+      case kDevTimeoutEmpty:
+      case kDevTimeoutAcc:
+        throw EngineError(LS_EDEVICE, "device reported: a wait inside a kernel timed out");
+      default:
+        throw EngineError(LS_EDEVICE, "device reported: unknown error " + std::to_string(code));
+    }
+  });
+}
+
+int ls_build_slots(const ls_slots_args* args, void* stream) {
+  return guarded([&] {
+    REQUIRE(args, LS_EINVAL, "slot maps: null argument struct");
+    run_build_slots(*args, static_cast<cudaStream_t>(stream));
+  });
+}
+
+int ls_qk_norm_rope(const ls_qk_norm_args* args, void* stream) {
+  return guarded([&] {
+    REQUIRE(args, LS_EINVAL, "qk norm: null argument struct");
+    run_qk_norm_rope(*args, static_cast<cudaStream_t>(stream));
+  });
+}
+
+size_t ls_prefix_attention_workspace_bytes(int n_tokens, int n_requests, int n_heads, int n_kv_heads, int head_dim,
+                                           int prefix_len, int max_new, int max_len) {
+  size_t bytes = 0;
+  guarded([&] {
+    check_prefix_sizes(n_tokens, n_requests, n_heads, n_kv_heads, head_dim, prefix_len, max_new, max_len);
+    bytes = std::max<size_t>(256, make_plan(n_tokens, n_requests, n_heads, n_kv_heads, head_dim, prefix_len,
+                                            max_new, max_len, sm_count()).total);
+  });
+  return bytes;   // 0: refused, see ls_last_error(NULL)
+}
+
+int ls_prefix_attention(const ls_prefix_attention_args* args, void* stream) {
+  return guarded([&] {
+    REQUIRE(args, LS_EINVAL, "prefix attention: null argument struct");
+    run_prefix_attention(*args, static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,208 @@
+// Block tables and slot maps from request lengths, on the GPU.
+//
+// Request i holds len_i tokens in blocks of `page` slots (its table row) and
+// changes by delta_i: it grows (delta_i new tokens) or is cut back (rejected
+// drafts, a finished request). With have = ceil(len / page) and
+// need = ceil((len + delta) / page) it takes max(0, need - have) blocks and
+// gives back max(0, have - need). The free blocks are a stack; what is given
+// back is pushed first, in request order and ascending block index, then the
+// k-th new block (request order) is popped: entry count + given - 1 - k. New
+// token j of request i sits at position len_i + j, in slot
+// table[i][pos / page] * page + pos % page.
+//
+// One launch, one thread-block cluster. Every CTA computes the three running
+// sums over the requests (tokens, blocks taken, blocks given back) by itself,
+// a few KB from L2, so no CTA waits for another's; then tokens and blocks are
+// spread over the cluster, each found by a binary search in the sums. A pop
+// that reaches below the stack's old top reads the giving request's table
+// entry itself and pushes write only above it, so no read of the call meets a
+// write of the call; lens and the count, which may be updated in place, are
+// written after a cluster barrier. Nothing changes when the call cannot be
+// done as a whole.
+//
+// Bound: launch and dependent-load latency (a decode step moves a few KB).
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include "common.cuh"
+
+namespace ls {
+
+constexpr int kSlotThreads = 512;
+constexpr int kSlotMaxCluster = 8;       // portable cluster size
+constexpr int kSlotMaxRequests = 16384;  // three int32 sums a request in shared memory: 192 KB
+
+struct SlotArgs {
+  const int* lens;
+  const int* delta;
+  int n_requests;
+  int* table;
+  long table_stride;
+  int table_width;
+  int* free_blocks;
+  int free_capacity;
+  const int* free_count;
+  int n_blocks;
+  int page_shift;
+  int base;
+  int max_tokens;
+  int* slots;
+  int* positions;
+  int* requests;
+  int* token_start;
+  int* lens_out;
+  int* free_count_out;
+  int* status;
+};
+
+inline size_t slot_smem_bytes(int n_requests) { return sizeof(int) * 3 * ((size_t)n_requests + 1); }
+
+// Last index i with sums[i] <= k, for sums ascending, sums[0] = 0 and k < sums[n].
+__device__ __forceinline__ int owner_of(const int* sums, int n, int k) {
+  int lo = 0, hi = n;   // sums[lo] <= k < sums[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (sums[mid] <= k) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ int s_sums[];
+  const int R = a.n_requests;
+  int* s_tok = s_sums;
+  int* s_grow = s_sums + (R + 1);
+  int* s_back = s_sums + 2 * (R + 1);
+  __shared__ long long s_part[kSlotThreads / 32][3];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int page = 1 << a.page_shift;
+  const long capacity = (long)a.table_width << a.page_shift;
+
+  // running sums: each thread adds a run of consecutive requests, the block
+  // scans the runs (64-bit: lengths may be garbage), the thread lays them out
+  const int per = (R + kSlotThreads - 1) / kSlotThreads;
+  const int r0 = min(R, tid * per), r1 = min(R, r0 + per);
+  long long sum[3] = {0, 0, 0};
+  int bad = 0;
+  for (int i = r0; i < r1; ++i) {
+    const long len = a.lens[i], now = len + a.delta[i];
+    if (len < 0 || len > capacity || now < 0 || now > capacity) {
+      bad = 1;
+      continue;
+    }
+    const int have = (int)((len + page - 1) >> a.page_shift), need = (int)((now + page - 1) >> a.page_shift);
+    sum[0] += max(0L, now - len);
+    sum[1] += max(0, need - have);
+    sum[2] += max(0, have - need);
+  }
+  const long count = a.free_count[0];
+  long long upto[3];
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    long long v = sum[q];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += u;
+    }
+    upto[q] = v;
+    if (lane == 31) s_part[warp][q] = v;
+  }
+  bad = __syncthreads_or(bad);
+  long long total[3] = {0, 0, 0};
+#pragma unroll
+  for (int q = 0; q < 3; ++q) {
+    long long before = 0;
+    for (int w = 0; w < kSlotThreads / 32; ++w) {
+      if (w == warp) before = total[q];
+      total[q] += s_part[w][q];
+    }
+    upto[q] += before - sum[q];
+  }
+  int code = kDevOk;
+  if (bad || count < 0 || count > a.free_capacity) code = kDevBadLength;
+  else if (total[0] > a.max_tokens) code = kDevTooManyTokens;
+  else if (total[1] > count + total[2]) code = kDevNoBlocks;
+  else if (count + total[2] - total[1] > a.free_capacity) code = kDevBadLength;
+
+  const int rank = (int)cluster.block_rank(), n_cta = (int)cluster.num_blocks();
+  const int at = rank * kSlotThreads + tid, step = n_cta * kSlotThreads;
+  if (code != kDevOk) {   // all or nothing
+    if (at == 0) atomicCAS(a.status, kDevOk, code);
+    for (int k = at; k < a.max_tokens; k += step) {
+      a.slots[k] = -1;
+      a.positions[k] = 0;
+      a.requests[k] = -1;
+    }
+    for (int i = at; i <= R; i += step) a.token_start[i] = 0;
+    if (a.lens_out != a.lens)
+      for (int i = at; i < R; i += step) a.lens_out[i] = a.lens[i];
+    if (a.free_count_out != a.free_count && at == 0) a.free_count_out[0] = (int)count;
+    return;
+  }
+
+  int t = (int)upto[0], g = (int)upto[1], b = (int)upto[2];
+  for (int i = r0; i < r1; ++i) {
+    const int len = a.lens[i], now = len + a.delta[i];
+    const int have = (len + page - 1) >> a.page_shift, need = (now + page - 1) >> a.page_shift;
+    s_tok[i] = t;
+    s_grow[i] = g;
+    s_back[i] = b;
+    t += max(0, now - len);
+    g += max(0, need - have);
+    b += max(0, have - need);
+  }
+  const int n_tok = (int)total[0], n_take = (int)total[1], n_give = (int)total[2];
+  if (tid == 0) {
+    s_tok[R] = n_tok;
+    s_grow[R] = n_take;
+    s_back[R] = n_give;
+  }
+  __syncthreads();
+
+  // the p-th block given back by this call
+  auto given = [&](int p) {
+    const int i = owner_of(s_back, R, p);
+    const int now = a.lens[i] + a.delta[i];
+    return a.table[i * a.table_stride + ((now + page - 1) >> a.page_shift) + (p - s_back[i])];
+  };
+  // the k-th new block of this call
+  auto taken = [&](int k) {
+    const long p = count + n_give - 1 - k;
+    return p < count ? a.free_blocks[p] : given((int)(p - count));
+  };
+
+  for (int k = at; k < a.max_tokens; k += step) {
+    int slot = -1, position = 0, request = -1;
+    if (k < n_tok) {
+      request = owner_of(s_tok, R, k);
+      const int len = a.lens[request];
+      const int pos = len + (k - s_tok[request]);
+      const int have = (len + page - 1) >> a.page_shift, blk = pos >> a.page_shift;
+      const int block = blk < have ? a.table[request * a.table_stride + blk]
+                                   : taken(s_grow[request] + blk - have);
+      if (block < 0 || block >= a.n_blocks) atomicCAS(a.status, kDevOk, kDevBadIndex);
+      else slot = (block << a.page_shift) + (pos & (page - 1));
+      position = a.base + pos;
+    }
+    a.slots[k] = slot;
+    a.positions[k] = position;
+    a.requests[k] = request;
+  }
+  for (int k = at; k < n_take; k += step) {
+    const int i = owner_of(s_grow, R, k);
+    const int have = (a.lens[i] + page - 1) >> a.page_shift;
+    a.table[i * a.table_stride + have + (k - s_grow[i])] = taken(k);
+  }
+  for (long p = count + at; p < count + n_give - n_take; p += step) a.free_blocks[p] = given((int)(p - count));
+  for (int i = at; i <= R; i += step) a.token_start[i] = s_tok[i];
+  cluster.sync();   // every CTA has read lens and the count
+  for (int i = at; i < R; i += step) a.lens_out[i] = a.lens[i] + a.delta[i];
+  if (at == 0) a.free_count_out[0] = (int)(count + n_give - n_take);
+}
+
+}  // namespace ls
