@@ -26,7 +26,7 @@
 // S = sum of the terms' products, and P likewise, so nothing of fp32's 24 bits
 // is lost to the 16-bit operands. With 16-bit q and output P is rounded once
 // to the cache's type, as fine as the output's own rounding. An f16 P is
-// scaled by 2^8 (and the sum with it), which keeps small weights and low
+// scaled by 2^7 (and the sum with it), which keeps small weights and low
 // terms out of the subnormals. Scores, running max, sums and outputs are fp32.
 #pragma once
 
@@ -63,7 +63,8 @@ struct PrefixAttnArgs {
   float2* part_ml;
   int prefix_parts, prefix_chunk;    // key ranges of the prefix, positions each
   int suffix_parts, suffix_chunk;
-  int prefix_tiles, suffix_tiles;    // row tiles of 16
+  int prefix_tiles, suffix_tiles;    // row tiles of 16 (prefix: of its own kernel's rows)
+  bool prefix_units;                 // the unit kernel also does the prefix
   int* status;
 };
 
@@ -111,7 +112,7 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t (&term)[TERMS]
 
 // log2 of the factor on every weight p (it cancels in o / l).
 __device__ __forceinline__ float weight_bias(__nv_bfloat16) { return 0.f; }
-__device__ __forceinline__ float weight_bias(__half) { return 8.f; }
+__device__ __forceinline__ float weight_bias(__half) { return 7.f; }
 
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
                                          __nv_bfloat16) {
@@ -204,10 +205,13 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
   const int gid = lane >> 2, tig = lane & 3;
   const int G = a.nh / a.nkv;
   const int mask = (1 << a.page_shift) - 1;
+  pdl_launch_dependents();
+  // A prefix kernel ahead of this one runs on beside it; this grid is not done
+  // before that one is, which every way out of it below waits for
 
   // the unit
   long u = blockIdx.x;
-  const long n_prefix = (long)a.prefix_parts * a.prefix_tiles * a.nkv;
+  const long n_prefix = a.prefix_units ? (long)a.prefix_parts * a.prefix_tiles * a.nkv : 0;
   const bool suffix = u >= n_prefix;
   int part, tile, g, start = 0, n = a.n_tokens, len = a.prefix_len, seen0;   // seen0: positions the first token sees
   const int* table = a.prefix_table;
@@ -225,12 +229,12 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
     u /= a.suffix_tiles;
     g = (int)(u % a.nkv);
     const int i = (int)(u / a.nkv);
-    if (!request_range(a, i, start, n, len)) return;
+    if (!request_range(a, i, start, n, len)) return pdl_wait();
     table = a.block_table + i * a.table_stride;
     seen0 = len - n + 1;
   }
   const int rows = n * G;
-  if (tile * 16 >= rows) return;
+  if (tile * 16 >= rows) return pdl_wait();
   const int seen_by_all = seen0 + (suffix ? tile * 16 / G : 0);   // positions every row of the tile sees
   const int chunk = suffix ? a.suffix_chunk : a.prefix_chunk;
   const int k0 = part * chunk, k1 = min(len, k0 + chunk);
@@ -410,6 +414,7 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
   __syncthreads();
   constexpr int TPR = kUnitThreads / 16;         // threads of a row
   const int r = threadIdx.x / TPR, c0 = (threadIdx.x % TPR) * (HD / TPR);
+  pdl_wait();
   if (tile * 16 + r >= rows) return;
   float mm = -INFINITY;
 #pragma unroll
@@ -455,6 +460,7 @@ constexpr int kJoinThreads = 128;
 template <int HD, typename Q>
 __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArgs a) {
   constexpr int TPR = HD / 4;
+  pdl_wait();
   const long row = (long)blockIdx.x * (kJoinThreads / TPR) + threadIdx.x / TPR;
   if (row >= (long)a.n_tokens * a.nh) return;
   const int c = (threadIdx.x % TPR) * 4;

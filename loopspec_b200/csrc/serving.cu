@@ -8,6 +8,7 @@
 
 #include "host.cuh"
 #include "prefix_attn.cuh"
+#include "prefix_tc.cuh"
 #include "qk_norm.cuh"
 #include "slots.cuh"
 
@@ -143,60 +144,82 @@ void run_qk_norm_rope(const ls_qk_norm_args& p, cudaStream_t stream) {
 }
 
 // ------------------------------------------------------------ prefix attention
-// How a call is cut into units: a function of its sizes alone.
+// How a call is cut into units: a function of its sizes and types alone.
 struct PrefixPlan {
+  int tc_tiles;     // 128-row tiles a CTA of the tcgen05 kernel takes; 0: the unit kernel does the prefix
   int prefix_parts, prefix_chunk, suffix_parts, suffix_chunk, prefix_tiles, suffix_tiles;
   size_t o_bytes, ml_bytes, total;
 };
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Key ranges for `len` positions of `units` row tiles: enough that the SMs
-// hold about two units each, none under 256 positions.
-void cut(long units, int len, int sms, int& parts, int& chunk) {
+// Key ranges of `len` positions for `units` row tiles: as many as keep
+// `resident` units on the GPU, none under `least` positions.
+void cut(long units, int len, long resident, int least, int grain, int& parts, int& chunk) {
   parts = chunk = 0;
   if (len == 0) return;
-  const long want = std::max(1L, (2L * sms) / std::max(1L, units));
-  const int most = std::max(1, len / 256);
+  const long want = std::max(1L, resident / std::max(1L, units));
+  const int most = std::max(1, len / least);
   parts = (int)std::min<long>(want, most);
-  chunk = cdiv(cdiv(len, parts), 64) * 64;
+  chunk = cdiv(cdiv(len, parts), grain) * grain;
   parts = cdiv(len, chunk);
 }
 
 PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int prefix_len, int max_new,
-                     int max_len, int sms) {
+                     int max_len, bool split_q, int sms) {
   PrefixPlan p{};
   const int G = nh / nkv;
-  p.prefix_tiles = cdiv((long)n_tokens * G, 16);
+  const long rows = (long)n_tokens * G;
+  p.tc_tiles = split_q || rows <= 16 || prefix_len == 0 ? 0 : rows > kTcRows ? 2 : 1;
   p.suffix_tiles = cdiv((long)std::min(max_new, n_tokens) * G, 16);
-  cut((long)p.prefix_tiles * nkv, prefix_len, sms, p.prefix_parts, p.prefix_chunk);
-  cut((long)p.suffix_tiles * nkv * n_requests, max_len, sms, p.suffix_parts, p.suffix_chunk);
-  const size_t rows = (size_t)(p.prefix_parts + p.suffix_parts) * n_tokens * nh;
-  p.o_bytes = round256(rows * hd * sizeof(float));
-  p.ml_bytes = round256(rows * sizeof(float2));
+  if (p.tc_tiles) {
+    p.prefix_tiles = cdiv(rows, kTcRows * p.tc_tiles);
+    cut((long)p.prefix_tiles * nkv, prefix_len, sms, kTcKeys, kTcKeys, p.prefix_parts, p.prefix_chunk);
+  } else {
+    p.prefix_tiles = cdiv(rows, 16);
+    cut((long)p.prefix_tiles * nkv, prefix_len, 2L * sms, 256, 64, p.prefix_parts, p.prefix_chunk);
+  }
+  cut((long)p.suffix_tiles * nkv * n_requests, max_len, 2L * sms, 256, 64, p.suffix_parts, p.suffix_chunk);
+  const size_t part_rows = (size_t)(p.prefix_parts + p.suffix_parts) * n_tokens * nh;
+  p.o_bytes = round256(part_rows * hd * sizeof(float));
+  p.ml_bytes = round256(part_rows * sizeof(float2));
   p.total = p.o_bytes + p.ml_bytes;
   return p;
 }
 
+template <int HD, typename C, int MT>
+void launch_tc(const PrefixAttnArgs& a, cudaStream_t stream) {
+  const size_t smem = TcLayout<HD, MT>::kSmem;
+  allow_smem(prefix_tc_kernel<HD, C, MT>, smem);
+  launch(prefix_tc_kernel<HD, C, MT>, dim3((unsigned)(a.prefix_tiles * a.nkv * a.prefix_parts)),
+         dim3(TcLayout<HD, MT>::kThreads), smem, stream, false, a);
+}
+
 template <int HD, typename Q, typename C, int TERMS>
-void launch_prefix(const PrefixAttnArgs& a, cudaStream_t stream) {
-  const long units = (long)a.prefix_parts * a.prefix_tiles * a.nkv +
+void launch_prefix(PrefixAttnArgs a, int tc_tiles, cudaStream_t stream) {
+  if constexpr (TERMS == 1) {
+    if (tc_tiles == 1) launch_tc<HD, C, 1>(a, stream);
+    if (tc_tiles == 2) launch_tc<HD, C, 2>(a, stream);
+  }
+  a.prefix_units = tc_tiles == 0;
+  const long units = (a.prefix_units ? (long)a.prefix_parts * a.prefix_tiles * a.nkv : 0) +
                      (long)a.suffix_parts * a.suffix_tiles * a.nkv * a.n_requests;
   REQUIRE(units <= INT32_MAX, LS_EINVAL, "prefix attention: too many units for one launch");
   if (units > 0) {
     const size_t smem = unit_smem_bytes<HD>();
     allow_smem(prefix_unit_kernel<HD, Q, C, TERMS>, smem);
-    launch(prefix_unit_kernel<HD, Q, C, TERMS>, dim3((unsigned)units), dim3(kUnitThreads), smem, stream, false, a);
+    launch(prefix_unit_kernel<HD, Q, C, TERMS>, dim3((unsigned)units), dim3(kUnitThreads), smem, stream,
+           tc_tiles != 0, a);
   }
   const int per = kJoinThreads / (HD / 4);
   launch(prefix_join_kernel<HD, Q>, dim3((unsigned)cdiv((long)a.n_tokens * a.nh, per)), dim3(kJoinThreads), 0,
-         stream, false, a);
+         stream, true, a);
 }
 
 template <typename Q, typename C, int TERMS>
-void launch_prefix(const PrefixAttnArgs& a, int hd, cudaStream_t stream) {
-  if (hd == 64) launch_prefix<64, Q, C, TERMS>(a, stream);
-  else launch_prefix<128, Q, C, TERMS>(a, stream);
+void launch_prefix(const PrefixAttnArgs& a, int hd, int tc_tiles, cudaStream_t stream) {
+  if (hd == 64) launch_prefix<64, Q, C, TERMS>(a, tc_tiles, stream);
+  else launch_prefix<128, Q, C, TERMS>(a, tc_tiles, stream);
 }
 
 void check_prefix_sizes(int n_tokens, int n_requests, int nh, int nkv, int hd, int prefix_len, int max_new,
@@ -214,8 +237,8 @@ void run_prefix_attention(const ls_prefix_attention_args& p, cudaStream_t stream
   REQUIRE((p.cache_type == LS_BF16 || p.cache_type == LS_F16) &&
               (p.q_type == LS_F32 || p.q_type == p.cache_type),
           LS_EINVAL, "prefix attention: the cache must be bf16 or f16, and q of its type or fp32");
-  REQUIRE(p.n_slots >= 1 && std::isfinite(p.scale), LS_EINVAL,
-          "prefix attention: n_slots must be positive and the scale finite");
+  REQUIRE(p.n_slots >= 1 && std::isfinite(p.scale) && p.scale > 0.f, LS_EINVAL,
+          "prefix attention: n_slots must be positive and the scale positive and finite");
   const int shift = page_shift_of(p.page_size, "prefix attention");
   const int64_t qd = (int64_t)p.n_heads * p.head_dim, kd = (int64_t)p.n_kv_heads * p.head_dim;
   REQUIRE(p.q_stride >= qd && p.out_stride >= qd && p.slot_stride >= kd &&
@@ -230,7 +253,7 @@ void run_prefix_attention(const ls_prefix_attention_args& p, cudaStream_t stream
               p.q_stride * eb % 16 == 0 && p.out_stride * eb % 16 == 0 && p.slot_stride * 2 % 16 == 0,
           LS_EINVAL, "prefix attention: pointers and row strides must be 16-byte aligned");
   const PrefixPlan plan = make_plan(p.n_tokens, p.n_requests, p.n_heads, p.n_kv_heads, p.head_dim, p.prefix_len,
-                                    p.max_new, p.max_len, sm_count());
+                                    p.max_new, p.max_len, p.q_type == LS_F32, sm_count());
   REQUIRE((reinterpret_cast<uintptr_t>(p.workspace) & 255) == 0, LS_EINVAL,
           "prefix attention: workspace must be 256-byte aligned");
   REQUIRE(p.workspace_bytes >= plan.total, LS_EINVAL,
@@ -268,10 +291,10 @@ void run_prefix_attention(const ls_prefix_attention_args& p, cudaStream_t stream
   a.prefix_tiles = plan.prefix_tiles;
   a.suffix_tiles = plan.suffix_tiles;
   a.status = p.status;
-  if (p.q_type == LS_BF16) launch_prefix<bf16, bf16, 1>(a, p.head_dim, stream);
-  else if (p.q_type == LS_F16) launch_prefix<__half, __half, 1>(a, p.head_dim, stream);
-  else if (p.cache_type == LS_BF16) launch_prefix<float, bf16, 3>(a, p.head_dim, stream);
-  else launch_prefix<float, __half, 2>(a, p.head_dim, stream);
+  if (p.q_type == LS_BF16) launch_prefix<bf16, bf16, 1>(a, p.head_dim, plan.tc_tiles, stream);
+  else if (p.q_type == LS_F16) launch_prefix<__half, __half, 1>(a, p.head_dim, plan.tc_tiles, stream);
+  else if (p.cache_type == LS_BF16) launch_prefix<float, bf16, 3>(a, p.head_dim, plan.tc_tiles, stream);
+  else launch_prefix<float, __half, 2>(a, p.head_dim, plan.tc_tiles, stream);
 }
 
 }  // namespace
@@ -326,8 +349,9 @@ size_t ls_prefix_attention_workspace_bytes(int n_tokens, int n_requests, int n_h
   size_t bytes = 0;
   guarded([&] {
     check_prefix_sizes(n_tokens, n_requests, n_heads, n_kv_heads, head_dim, prefix_len, max_new, max_len);
-    bytes = std::max<size_t>(256, make_plan(n_tokens, n_requests, n_heads, n_kv_heads, head_dim, prefix_len,
-                                            max_new, max_len, sm_count()).total);
+    for (const bool split_q : {false, true})   // enough for either type of q
+      bytes = std::max({(size_t)256, bytes, make_plan(n_tokens, n_requests, n_heads, n_kv_heads, head_dim, prefix_len,
+                                                      max_new, max_len, split_q, sm_count()).total});
   });
   return bytes;   // 0: refused, see ls_last_error(NULL)
 }
