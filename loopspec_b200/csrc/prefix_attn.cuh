@@ -272,15 +272,17 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
   unsigned char* ring = s_ring + (size_t)warp * kUnitStages * unit_stage_bytes<HD>();
   const C* kp = static_cast<const C*>(a.k_pool) + (long)g * HD;
   const C* vp = static_cast<const C*>(a.v_pool) + (long)g * HD;
+  // the block of key `key + lane`: loaded a step ahead of its copy
+  auto block_of = [&](int key) {
+    return lane < kUnitKeys && key + lane < k1 ? table[(key + lane) >> a.page_shift] : 0;
+  };
   // stage s <- keys [key, key + 16): rows past the range or with a bad block
   // are filled with zeros, so what the pool holds there never enters a product
-  auto issue = [&](int key, int s) {
+  auto issue = [&](int key, int block, int s) {
     unsigned char* dst = ring + s * unit_stage_bytes<HD>();
     int slot = -1;
     if (lane < kUnitKeys && key + lane < k1) {
-      const int pos = key + lane;
-      const int block = table[pos >> a.page_shift];
-      const long sl = ((long)block << a.page_shift) + (pos & mask);
+      const long sl = ((long)block << a.page_shift) + ((key + lane) & mask);
       if (block < 0 || sl >= a.n_slots) atomicCAS(a.status, kDevOk, kDevBadIndex);
       else slot = (int)sl;
     }
@@ -300,33 +302,42 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
   const int first = k0 + warp * kUnitKeys, step = kUnitWarps * kUnitKeys;
+  {
+    int block[kUnitStages - 1];
 #pragma unroll
-  for (int s = 0; s < kUnitStages - 1; ++s) {
-    if (first + s * step < k1) issue(first + s * step, s);
-    cp_async_commit();
+    for (int s = 0; s < kUnitStages - 1; ++s) block[s] = block_of(first + s * step);
+#pragma unroll
+    for (int s = 0; s < kUnitStages - 1; ++s) {
+      if (first + s * step < k1) issue(first + s * step, block[s], s);
+      cp_async_commit();
+    }
   }
+  int ahead = block_of(first + (kUnitStages - 1) * step);
   int s = 0;
   for (int key = first; key < k1; key += step) {
     const int next = key + (kUnitStages - 1) * step;
     int sn = s + kUnitStages - 1;
     if (sn >= kUnitStages) sn -= kUnitStages;
-    if (next < k1) issue(next, sn);
+    if (next < k1) issue(next, ahead, sn);
     cp_async_commit();
+    ahead = block_of(next + step);
     cp_async_wait<kUnitStages - 1>();
     __syncwarp();
     const unsigned char* kb = ring + s * unit_stage_bytes<HD>();
     const unsigned char* vb = kb + kUnitKeys * RB;
     float sc[2][4];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-      const unsigned char* kr = kb + (nt * 8 + gid) * RB;
+    for (int nt = 0; nt < 2; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+    // K fragments of both key octets: lane l names row l % 8 of matrix l / 8
+    const int kr = (lane & 7) + ((lane >> 4) << 3), kc = ((lane >> 3) & 1) * 8;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const uint32_t b0 = *reinterpret_cast<const uint32_t*>(kr + (ks * 16 + tig * 2) * 2);
-        const uint32_t b1 = *reinterpret_cast<const uint32_t*>(kr + (ks * 16 + 8 + tig * 2) * 2);
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t kf[4];
+      ldmatrix_x4(kf, kb + kr * RB + (ks * 16 + kc) * 2);
 #pragma unroll
-        for (int i = 0; i < TERMS; ++i) mma16816(sc[nt], qf[i][ks], b0, b1, C());
+      for (int i = 0; i < TERMS; ++i) {
+        mma16816(sc[0], qf[i][ks], kf[0], kf[1], C());
+        mma16816(sc[1], qf[i][ks], kf[2], kf[3], C());
       }
     }
     // scores in powers of two; masked ones leave by selection, whatever they hold

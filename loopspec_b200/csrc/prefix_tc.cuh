@@ -35,9 +35,9 @@ struct TcLayout {
   static constexpr int kMma = kProducer + 4;               // the issuing warp
   static constexpr int kTile = kTcKeys * HD * 2;           // bytes of a K, V or Q tile
   static constexpr int kStages = HD == 64 ? 8 : MT == 1 ? 6 : 5;
-  static constexpr int kAhead = kStages - 2;               // copies in flight; see the producer
   static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 1;
   static constexpr int kSmem = MT * kTile + kStages * kTile + 2 * kTcKeys * 4 + kBars * 8 + 16;
+  static constexpr int kPoly = 3;                          // eighths of the exponentials on the FMA units
   static constexpr uint32_t kScores = 0, kOut = 256;       // tensor memory columns
 };
 
@@ -45,28 +45,58 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// D[tmem] (+)= A[tmem] * B[smem], A packed two 16-bit values a column.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t accumulate) {
+// The issuing warp runs its loop as one: every lane computes the same operands,
+// which keeps them in uniform registers, and only the instruction itself is
+// predicated on the elected lane. (With the loop inside `if (lane == 0)` each
+// product cost ~70 cycles to issue, twice what N = 64 needs to execute.)
+// Matrix descriptors are passed by their low words; `hi` is the same for all.
+__device__ __forceinline__ void tc_mma_ss(uint32_t leader, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
+                                          uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+      "mov.b64 a, {%2, %4};\n\tmov.b64 b, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], a, b, %5, p;\n\t}" ::"r"(leader),
+      "r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
-// MN-major operand, 128-byte swizzle: 64 elements of MN a 128-byte row, 8 rows
-// of K an atom (1024 bytes apart), the next 64 of MN `mn_bytes` away.
-__device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t smem_addr, uint32_t mn_bytes) {
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr >> 4) & 0x3FFF);
-  d |= (uint64_t)((mn_bytes >> 4) & 0x3FFF) << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
+// D[tmem] (+)= A[tmem] * B[smem], A packed two 16-bit values a column.
+__device__ __forceinline__ void tc_mma_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t hi,
+                                          uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+      "mov.b64 b, {%3, %4};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], b, %5, p;\n\t}" ::"r"(leader),
+      "r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+      : "memory");
 }
+
+__device__ __forceinline__ void tc_commit_if(uint32_t leader, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %0, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(leader),
+      "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t leader;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(leader));
+  return leader;
+}
+
+// Low word of a 128-byte-swizzled operand's descriptor. K-major: rows of 128
+// bytes, 8-row groups 1024 bytes apart (`mn_bytes` unused). MN-major: 64
+// elements of MN a row, 8 rows of K a group, the next 64 of MN `mn_bytes` away.
+__device__ __forceinline__ uint32_t umma_lo(uint32_t smem_addr, uint32_t mn_bytes) {
+  return ((smem_addr >> 4) & 0x3FFF) | ((mn_bytes >> 4) << 16);
+}
+// High word: group stride 1024, descriptor version 1, 128-byte swizzle.
+constexpr uint32_t kUmmaHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 
 template <typename C>
 __host__ __device__ constexpr uint32_t tc_idesc(int M, int N, bool b_mn_major) {
@@ -105,9 +135,60 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Packed pairs of fp32 (one instruction for two).
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
+  return d;
+}
+__device__ __forceinline__ float2 unpair(uint64_t a) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^x of a pair on the FMA units, for 16-bit weights: x = n + f with n = round(x)
+// (added to 1.5 * 2^23 it sits in the low mantissa bits), |f| <= 1/2, 2^f by the
+// cubic that minimises the largest relative error there (Remez exchange: 7.5e-5,
+// a fiftieth of bf16's half unit, a seventh of f16's), n added to the exponent.
+// Below 2^-126 the result stays about 2^-127 instead of 0.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+  constexpr float kMagic = 12582912.f;
+  const float2 v = unpair(x);
+  x = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  const uint64_t t = add2(x, pair(kMagic, kMagic));
+  const uint64_t f = fma2(add2(t, pair(-kMagic, -kMagic)), pair(-1.f, -1.f), x);
+  uint64_t y = fma2(f, pair(0.055171669f, 0.055171669f), pair(0.24261112f, 0.24261112f));
+  y = fma2(y, f, pair(0.69326099f, 0.69326099f));
+  y = fma2(y, f, pair(0.99992807f, 0.99992807f));
+  const float2 n = unpair(t), r = unpair(y);
+  return pair(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(n.x) << 23)),
+              __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
+}
+
 // A whole warp's wait: all lanes agree on the outcome, so none leaves the others in a collective.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+
+// Arrive on `bar` once this thread's cp.async copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void producers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -142,7 +223,7 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
   auto live_warps = [&](int t) { return max(0, min(4, (rows - row0 - t * kTcRows + 31) / 32)); };
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      mbar_init(full0 + 8 * s, 4);
+      mbar_init(full0 + 8 * s, 128);
       mbar_init(empty0 + 8 * s, 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -211,7 +292,8 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
         }
         float mx[4] = {m, m, m, m};
 #pragma unroll
-        for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+        for (int i = 0; i < 128; i += 2)
+          mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         // m and top are raw scores; their distance counts after the scale
         const bool move = m == -INFINITY ? top != -INFINITY : (top - m) * a.scale_log2 > kTcGrow;
@@ -235,19 +317,29 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
           }
         }
         const float base = (m == -INFINITY ? 0.f : m * a.scale_log2) - weight_bias(C());
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        // Of eight pairs kPoly go to the FMA units, the others to the special
+        // function units, which do 4 of these a cycle and SM quarter
+        const uint64_t scale = pair(a.scale_log2, a.scale_log2), minus = pair(-base, -base);
+        uint64_t sum[2] = {0, 0};
         uint32_t p[64];
 #pragma unroll
         for (int i = 0; i < 64; ++i) {
-          const float x = exp2_fast(fmaf(__uint_as_float(s[2 * i]), a.scale_log2, -base));
-          const float y = exp2_fast(fmaf(__uint_as_float(s[2 * i + 1]), a.scale_log2, -base));
-          sum[i & 1] += x;
-          sum[2 + (i & 1)] += y;
-          p[i] = pack2(x, y, C());
+          const uint64_t x = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, minus);
+          uint64_t w;
+          if ((i * L::kPoly) % 8 < L::kPoly) {
+            w = exp2_poly(x);
+          } else {
+            const float2 v = unpair(x);
+            w = pair(exp2_fast(v.x), exp2_fast(v.y));
+          }
+          sum[i & 1] = add2(sum[i & 1], w);
+          const float2 v = unpair(w);
+          p[i] = pack2(v.x, v.y, C());
+          if (i == 31) tmem_st_x32(sc, p);
         }
-        tmem_st_x32(sc, p);
         tmem_st_x32(sc + 32, p + 32);
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const float2 total = unpair(add2(sum[0], sum[1]));
+        l += total.x + total.y;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -283,36 +375,26 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
     const C* kp = static_cast<const C*>(a.k_pool) + (long)g * HD + c * 8;
     const C* vp = static_cast<const C*>(a.v_pool) + (long)g * HD + c * 8;
     const int mask = (1 << a.page_shift) - 1;
-    // the slot of key `tid` of tile j, or -1: past the range, or a bad block
-    auto slot_of = [&](int j) {
+    // the block of key `tid` of tile j: loaded a tile ahead, looked at when its turn comes
+    auto block_of = [&](int j) {
       const int pos = k0 + j * kTcKeys + tid;
-      if (pos >= k1) return -1;
-      const int block = a.prefix_table[pos >> a.page_shift];
-      const long sl = ((long)block << a.page_shift) + (pos & mask);
-      if (block < 0 || sl >= a.n_slots) {
-        atomicCAS(a.status, kDevOk, kDevBadIndex);
-        return -1;
-      }
-      return (int)sl;
+      return pos < k1 ? a.prefix_table[pos >> a.page_shift] : 0;
     };
-    int next = slot_of(0);
+    int next = block_of(0);
     bool ok = true;
-    // copy i (2 j: K, 2 j + 1: V) goes to stage i % ST; it is announced once
-    // kAhead newer ones are issued. A stage comes free when copies up to the
-    // one after it have been used (V of a tile and K of the next are used in
-    // turn), so kAhead = ST - 2 never waits for an unannounced copy.
-    auto announce = [&](int i) {
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(full0 + 8 * (i % ST));
-    };
+    // copy i (2 j: K, 2 j + 1: V) goes to stage i % ST; the barrier counts each
+    // thread's part in when it has landed, so the producers run a ring ahead
     int issued = 0;
     // after a wait that timed out the warp copies no more but stays in the barriers
     for (int j = 0; j < n; ++j) {
       int* slots = s_slot + (j & 1) * kTcKeys;
-      slots[tid] = next;
+      const int pos = k0 + j * kTcKeys + tid;
+      const long sl = ((long)next << a.page_shift) + (pos & mask);
+      const bool fits = next >= 0 && sl < a.n_slots;
+      if (!fits && pos < k1) atomicCAS(a.status, kDevOk, kDevBadIndex);
+      slots[tid] = fits && pos < k1 ? (int)sl : -1;   // -1: filled with zeros
+      if (j + 1 < n) next = block_of(j + 1);
       producers_sync();
-      if (j + 1 < n) next = slot_of(j + 1);
 #pragma unroll 1
       for (int kv = 0; kv < 2 && ok; ++kv) {
         const int st = issued % ST;
@@ -323,52 +405,51 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
 #pragma unroll
         for (int i = 0; i < kTcKeys / RPI; ++i) {
           const int r = r0 + i * RPI;
-          const int sl = slots[r];
-          cp_async16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (long)max(sl, 0) * a.slot_stride, sl >= 0);
+          const int slot = slots[r];
+          cp_async16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (long)max(slot, 0) * a.slot_stride, slot >= 0);
         }
-        cp_async_commit();
-        if (issued >= L::kAhead) {
-          cp_async_wait<L::kAhead>();
-          announce(issued - L::kAhead);
-        }
+        cp_async_arrive(full0 + 8 * st);
         ++issued;
       }
     }
+    cp_async_commit();
     cp_async_wait<0>();
-    for (int i = max(0, issued - L::kAhead); i < issued; ++i) announce(i);
   } else {
     // ------------------------------------------------------------------- issue
     if (MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == L::kMma && lane == 0) {
+    if (warp == L::kMma) {
       constexpr uint32_t idesc_s = tc_idesc<C>(kTcRows, kTcKeys, false);
       constexpr uint32_t idesc_o = tc_idesc<C>(kTcRows, HD, true);
-      const uint32_t ring = smem_u32(s_ring), q0 = smem_u32(s_q);
+      const uint32_t leader = elect_one();
+      const uint32_t ring_k = umma_lo(smem_u32(s_ring), 0), ring_v = umma_lo(smem_u32(s_ring), kBlock),
+                     q0 = umma_lo(smem_u32(s_q), 0);
       auto wait_full = [&](int i) {
-        const bool ok = mbar_wait(full0 + 8 * (i % ST), (i / ST) & 1, a.status, kDevTimeoutFull);
+        const bool ok = warp_wait(full0 + 8 * (i % ST), (i / ST) & 1, a.status, kDevTimeoutFull);
+        fence_proxy_async();                       // copies came by the generic proxy; the products read by the async one
         tc_fence_after();
         return ok;
       };
       auto release = [&](int i) {                  // copy i's stage, if another copy will want it
-        if (i + ST < 2 * n) tc_commit(empty0 + 8 * (i % ST));
+        if (i + ST < 2 * n) tc_commit_if(leader, empty0 + 8 * (i % ST));
       };
       auto scores = [&](int t, int b, int j) {     // S[b] = Q[t] K[j]^T
-        const uint32_t k = ring + (2 * j % ST) * L::kTile, q = q0 + t * L::kTile;
+        const uint32_t k = ring_k + ((2 * j % ST) * L::kTile >> 4), q = q0 + (t * L::kTile >> 4);
 #pragma unroll
         for (int i = 0; i < HD / 16; ++i) {
-          const uint32_t off = (i >> 2) * kBlock + (i & 3) * 32;
-          tc_mma_bf16(tmem + L::kScores + b * 128, umma_desc_sw128(q + off), umma_desc_sw128(k + off), idesc_s, i != 0);
+          const uint32_t off = ((i >> 2) * kBlock + (i & 3) * 32) >> 4;
+          tc_mma_ss(leader, tmem + L::kScores + b * 128, q + off, k + off, kUmmaHi, idesc_s, i != 0);
         }
-        tc_commit(s_full + 8 * b);
+        tc_commit_if(leader, s_full + 8 * b);
       };
       auto outputs = [&](int t, int b, int j) {    // O[t] += P[b] V[j]
-        const uint32_t v = ring + ((2 * j + 1) % ST) * L::kTile;
+        const uint32_t v = ring_v + (((2 * j + 1) % ST) * L::kTile >> 4);
 #pragma unroll
         for (int i = 0; i < kTcKeys / 16; ++i)
-          tc_mma_ts(tmem + L::kOut + t * 128, tmem + L::kScores + b * 128 + i * 8,
-                    umma_desc_sw128_mn(v + i * 2048, kBlock), idesc_o, (j | i) != 0);
-        tc_commit(pv_done + 8 * t);
+          tc_mma_ts(leader, tmem + L::kOut + t * 128, tmem + L::kScores + b * 128 + i * 8, v + (i * 2048 >> 4), kUmmaHi,
+                    idesc_o, i != 0 ? 1u : (uint32_t)(j != 0));
+        tc_commit_if(leader, pv_done + 8 * t);
       };
-      bool ok = mbar_wait(q_full, 0, a.status, kDevTimeoutFull) && wait_full(0);
+      bool ok = warp_wait(q_full, 0, a.status, kDevTimeoutFull) && wait_full(0);
       if (ok) {
         for (int t = 0; t < tiles_here; ++t) scores(t, t, 0);
         release(0);
@@ -382,14 +463,15 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
             scores(0, (j + 1) & 1, j + 1);
             release(2 * j + 2);
           }
-          if (!(ok = wait_full(2 * j + 1) && mbar_wait(p_full + 8 * (j & 1), (j >> 1) & 1, a.status, kDevTimeoutAcc))) break;
+          ok = wait_full(2 * j + 1) && warp_wait(p_full + 8 * (j & 1), (j >> 1) & 1, a.status, kDevTimeoutAcc);
+          if (!ok) break;
           tc_fence_after();
           outputs(0, j & 1, j);
           release(2 * j + 1);
         } else {
           if (!(ok = wait_full(2 * j + 1))) break;
           for (int t = 0; t < tiles_here; ++t) {
-            if (!(ok = mbar_wait(p_full + 8 * t, j & 1, a.status, kDevTimeoutAcc))) break;
+            if (!(ok = warp_wait(p_full + 8 * t, j & 1, a.status, kDevTimeoutAcc))) break;
             tc_fence_after();
             outputs(t, t, j);
             if (t + 1 == tiles_here) release(2 * j + 1);
@@ -402,7 +484,6 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
         }
       }
     }
-    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();

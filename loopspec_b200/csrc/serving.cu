@@ -179,7 +179,7 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
     p.prefix_tiles = cdiv(rows, 16);
     cut((long)p.prefix_tiles * nkv, prefix_len, 2L * sms, 256, 64, p.prefix_parts, p.prefix_chunk);
   }
-  cut((long)p.suffix_tiles * nkv * n_requests, max_len, 2L * sms, 256, 64, p.suffix_parts, p.suffix_chunk);
+  cut((long)p.suffix_tiles * nkv * n_requests, max_len, 8L * sms, 256, 64, p.suffix_parts, p.suffix_chunk);
   const size_t part_rows = (size_t)(p.prefix_parts + p.suffix_parts) * n_tokens * nh;
   p.o_bytes = round256(part_rows * hd * sizeof(float));
   p.ml_bytes = round256(part_rows * sizeof(float2));
