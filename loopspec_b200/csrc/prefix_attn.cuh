@@ -70,19 +70,29 @@ struct PrefixAttnArgs {
 
 constexpr int kUnitThreads = 128;
 constexpr int kUnitKeys = 16;      // keys of a warp's stage
-constexpr int kUnitStages = 3;
 constexpr int kUnitWarps = kUnitThreads / 32;
+// Stages of a warp's ring and CTAs an SM: 16-bit queries of 128 take 166
+// registers a thread, so a third CTA fits beside two when the rings shrink to
+// two stages (one copy in flight a warp, 12 warps); fp32 queries hold two or
+// three terms of q and leave room for two CTAs with three stages.
+template <int HD, int TERMS>
+__host__ __device__ constexpr int unit_stages() { return HD == 128 && TERMS == 1 ? 2 : 3; }
+template <int HD, int TERMS>
+__host__ __device__ constexpr int unit_ctas() { return HD == 128 ? (TERMS == 1 ? 3 : 2) : TERMS == 3 ? 3 : 4; }
 
 template <int HD>
 __host__ __device__ constexpr int unit_row_bytes() { return HD * 2 + 16; }   // padded: fragment reads hit distinct banks
 template <int HD>
 __host__ __device__ constexpr int unit_stage_bytes() { return 2 * kUnitKeys * unit_row_bytes<HD>(); }
-template <int HD>
-constexpr size_t unit_smem_bytes() { return (size_t)kUnitWarps * kUnitStages * unit_stage_bytes<HD>(); }
+template <int HD, int TERMS>
+constexpr size_t unit_smem_bytes() { return (size_t)kUnitWarps * unit_stages<HD, TERMS>() * unit_stage_bytes<HD>(); }
 
-// Joining the warps reuses the rings: kUnitWarps x 16 rows of HD floats.
-static_assert(unit_smem_bytes<64>() >= sizeof(float) * kUnitWarps * 16 * 64, "join buffer");
-static_assert(unit_smem_bytes<128>() >= sizeof(float) * kUnitWarps * 16 * 128, "join buffer");
+// Joining the warps reuses the rings: kUnitWarps x 16 rows of HD floats, padded
+// so that the 8 rows a warp stores at once lie in different banks.
+template <int HD>
+__host__ __device__ constexpr int unit_join_row() { return HD + 8; }
+static_assert(unit_smem_bytes<64, 1>() >= sizeof(float) * kUnitWarps * 16 * unit_join_row<64>(), "join buffer");
+static_assert(unit_smem_bytes<128, 1>() >= sizeof(float) * kUnitWarps * 16 * unit_join_row<128>(), "join buffer");
 
 // Two fp32 values as a packed pair of the cache's type, lower index in the low half.
 __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) { return pack_bf16(a, b); }
@@ -193,7 +203,8 @@ __device__ __forceinline__ void add_by_weight(float (&o)[HD / 8][4], const float
 // grid: 1-D over prefix units (part, row tile, kv head), then suffix units
 // (part, row tile, kv head, request).
 template <int HD, typename Q, typename C, int TERMS>
-__global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArgs a) {
+__global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS>()) prefix_unit_kernel(PrefixAttnArgs a) {
+  constexpr int ST = unit_stages<HD, TERMS>();
   constexpr int RB = unit_row_bytes<HD>();
   constexpr int KS = HD / 16;
   constexpr int NT = HD / 8;
@@ -210,35 +221,72 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
   // before that one is, which every way out of it below waits for
 
   // the unit
-  long u = blockIdx.x;
-  const long n_prefix = a.prefix_units ? (long)a.prefix_parts * a.prefix_tiles * a.nkv : 0;
+  unsigned u = blockIdx.x;
+  const unsigned n_prefix = a.prefix_units ? (unsigned)(a.prefix_parts * a.prefix_tiles * a.nkv) : 0;
   const bool suffix = u >= n_prefix;
-  int part, tile, g, start = 0, n = a.n_tokens, len = a.prefix_len, seen0;   // seen0: positions the first token sees
-  const int* table = a.prefix_table;
-  if (!suffix) {
-    part = (int)(u % a.prefix_parts);
-    u /= a.prefix_parts;
-    tile = (int)(u % a.prefix_tiles);
-    g = (int)(u / a.prefix_tiles);
-    seen0 = len;
-  } else {
-    u -= n_prefix;
-    part = (int)(u % a.suffix_parts);
-    u /= a.suffix_parts;
-    tile = (int)(u % a.suffix_tiles);
-    u /= a.suffix_tiles;
-    g = (int)(u % a.nkv);
-    const int i = (int)(u / a.nkv);
-    if (!request_range(a, i, start, n, len)) return pdl_wait();
-    table = a.block_table + i * a.table_stride;
-    seen0 = len - n + 1;
-  }
+  if (suffix) u -= n_prefix;
+  const unsigned parts = suffix ? a.suffix_parts : a.prefix_parts, tiles = suffix ? a.suffix_tiles : a.prefix_tiles;
+  const int part = (int)(u % parts);
+  u /= parts;
+  const int tile = (int)(u % tiles);
+  u /= tiles;
+  const int g = (int)(u % (unsigned)a.nkv), req = (int)(u / (unsigned)a.nkv);   // req 0 for the prefix
+  const int* table = suffix ? a.block_table + req * a.table_stride : a.prefix_table;
+  const int bound = suffix ? a.max_len : a.prefix_len;                          // positions the table covers
+  const int chunk = suffix ? a.suffix_chunk : a.prefix_chunk;
+  const int k0 = part * chunk;
+  const int first = k0 + warp * kUnitKeys, step = kUnitWarps * kUnitKeys;
+  // the block of key `key + lane`: loaded a step ahead of its copy, the first
+  // ones beside the request's length
+  auto block_of = [&](int key) {
+    return lane < kUnitKeys && key + lane < bound ? table[(key + lane) >> a.page_shift] : 0;
+  };
+  int block[ST - 1];
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s) block[s] = block_of(first + s * step);
+  int ahead = block_of(first + (ST - 1) * step);
+  int start = 0, n = a.n_tokens, len = a.prefix_len;
+  if (suffix && !request_range(a, req, start, n, len)) return pdl_wait();
   const int rows = n * G;
   if (tile * 16 >= rows) return pdl_wait();
-  const int seen_by_all = seen0 + (suffix ? tile * 16 / G : 0);   // positions every row of the tile sees
-  const int chunk = suffix ? a.suffix_chunk : a.prefix_chunk;
-  const int k0 = part * chunk, k1 = min(len, k0 + chunk);
+  const int seen0 = suffix ? len - n + 1 : len;                   // positions the first token sees
+  const int seen_by_all = seen0 + (suffix ? tile * 16 / G : 0);   // ... every row of the tile
+  const int k1 = min(len, k0 + chunk);
   const int slot_part = suffix ? a.prefix_parts + part : part;
+
+  unsigned char* ring = s_ring + (size_t)warp * ST * unit_stage_bytes<HD>();
+  const C* kp = static_cast<const C*>(a.k_pool) + (long)g * HD;
+  const C* vp = static_cast<const C*>(a.v_pool) + (long)g * HD;
+  // stage s <- keys [key, key + 16): rows past the range or with a bad block
+  // are filled with zeros, so what the pool holds there never enters a product
+  auto issue = [&](int key, int block, int s) {
+    unsigned char* dst = ring + s * unit_stage_bytes<HD>();
+    int slot = -1;
+    if (lane < kUnitKeys && key + lane < k1) {
+      const long sl = ((long)block << a.page_shift) + ((key + lane) & mask);
+      if (block < 0 || sl >= a.n_slots) atomicCAS(a.status, kDevOk, kDevBadIndex);
+      else slot = (int)sl;
+    }
+#pragma unroll
+    for (int i = 0; i < kUnitKeys / LR; ++i) {
+      const int r = i * LR + lane / CH, c = lane % CH;
+      const int sl = __shfl_sync(0xffffffffu, slot, r);
+      const long off = (long)max(sl, 0) * a.slot_stride + c * 8;
+      cp_async16(dst + r * RB + c * 16, kp + off, sl >= 0);
+      cp_async16(dst + (kUnitKeys + r) * RB + c * 16, vp + off, sl >= 0);
+    }
+  };
+
+  float o[NT][4];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s) {
+    if (first + s * step < k1) issue(first + s * step, block[s], s);
+    cp_async_commit();
+  }
 
   // this thread's two rows: token, head, and the number of positions it sees
   long row_at[2];                                // t * nh + h, or -1
@@ -269,65 +317,26 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
     }
   }
 
-  unsigned char* ring = s_ring + (size_t)warp * kUnitStages * unit_stage_bytes<HD>();
-  const C* kp = static_cast<const C*>(a.k_pool) + (long)g * HD;
-  const C* vp = static_cast<const C*>(a.v_pool) + (long)g * HD;
-  // the block of key `key + lane`: loaded a step ahead of its copy
-  auto block_of = [&](int key) {
-    return lane < kUnitKeys && key + lane < k1 ? table[(key + lane) >> a.page_shift] : 0;
-  };
-  // stage s <- keys [key, key + 16): rows past the range or with a bad block
-  // are filled with zeros, so what the pool holds there never enters a product
-  auto issue = [&](int key, int block, int s) {
-    unsigned char* dst = ring + s * unit_stage_bytes<HD>();
-    int slot = -1;
-    if (lane < kUnitKeys && key + lane < k1) {
-      const long sl = ((long)block << a.page_shift) + ((key + lane) & mask);
-      if (block < 0 || sl >= a.n_slots) atomicCAS(a.status, kDevOk, kDevBadIndex);
-      else slot = (int)sl;
-    }
-#pragma unroll
-    for (int i = 0; i < kUnitKeys / LR; ++i) {
-      const int r = i * LR + lane / CH, c = lane % CH;
-      const int sl = __shfl_sync(0xffffffffu, slot, r);
-      const long off = (long)max(sl, 0) * a.slot_stride + c * 8;
-      cp_async16(dst + r * RB + c * 16, kp + off, sl >= 0);
-      cp_async16(dst + (kUnitKeys + r) * RB + c * 16, vp + off, sl >= 0);
-    }
-  };
-
-  float o[NT][4];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-  const int first = k0 + warp * kUnitKeys, step = kUnitWarps * kUnitKeys;
-  {
-    int block[kUnitStages - 1];
-#pragma unroll
-    for (int s = 0; s < kUnitStages - 1; ++s) block[s] = block_of(first + s * step);
-#pragma unroll
-    for (int s = 0; s < kUnitStages - 1; ++s) {
-      if (first + s * step < k1) issue(first + s * step, block[s], s);
-      cp_async_commit();
-    }
-  }
-  int ahead = block_of(first + (kUnitStages - 1) * step);
   int s = 0;
   for (int key = first; key < k1; key += step) {
-    const int next = key + (kUnitStages - 1) * step;
-    int sn = s + kUnitStages - 1;
-    if (sn >= kUnitStages) sn -= kUnitStages;
+    const int next = key + (ST - 1) * step;
+    int sn = s + ST - 1;
+    if (sn >= ST) sn -= ST;
     if (next < k1) issue(next, ahead, sn);
     cp_async_commit();
     ahead = block_of(next + step);
-    cp_async_wait<kUnitStages - 1>();
+    cp_async_wait<ST - 1>();
     __syncwarp();
     const unsigned char* kb = ring + s * unit_stage_bytes<HD>();
     const unsigned char* vb = kb + kUnitKeys * RB;
-    float sc[2][4];
+    // chains of products that wait for one another cost ~20 cycles a link:
+    // each term (or half of the head) has accumulators of its own
+    constexpr int CHAINS = TERMS == 1 ? 2 : TERMS;
+    float acc[CHAINS][2][4];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+    for (int i = 0; i < CHAINS; ++i)
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) acc[i][nt][0] = acc[i][nt][1] = acc[i][nt][2] = acc[i][nt][3] = 0.f;
     // K fragments of both key octets: lane l names row l % 8 of matrix l / 8
     const int kr = (lane & 7) + ((lane >> 4) << 3), kc = ((lane >> 3) & 1) * 8;
 #pragma unroll
@@ -336,10 +345,20 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
       ldmatrix_x4(kf, kb + kr * RB + (ks * 16 + kc) * 2);
 #pragma unroll
       for (int i = 0; i < TERMS; ++i) {
-        mma16816(sc[0], qf[i][ks], kf[0], kf[1], C());
-        mma16816(sc[1], qf[i][ks], kf[2], kf[3], C());
+        const int ch = TERMS == 1 ? ks & 1 : i;
+        mma16816(acc[ch][0], qf[i][ks], kf[0], kf[1], C());
+        mma16816(acc[ch][1], qf[i][ks], kf[2], kf[3], C());
       }
     }
+    float sc[2][4];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[nt][e] = acc[CHAINS - 1][nt][e];        // smallest terms first
+#pragma unroll
+        for (int i = CHAINS - 2; i >= 0; --i) sc[nt][e] += acc[i][nt][e];
+      }
     // scores in powers of two; masked ones leave by selection, whatever they hold
     float mx[2] = {m[0], m[1]};
 #pragma unroll
@@ -400,7 +419,7 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
     }
     }
     __syncwarp();   // the stage is refilled by the next turn's copy
-    if (++s == kUnitStages) s = 0;
+    if (++s == ST) s = 0;
   }
   cp_async_wait<0>();
 
@@ -420,7 +439,7 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
   for (int i = 0; i < NT; ++i)
 #pragma unroll
     for (int e = 0; e < 2; ++e)
-      *reinterpret_cast<float2*>(s_o + ((warp * 16 + gid + 8 * e) * HD + i * 8 + tig * 2)) =
+      *reinterpret_cast<float2*>(s_o + ((warp * 16 + gid + 8 * e) * unit_join_row<HD>() + i * 8 + tig * 2)) =
           make_float2(o[i][2 * e], o[i][2 * e + 1]);
   __syncthreads();
   constexpr int TPR = kUnitThreads / 16;         // threads of a row
@@ -445,7 +464,7 @@ __global__ void __launch_bounds__(kUnitThreads) prefix_unit_kernel(PrefixAttnArg
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kUnitWarps; ++w) {
-      const float4 v = *reinterpret_cast<const float4*>(s_o + (w * 16 + r) * HD + c0 + c);
+      const float4 v = *reinterpret_cast<const float4*>(s_o + (w * 16 + r) * unit_join_row<HD>() + c0 + c);
       acc.x += v.x * wt[w];
       acc.y += v.y * wt[w];
       acc.z += v.z * wt[w];

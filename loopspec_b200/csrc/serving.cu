@@ -206,7 +206,7 @@ void launch_prefix(PrefixAttnArgs a, int tc_tiles, cudaStream_t stream) {
                      (long)a.suffix_parts * a.suffix_tiles * a.nkv * a.n_requests;
   REQUIRE(units <= INT32_MAX, LS_EINVAL, "prefix attention: too many units for one launch");
   if (units > 0) {
-    const size_t smem = unit_smem_bytes<HD>();
+    const size_t smem = unit_smem_bytes<HD, TERMS>();
     allow_smem(prefix_unit_kernel<HD, Q, C, TERMS>, smem);
     launch(prefix_unit_kernel<HD, Q, C, TERMS>, dim3((unsigned)units), dim3(kUnitThreads), smem, stream,
            tc_tiles != 0, a);
