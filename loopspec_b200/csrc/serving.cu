@@ -3,6 +3,7 @@
 // picks the kernel variant and enqueues; none waits or allocates.
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -17,10 +18,23 @@ typedef __nv_bfloat16 bf16;
 
 namespace {
 
-int sm_count() {
-  int dev = 0, sms = 0;
+int current_device() {
+  int dev = 0;
   CK(cudaGetDevice(&dev));
-  CK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  return dev;
+}
+
+// Facts of a device and grants to a kernel on it are looked up once a process.
+constexpr int kMaxDevices = 64;
+
+int sm_count() {
+  static std::atomic<int> known[kMaxDevices];
+  const int dev = current_device();
+  int sms = dev < kMaxDevices ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (sms == 0) {
+    CK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    if (dev < kMaxDevices) known[dev].store(sms, std::memory_order_relaxed);
+  }
   return sms;
 }
 
@@ -37,11 +51,14 @@ int page_shift_of(int page_size, const char* who) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 long type_bytes(int type) { return type == LS_F32 ? 4 : 2; }
 
-// Dynamic shared memory above the default limit is granted once a kernel and device.
-template <typename K>
-void allow_smem(K kernel, size_t bytes) {
-  if (bytes > 48 * 1024)
-    CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+// Let `kernel` have up to `most` bytes of dynamic shared memory on this device.
+template <auto kernel>
+void allow_smem(size_t most) {
+  static std::atomic<bool> granted[kMaxDevices];
+  const int dev = current_device();
+  if (dev < kMaxDevices && granted[dev].load(std::memory_order_relaxed)) return;
+  CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+  if (dev < kMaxDevices) granted[dev].store(true, std::memory_order_relaxed);
 }
 
 template <typename F>
@@ -78,7 +95,7 @@ void run_build_slots(const ls_slots_args& p, cudaStream_t stream) {
              p.free_blocks, p.free_capacity, p.free_count, p.n_blocks, shift, p.base, p.max_tokens,
              p.slots, p.positions, p.requests, p.token_start, p.lens_out, p.free_count_out, p.status};
   const size_t smem = slot_smem_bytes(p.n_requests);
-  allow_smem(build_slots_kernel, smem);
+  if (smem > 48 * 1024) allow_smem<build_slots_kernel>(slot_smem_bytes(kSlotMaxRequests));
   // one CTA while every thread has at most 4 tokens; more CTAs share the
   // stores of a prompt batch but each repeats the sums
   int ctas = 1;
@@ -190,7 +207,7 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
 template <int HD, typename C, int MT>
 void launch_tc(const PrefixAttnArgs& a, cudaStream_t stream) {
   const size_t smem = TcLayout<HD, MT>::kSmem;
-  allow_smem(prefix_tc_kernel<HD, C, MT>, smem);
+  allow_smem<prefix_tc_kernel<HD, C, MT>>(smem);
   launch(prefix_tc_kernel<HD, C, MT>, dim3((unsigned)(a.prefix_tiles * a.nkv * a.prefix_parts)),
          dim3(TcLayout<HD, MT>::kThreads), smem, stream, false, a);
 }
@@ -207,7 +224,7 @@ void launch_prefix(PrefixAttnArgs a, int tc_tiles, cudaStream_t stream) {
   REQUIRE(units <= INT32_MAX, LS_EINVAL, "prefix attention: too many units for one launch");
   if (units > 0) {
     const size_t smem = unit_smem_bytes<HD, TERMS>();
-    allow_smem(prefix_unit_kernel<HD, Q, C, TERMS>, smem);
+    allow_smem<prefix_unit_kernel<HD, Q, C, TERMS>>(smem);
     launch(prefix_unit_kernel<HD, Q, C, TERMS>, dim3((unsigned)units), dim3(kUnitThreads), smem, stream,
            tc_tiles != 0, a);
   }

@@ -9,11 +9,14 @@ them. With page_size 1 a block table is a timeline's row of slots, as in
 
 from __future__ import annotations
 
+import torch
+
 from . import _lib
-from .qk_norm import check_pools, type_code
-from .status import enqueue, require
+from .qk_norm import TYPE_CODES, check_pools
+from .status import enqueue, on_stream
 
 _pack = _lib.packer(_lib.PrefixAttentionArgs)
+_i32 = torch.int32
 
 
 def workspace_bytes(n_tokens, n_heads, n_kv_heads, head_dim, *, n_requests, prefix_len, max_new, max_len):
@@ -39,46 +42,45 @@ def prefix_attention(q, k_pool, v_pool, prefix_table, prefix_len, block_table, l
     workspace    uint8 CUDA tensor of workspace_bytes(...) bytes, kept by the caller or made here;
                  calls that share one must be on one stream
     """
-    import torch
     n_slots, n_kv, hd, slot_stride = check_pools(k_pool, v_pool, "prefix attention")
-    n, nh, width = q.shape
-    row = q.stride()
-    require(width == hd and q.is_cuda and row[2] == 1 and row[1] == hd,
-            "prefix attention: q must be a CUDA tensor [T, n_heads, head_dim] with contiguous rows")
-    i32 = torch.int32
+    shape, row, dtype = q.shape, q.stride(), q.dtype
+    n, nh, width = shape
+    if not (width == hd and q.is_cuda and row[2] == 1 and row[1] == hd and dtype in TYPE_CODES):
+        raise ValueError("prefix attention: q must be a CUDA tensor [T, n_heads, head_dim] with contiguous rows")
     n_req, blocks = block_table.shape
-    require(block_table.dtype is i32 and block_table.is_cuda and (blocks <= 1 or block_table.stride(1) == 1),
-            "prefix attention: block_table must be an int32 CUDA tensor with contiguous rows")
-    require(lens.dtype is i32 and token_start.dtype is i32 and lens.is_cuda and token_start.is_cuda
+    columns = block_table.stride()
+    if not (block_table.dtype is _i32 and block_table.is_cuda and (blocks <= 1 or columns[1] == 1)):
+        raise ValueError("prefix attention: block_table must be an int32 CUDA tensor with contiguous rows")
+    if not (lens.dtype is _i32 and token_start.dtype is _i32 and lens.is_cuda and token_start.is_cuda
             and lens.is_contiguous() and token_start.is_contiguous() and lens.numel() == n_req
-            and token_start.numel() == n_req + 1,
-            "prefix attention: lens [n_requests] and token_start [n_requests + 1] must be int32 contiguous CUDA tensors")
+            and token_start.numel() == n_req + 1):
+        raise ValueError("prefix attention: lens [n_requests] and token_start [n_requests + 1] must be int32 "
+                         "contiguous CUDA tensors")
     if max_len is None:
         max_len = blocks * page_size
-    require(page_size >= 1 and max_len <= blocks * page_size, "prefix attention: max_len exceeds the block table")
-    if prefix_len:
-        require(prefix_table is not None and prefix_table.dtype is i32 and prefix_table.is_cuda
-                and prefix_table.is_contiguous() and prefix_table.numel() * page_size >= prefix_len > 0,
-                "prefix attention: prefix_table must be an int32 contiguous CUDA tensor that covers prefix_len")
+    if not (page_size >= 1 and max_len <= blocks * page_size):
+        raise ValueError("prefix attention: max_len exceeds the block table")
+    if prefix_len and not (prefix_table is not None and prefix_table.dtype is _i32 and prefix_table.is_cuda
+                           and prefix_table.is_contiguous() and prefix_table.numel() * page_size >= prefix_len > 0):
+        raise ValueError("prefix attention: prefix_table must be an int32 contiguous CUDA tensor that covers prefix_len")
     if scale is None:
         scale = hd ** -0.5
     if out is None or workspace is None:
-        with torch.cuda.stream(torch.cuda.current_stream(q.device) if stream is None
-                               else torch.cuda.ExternalStream(stream, q.device)):
+        with on_stream(q.device, stream):
             if out is None:
-                out = torch.empty(n, nh, hd, dtype=q.dtype, device=q.device)
+                out = torch.empty(n, nh, hd, dtype=dtype, device=q.device)
             if workspace is None:
                 need = workspace_bytes(n, nh, n_kv, hd, n_requests=n_req, prefix_len=prefix_len, max_new=max_new,
                                        max_len=max_len)
                 workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     to = out.stride()
-    require(out.shape == q.shape and out.dtype is q.dtype and out.is_cuda and to[2] == 1 and to[1] == hd,
-            "prefix attention: out must be a CUDA tensor of q's shape and type with contiguous rows")
+    if not (out.shape == shape and out.dtype is dtype and out.is_cuda and to[2] == 1 and to[1] == hd):
+        raise ValueError("prefix attention: out must be a CUDA tensor of q's shape and type with contiguous rows")
     before = (q.data_ptr(), row[0] if n > 1 else nh * hd, k_pool.data_ptr(), v_pool.data_ptr(), slot_stride,
               prefix_table.data_ptr() if prefix_len else 0, block_table.data_ptr(),
-              block_table.stride(0) if n_req > 1 else blocks, lens.data_ptr(), token_start.data_ptr(),
+              columns[0] if n_req > 1 else blocks, lens.data_ptr(), token_start.data_ptr(),
               out.data_ptr(), to[0] if n > 1 else nh * hd, workspace.data_ptr(), workspace.numel())
-    after = (type_code(q.dtype, "prefix attention"), type_code(k_pool.dtype, "prefix attention"), n, n_req, nh, n_kv,
-             hd, prefix_len, max_new, max_len, page_size, n_slots, scale)
+    after = (TYPE_CODES[dtype], TYPE_CODES[k_pool.dtype], n, n_req, nh, n_kv, hd, prefix_len, max_new, max_len,
+             page_size, n_slots, scale)
     enqueue(_lib.lib().ls_prefix_attention, _pack, before, after, q.device, status, stream)
     return out

@@ -10,10 +10,13 @@ the host never learns a length.
 
 from __future__ import annotations
 
+import torch
+
 from . import _lib
-from .status import enqueue, require
+from .status import enqueue
 
 _pack = _lib.packer(_lib.SlotsArgs)
+_i32 = torch.int32
 
 
 class SlotMap:
@@ -26,7 +29,6 @@ class SlotMap:
     """
 
     def __init__(self, n_requests, max_tokens, device="cuda", lens=None, free_count=None):
-        import torch
         n, t = n_requests, max_tokens
         whole = torch.empty(3 * t + 2 * n + 2, dtype=torch.int32, device=device)
         self.slots, self.positions, self.requests = whole[:t], whole[t:2 * t], whole[2 * t:3 * t]
@@ -46,17 +48,17 @@ def build_slots(lens, delta, block_table, free_blocks, free_count, *, page_size,
     All or nothing: on a bad length, too few free blocks or more new tokens
     than out.slots holds, nothing changes and the status says why.
     """
-    import torch
-    i32 = torch.int32
     for t in (lens, delta, free_blocks, free_count, out.lens, out.free_count):
-        require(t.dtype is i32 and t.is_cuda and t.is_contiguous(), "slot maps: int32 contiguous CUDA tensors expected")
+        if not (t.dtype is _i32 and t.is_cuda and t.is_contiguous()):
+            raise ValueError("slot maps: int32 contiguous CUDA tensors expected")
     n, width = block_table.shape
-    require(block_table.dtype is i32 and block_table.is_cuda and block_table.stride(1) == 1,
-            "slot maps: block_table must be an int32 CUDA tensor with contiguous rows")
-    require(lens.numel() == n and delta.numel() == n and out.lens.numel() == n and out.token_start.numel() == n + 1
-            and free_count.numel() == 1 and out.free_count.numel() == 1,
-            "slot maps: lens, delta, block_table and out must describe the same requests")
-    before = (lens.data_ptr(), delta.data_ptr(), block_table.data_ptr(), block_table.stride(0) if n > 1 else width,
+    row = block_table.stride()
+    if not (block_table.dtype is _i32 and block_table.is_cuda and row[1] == 1):
+        raise ValueError("slot maps: block_table must be an int32 CUDA tensor with contiguous rows")
+    if not (lens.numel() == n == delta.numel() == out.lens.numel() and out.token_start.numel() == n + 1
+            and free_count.numel() == 1 == out.free_count.numel()):
+        raise ValueError("slot maps: lens, delta, block_table and out must describe the same requests")
+    before = (lens.data_ptr(), delta.data_ptr(), block_table.data_ptr(), row[0] if n > 1 else width,
               free_blocks.data_ptr(), free_count.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(),
               out.requests.data_ptr(), out.token_start.data_ptr(), out.lens.data_ptr(), out.free_count.data_ptr())
     after = (n, width, free_blocks.numel(), n_blocks, page_size, base, out.slots.numel())

@@ -10,12 +10,13 @@ without one waits for its kernels and raises at once.
 
 from __future__ import annotations
 
+import torch
+
 from . import _lib
 
 
 class DeviceStatus:
     def __init__(self, device="cuda"):
-        import torch
         self.word = torch.zeros(1, dtype=torch.int32, device=device)
         self.ptr = self.word.data_ptr()
 
@@ -23,7 +24,6 @@ class DeviceStatus:
         """Wait for the stream (default: the current one); raise EngineError
         with LS_ECAPACITY or LS_EDEVICE, and clear the word, if a call on it
         recorded a fault."""
-        import torch
         device = self.word.device
         if stream is None:
             stream = torch.cuda.current_stream(device).cuda_stream
@@ -31,24 +31,33 @@ class DeviceStatus:
             _lib.check(_lib.lib().ls_check_status(self.ptr, stream))
 
 
+# The current stream's handle without the Stream object around it, which costs
+# 2 of the ~8 microseconds that a small call takes on the host.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def enqueue(call, pack, before, after, device, status, stream):
     """Run `call(struct, stream)` on the tensors' device, where the struct is
     pack(*before, status word, *after); with no status, wait and raise."""
-    import torch
     if stream is None:
-        stream = torch.cuda.current_stream(device).cuda_stream
+        stream = _raw_stream(device.index)
     if status is None:
         with torch.cuda.device(device), torch.cuda.stream(torch.cuda.ExternalStream(stream, device)):
             own = DeviceStatus(device)
             _lib.check(call(pack(*before, own.ptr, *after), stream))
             own.check(stream)
-    elif device.index == torch.cuda.current_device():
-        _lib.check(call(pack(*before, status.ptr, *after), stream))
+        return
+    if device.index == torch.cuda.current_device():
+        code = call(pack(*before, status.ptr, *after), stream)
     else:
         with torch.cuda.device(device):
-            _lib.check(call(pack(*before, status.ptr, *after), stream))
+            code = call(pack(*before, status.ptr, *after), stream)
+    if code:
+        _lib.check(code)
 
 
-def require(ok, message):
-    if not ok:
-        raise ValueError(message)
+def on_stream(device, stream):
+    """A context whose allocations belong to `stream` (a handle, or None for the current one)."""
+    return torch.cuda.stream(torch.cuda.current_stream(device) if stream is None
+                             else torch.cuda.ExternalStream(stream, device))
