@@ -93,23 +93,27 @@ void run_build_slots(const ls_slots_args& p, cudaStream_t stream) {
           LS_EINVAL, "slot maps: slots, positions and table entries must stay below 2^31");
   SlotArgs a{p.lens, p.delta, p.n_requests, p.block_table, (long)p.table_stride, p.table_width,
              p.free_blocks, p.free_capacity, p.free_count, p.n_blocks, shift, p.base, p.max_tokens,
-             p.slots, p.positions, p.requests, p.token_start, p.lens_out, p.free_count_out, p.status};
+             p.slots, p.positions, p.requests, p.token_start, p.lens_out, p.free_count_out, p.status, false};
   const size_t smem = slot_smem_bytes(p.n_requests);
   if (smem > 48 * 1024) allow_smem<build_slots_kernel>(slot_smem_bytes(kSlotMaxRequests));
-  // one CTA while every thread has at most 4 tokens; more CTAs share the
-  // stores of a prompt batch but each repeats the sums
-  int ctas = 1;
-  while (ctas < kSlotMaxCluster && (long)ctas * kSlotThreads * 4 < std::max(p.max_tokens, p.n_requests)) ctas *= 2;
+  a.in_place = p.lens_out == p.lens || p.free_count_out == p.free_count;
+  // a token a thread, on as many SMs as that takes: each CTA repeats the sums,
+  // but the token loop's dependent loads (length, block) are what takes time
+  const int work = std::max({p.max_tokens, p.n_requests, 1});
+  int ctas = std::min(cdiv(work, kSlotThreads), sm_count());
   cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  if (a.in_place) {
+    ctas = std::min(ctas, kSlotMaxCluster);
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kSlotThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
   CK(cudaLaunchKernelEx(&cfg, build_slots_kernel, a));
 }
 

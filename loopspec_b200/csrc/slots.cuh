@@ -10,15 +10,15 @@
 // token j of request i sits at position len_i + j, in slot
 // table[i][pos / page] * page + pos % page.
 //
-// One launch, one thread-block cluster. Every CTA computes the three running
-// sums over the requests (tokens, blocks taken, blocks given back) by itself,
-// a few KB from L2, so no CTA waits for another's; then tokens and blocks are
-// spread over the cluster, each found by a binary search in the sums. A pop
-// that reaches below the stack's old top reads the giving request's table
-// entry itself and pushes write only above it, so no read of the call meets a
-// write of the call; lens and the count, which may be updated in place, are
-// written after a cluster barrier. Nothing changes when the call cannot be
-// done as a whole.
+// One launch. Every CTA computes the three running sums over the requests
+// (tokens, blocks taken, blocks given back) by itself, a few KB from L2, so no
+// CTA waits for another's; then tokens and blocks are spread over the grid,
+// each found by a binary search in the sums. A pop that reaches below the
+// stack's old top reads the giving request's table entry itself and pushes
+// write only above it, so no read of the call meets a write of the call,
+// except where lens and the count are updated in place: then the grid is one
+// thread-block cluster (at most 8 CTAs) and they are written after a barrier.
+// Nothing changes when the call cannot be done as a whole.
 //
 // Bound: launch and dependent-load latency (a decode step moves a few KB).
 #pragma once
@@ -54,6 +54,7 @@ struct SlotArgs {
   int* lens_out;
   int* free_count_out;
   int* status;
+  bool in_place;
 };
 
 inline size_t slot_smem_bytes(int n_requests) { return sizeof(int) * 3 * ((size_t)n_requests + 1); }
@@ -71,13 +72,13 @@ __device__ __forceinline__ int owner_of(const int* sums, int n, int k) {
 
 __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
   namespace cg = cooperative_groups;
-  cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ int s_sums[];
   const int R = a.n_requests;
   int* s_tok = s_sums;
   int* s_grow = s_sums + (R + 1);
   int* s_back = s_sums + 2 * (R + 1);
-  __shared__ long long s_part[kSlotThreads / 32][3];
+  __shared__ long long s_tok_part[kSlotThreads / 32];
+  __shared__ int2 s_part[kSlotThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int page = 1 << a.page_shift;
   const long capacity = (long)a.table_width << a.page_shift;
@@ -86,7 +87,8 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
   // scans the runs (64-bit: lengths may be garbage), the thread lays them out
   const int per = (R + kSlotThreads - 1) / kSlotThreads;
   const int r0 = min(R, tid * per), r1 = min(R, r0 + per);
-  long long sum[3] = {0, 0, 0};
+  long long tok = 0;
+  int grow = 0, back = 0;   // table entries, below 2^31 in all
   int bad = 0;
   for (int i = r0; i < r1; ++i) {
     const long len = a.lens[i], now = len + a.delta[i];
@@ -95,42 +97,57 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
       continue;
     }
     const int have = (int)((len + page - 1) >> a.page_shift), need = (int)((now + page - 1) >> a.page_shift);
-    sum[0] += max(0L, now - len);
-    sum[1] += max(0, need - have);
-    sum[2] += max(0, have - need);
+    tok += max(0L, now - len);
+    grow += max(0, need - have);
+    back += max(0, have - need);
   }
   const long count = a.free_count[0];
-  long long upto[3];
+  long long tok_to = tok;
+  int grow_to = grow, back_to = back;
 #pragma unroll
-  for (int q = 0; q < 3; ++q) {
-    long long v = sum[q];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += u;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, tok_to, o);
+    const int g = __shfl_up_sync(0xffffffffu, grow_to, o), b = __shfl_up_sync(0xffffffffu, back_to, o);
+    if (lane >= o) {
+      tok_to += t;
+      grow_to += g;
+      back_to += b;
     }
-    upto[q] = v;
-    if (lane == 31) s_part[warp][q] = v;
+  }
+  if (lane == 31) {
+    s_tok_part[warp] = tok_to;
+    s_part[warp] = make_int2(grow_to, back_to);
   }
   bad = __syncthreads_or(bad);
-  long long total[3] = {0, 0, 0};
+  // the warps' totals: each warp scans the 16 of them again
+  long long n_tok_all = lane < kSlotThreads / 32 ? s_tok_part[lane] : 0;
+  int2 all = lane < kSlotThreads / 32 ? s_part[lane] : make_int2(0, 0);
 #pragma unroll
-  for (int q = 0; q < 3; ++q) {
-    long long before = 0;
-    for (int w = 0; w < kSlotThreads / 32; ++w) {
-      if (w == warp) before = total[q];
-      total[q] += s_part[w][q];
+  for (int o = 1; o < kSlotThreads / 32; o <<= 1) {
+    const long long t = __shfl_up_sync(0xffffffffu, n_tok_all, o);
+    const int g = __shfl_up_sync(0xffffffffu, all.x, o), b = __shfl_up_sync(0xffffffffu, all.y, o);
+    if (lane >= o) {
+      n_tok_all += t;
+      all.x += g;
+      all.y += b;
     }
-    upto[q] += before - sum[q];
   }
+  const int before = max(0, warp - 1);
+  const long long tok_before = __shfl_sync(0xffffffffu, n_tok_all, before);
+  const int grow_before = __shfl_sync(0xffffffffu, all.x, before), back_before = __shfl_sync(0xffffffffu, all.y, before);
+  const long long total_tok = __shfl_sync(0xffffffffu, n_tok_all, kSlotThreads / 32 - 1);
+  const long total_grow = __shfl_sync(0xffffffffu, all.x, kSlotThreads / 32 - 1),
+             total_back = __shfl_sync(0xffffffffu, all.y, kSlotThreads / 32 - 1);
+  tok_to += (warp ? tok_before : 0) - tok;
+  grow_to += (warp ? grow_before : 0) - grow;
+  back_to += (warp ? back_before : 0) - back;
   int code = kDevOk;
   if (bad || count < 0 || count > a.free_capacity) code = kDevBadLength;
-  else if (total[0] > a.max_tokens) code = kDevTooManyTokens;
-  else if (total[1] > count + total[2]) code = kDevNoBlocks;
-  else if (count + total[2] - total[1] > a.free_capacity) code = kDevBadLength;
+  else if (total_tok > a.max_tokens) code = kDevTooManyTokens;
+  else if (total_grow > count + total_back) code = kDevNoBlocks;
+  else if (count + total_back - total_grow > a.free_capacity) code = kDevBadLength;
 
-  const int rank = (int)cluster.block_rank(), n_cta = (int)cluster.num_blocks();
-  const int at = rank * kSlotThreads + tid, step = n_cta * kSlotThreads;
+  const int at = (int)blockIdx.x * kSlotThreads + tid, step = (int)gridDim.x * kSlotThreads;
   if (code != kDevOk) {   // all or nothing
     if (at == 0) atomicCAS(a.status, kDevOk, code);
     for (int k = at; k < a.max_tokens; k += step) {
@@ -145,7 +162,7 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
     return;
   }
 
-  int t = (int)upto[0], g = (int)upto[1], b = (int)upto[2];
+  int t = (int)tok_to, g = grow_to, b = back_to;
   for (int i = r0; i < r1; ++i) {
     const int len = a.lens[i], now = len + a.delta[i];
     const int have = (len + page - 1) >> a.page_shift, need = (now + page - 1) >> a.page_shift;
@@ -156,7 +173,7 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
     g += max(0, need - have);
     b += max(0, have - need);
   }
-  const int n_tok = (int)total[0], n_take = (int)total[1], n_give = (int)total[2];
+  const int n_tok = (int)total_tok, n_take = (int)total_grow, n_give = (int)total_back;
   if (tid == 0) {
     s_tok[R] = n_tok;
     s_grow[R] = n_take;
@@ -200,7 +217,7 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
   }
   for (long p = count + at; p < count + n_give - n_take; p += step) a.free_blocks[p] = given((int)(p - count));
   for (int i = at; i <= R; i += step) a.token_start[i] = s_tok[i];
-  cluster.sync();   // every CTA has read lens and the count
+  if (a.in_place) cg::this_cluster().sync();   // every CTA has read lens and the count
   for (int i = at; i < R; i += step) a.lens_out[i] = a.lens[i] + a.delta[i];
   if (at == 0) a.free_count_out[0] = (int)(count + n_give - n_take);
 }
