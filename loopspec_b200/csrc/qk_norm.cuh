@@ -85,8 +85,20 @@ __device__ __forceinline__ void load8_as(const void* p, int type, int i, float (
   else load8(static_cast<const float*>(p) + i, f);
 }
 
-// grid (n_tokens, parts): part p of a token's heads, kQkThreads*16/HD at a time.
-template <typename T, typename C, int HD, bool INTERLEAVED>
+// 8 consecutive values as loaded: they wait in this form, half the registers of fp32 for 16-bit types.
+template <typename T>
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const { load8(reinterpret_cast<const T*>(v), f); }
+};
+
+// grid (n_tokens, parts): part p of a token's heads, U passes of kQkThreads*16/HD
+// heads at a time, whose loads are all issued before the first is used.
+template <typename T, typename C, int HD, bool INTERLEAVED, int U>
 __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(QkNormArgs a) {
   constexpr int L = HD / 16;                 // lanes of one head
   constexpr int HEADS = kQkThreads / L;      // heads of a CTA at a time
@@ -95,10 +107,7 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(QkNormArgs a) 
   const int heads = a.nh + 2 * a.nkv;
   const int pos = a.positions[t];
   const int slot = a.slots ? a.slots[t] : t;
-  const bool pos_ok = pos >= 0 && pos < a.max_positions;
-  const bool slot_ok = pos_ok && slot >= 0 && slot < a.n_slots;
-  // a slot of -1 marks padding, whose K/V go nowhere
-  if (threadIdx.x == 0 && (!pos_ok || slot < -1 || slot >= a.n_slots)) atomicCAS(a.status, kDevOk, kDevBadIndex);
+  const T* src = static_cast<const T*>(a.qkv) + (long)t * a.qkv_stride;
 
   // this lane's chunks (units of 8 elements): the rotated ones hold whole
   // pairs, the rest are neighbours
@@ -115,6 +124,23 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(QkNormArgs a) 
     ca = turn_a ? j : rc + 2 * (j - rc / 2);
     cb = turn_a ? j + rc / 2 : ca + 1;
   }
+  // the first heads are on their way while the position is looked up
+  Raw8<T> xs[U], ys[U];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = min(h0 + u * HEADS + (int)threadIdx.x / L, heads - 1);   // past the last: read it again, store nothing
+      xs[u].load(src + (long)h * HD + 8 * ca);
+      ys[u].load(src + (long)h * HD + 8 * cb);
+    }
+  };
+  load(blockIdx.y * (HEADS * U));
+
+  const bool pos_ok = pos >= 0 && pos < a.max_positions;
+  const bool slot_ok = pos_ok && slot >= 0 && slot < a.n_slots;
+  // a slot of -1 marks padding, whose K/V go nowhere
+  if (threadIdx.x == 0 && (!pos_ok || slot < -1 || slot >= a.n_slots)) atomicCAS(a.status, kDevOk, kDevBadIndex);
+
   // cosines and sines: 8 pairs (i, i + rot/2), or 4 pairs of each chunk
   float cs[8], sn[8];
 #pragma unroll
@@ -140,74 +166,71 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(QkNormArgs a) 
     }
   }
 
-  const T* src = static_cast<const T*>(a.qkv) + (long)t * a.qkv_stride;
   T* q_row = static_cast<T*>(a.q_out) + (long)t * a.q_out_stride;
   C* k_row = static_cast<C*>(a.k_pool) + (long)(slot_ok ? slot : 0) * a.slot_stride;
   C* v_row = static_cast<C*>(a.v_pool) + (long)(slot_ok ? slot : 0) * a.slot_stride;
   // whole warps loop together: the norm's shuffles need every lane
-  for (int h0 = blockIdx.y * HEADS; h0 < heads; h0 += gridDim.y * HEADS) {
-    const int h = h0 + threadIdx.x / L;
-    const bool live = h < heads;
-    float x[8], y[8];
-    if (live) {
-      load8(src + (long)h * HD + 8 * ca, x);
-      load8(src + (long)h * HD + 8 * cb, y);
-    } else {
+  for (int h0 = blockIdx.y * (HEADS * U); h0 < heads; h0 += gridDim.y * (HEADS * U)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
-    }
-    float ss = 0.f;
+    for (int u = 0; u < U; ++u) {
+      float x[8], y[8];
+      xs[u].get(x);
+      ys[u].get(y);
+      const int h = h0 + u * HEADS + threadIdx.x / L;
+      float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
+      for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!live) continue;
-    if (h >= a.nh + a.nkv) {
-      if (slot_ok) {
-        store8(v_row + (long)(h - a.nh - a.nkv) * HD + 8 * ca, x);
-        store8(v_row + (long)(h - a.nh - a.nkv) * HD + 8 * cb, y);
-      }
-      continue;
-    }
-    float wx[8], wy[8];
-    const void* w = h < a.nh ? a.q_weight : a.k_weight;
-    load8_as(w, a.weight_type, 8 * ca, wx);
-    load8_as(w, a.weight_type, 8 * cb, wy);
-    const float inv = rsqrtf(ss / HD + a.eps);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = x[i] * inv * wx[i];
-      y[i] = y[i] * inv * wy[i];
-    }
-    // unrotated chunks stay out of the products: 0 * inf would spoil them
-    if (INTERLEAVED) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x1 = x[2 * i], x2 = x[2 * i + 1], y1 = y[2 * i], y2 = y[2 * i + 1];
-        if (turn_a) {
-          x[2 * i] = x1 * cs[i] - x2 * sn[i];
-          x[2 * i + 1] = x2 * cs[i] + x1 * sn[i];
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (h >= heads) continue;
+      if (h >= a.nh + a.nkv) {
+        if (slot_ok) {
+          store8(v_row + (long)(h - a.nh - a.nkv) * HD + 8 * ca, x);
+          store8(v_row + (long)(h - a.nh - a.nkv) * HD + 8 * cb, y);
         }
-        if (turn_b) {
-          y[2 * i] = y1 * cs[4 + i] - y2 * sn[4 + i];
-          y[2 * i + 1] = y2 * cs[4 + i] + y1 * sn[4 + i];
-        }
+        continue;
       }
-    } else if (turn_a) {
+      float wx[8], wy[8];
+      const void* w = h < a.nh ? a.q_weight : a.k_weight;
+      load8_as(w, a.weight_type, 8 * ca, wx);
+      load8_as(w, a.weight_type, 8 * cb, wy);
+      const float inv = rsqrtf(ss / HD + a.eps);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float x1 = x[i], x2 = y[i];
-        x[i] = x1 * cs[i] - x2 * sn[i];
-        y[i] = x2 * cs[i] + x1 * sn[i];
+        x[i] = x[i] * inv * wx[i];
+        y[i] = y[i] * inv * wy[i];
+      }
+      // unrotated chunks stay out of the products: 0 * inf would spoil them
+      if (INTERLEAVED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x1 = x[2 * i], x2 = x[2 * i + 1], y1 = y[2 * i], y2 = y[2 * i + 1];
+          if (turn_a) {
+            x[2 * i] = x1 * cs[i] - x2 * sn[i];
+            x[2 * i + 1] = x2 * cs[i] + x1 * sn[i];
+          }
+          if (turn_b) {
+            y[2 * i] = y1 * cs[4 + i] - y2 * sn[4 + i];
+            y[2 * i + 1] = y2 * cs[4 + i] + y1 * sn[4 + i];
+          }
+        }
+      } else if (turn_a) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x1 = x[i], x2 = y[i];
+          x[i] = x1 * cs[i] - x2 * sn[i];
+          y[i] = x2 * cs[i] + x1 * sn[i];
+        }
+      }
+      if (h < a.nh) {
+        store8(q_row + (long)h * HD + 8 * ca, x);
+        store8(q_row + (long)h * HD + 8 * cb, y);
+      } else if (slot_ok) {
+        store8(k_row + (long)(h - a.nh) * HD + 8 * ca, x);
+        store8(k_row + (long)(h - a.nh) * HD + 8 * cb, y);
       }
     }
-    if (h < a.nh) {
-      store8(q_row + (long)h * HD + 8 * ca, x);
-      store8(q_row + (long)h * HD + 8 * cb, y);
-    } else if (slot_ok) {
-      store8(k_row + (long)(h - a.nh) * HD + 8 * ca, x);
-      store8(k_row + (long)(h - a.nh) * HD + 8 * cb, y);
-    }
+    if (h0 + gridDim.y * (HEADS * U) < heads) load(h0 + gridDim.y * (HEADS * U));
   }
 }
 

@@ -118,12 +118,20 @@ void run_build_slots(const ls_slots_args& p, cudaStream_t stream) {
 }
 
 // ----------------------------------------------------------- norm and rotation
+template <typename T, typename C, int HD, int U>
+void launch_qk(const QkNormArgs& a, bool interleaved, cudaStream_t stream) {
+  const dim3 grid(a.n_tokens, cdiv(a.nh + 2 * a.nkv, kQkThreads * 16 / HD * U));
+  if (interleaved) launch(qk_norm_rope_kernel<T, C, HD, true, U>, grid, dim3(kQkThreads), 0, stream, false, a);
+  else launch(qk_norm_rope_kernel<T, C, HD, false, U>, grid, dim3(kQkThreads), 0, stream, false, a);
+}
+
+// One pass a CTA while the passes fit the GPU at once (about 8 CTAs an SM);
+// three for prompts, where loads in flight decide.
 template <typename T, typename C, int HD>
 void launch_qk(const QkNormArgs& a, bool interleaved, cudaStream_t stream) {
-  constexpr int kHeads = kQkThreads * 16 / HD;
-  const dim3 grid(a.n_tokens, cdiv(a.nh + 2 * a.nkv, kHeads));
-  if (interleaved) launch(qk_norm_rope_kernel<T, C, HD, true>, grid, dim3(kQkThreads), 0, stream, false, a);
-  else launch(qk_norm_rope_kernel<T, C, HD, false>, grid, dim3(kQkThreads), 0, stream, false, a);
+  const long passes = (long)a.n_tokens * cdiv(a.nh + 2 * a.nkv, kQkThreads * 16 / HD);
+  if (passes <= 8L * sm_count()) launch_qk<T, C, HD, 1>(a, interleaved, stream);
+  else launch_qk<T, C, HD, 3>(a, interleaved, stream);
 }
 
 template <typename T, typename C>
