@@ -65,6 +65,7 @@ struct PrefixAttnArgs {
   int suffix_parts, suffix_chunk;
   int prefix_tiles, suffix_tiles;    // row tiles of 16 (prefix: of its own kernel's rows)
   bool prefix_units;                 // the unit kernel also does the prefix
+  bool own, direct;                  // tcgen05 kernel: rows of one request and its own positions; whole results
   int* status;
 };
 

@@ -1,23 +1,35 @@
-// Shared-prefix attention on the 5th-generation tensor cores: the prefix units
-// of a batch with 16-bit queries (the formulas are in prefix_attn.cuh).
+// Shared-prefix attention on the 5th-generation tensor cores, for 16-bit
+// queries (the formulas are in prefix_attn.cuh).
 //
-// A unit is (MT row tiles of 128, kv head, key range); its rows are query
-// heads of any requests, since the prefix is the same for all. One CTA a unit:
-//   4 producer warps gather the range's K and V rows, 128 keys at a time,
-//     through the prefix's block table with 16-byte cp.async into a ring of
+// A unit is (MT row tiles of 128, kv head, key range). Either the rows are
+// query heads of any requests and the keys a range of the prefix (they are the
+// same for all; the result is a part to be joined), or, where requests bring
+// whole tiles of rows (prompts), the rows are one request's and the keys a
+// range of the prefix, the last range followed by the request's own positions;
+// with one range that is the whole result, which is normalised and stored.
+// One CTA a unit:
+//   3 producer warps gather K and V rows, a tile of 128 keys each in turn,
+//     through the block table with 16-byte cp.async into a ring of
 //     128-byte-swizzled tiles;
-//   one thread issues S = Q K^T and O += P V (tcgen05.mma, M = 128): K is the
+//   one warp issues S = Q K^T and O += P V (tcgen05.mma, M = 128): K is the
 //     K-major operand as gathered, V the MN-major one, so neither is moved
 //     again; S and O live in tensor memory;
-//   4 MT softmax warps own a row a thread: no reduction crosses threads. A
-//     thread reads its 128 scores, writes P over them in the operand's type
-//     (the A operand of the second product comes from tensor memory) and keeps
-//     the running maximum and sum. O is rescaled only when a row's maximum has
-//     grown by more than 2^8 since its reference was set: until then the old
-//     reference stays, weights reach 2^8, and nothing else changes, as the
-//     reference cancels in o / l.
+//   8 MT softmax warps: two threads a row, 64 of the tile's 128 scores each
+//     (with one thread a row two warps an SM quarter could not cover each
+//     other's latencies: 3200-3500 cycles a pair of tiles). They agree on the
+//     row's maximum through shared memory and write P over S in the operand's
+//     type (the A operand of the second product comes from tensor memory). O
+//     is rescaled only when a row's maximum has grown by more than 2^8 since
+//     its reference was set: until then the old reference stays, weights reach
+//     2^8, and nothing else changes, as the reference cancels in o / l.
 // With MT = 2 the tensor cores work on one row tile while the softmax warps
 // work on the other; with MT = 1 on the next key tile (two score buffers).
+//
+// A row must not see what later tokens of its request hold: their scores leave
+// by selection, but a weight of 0 times a NaN or infinity in V is NaN. So the
+// producers look at the V rows that only some of a unit's rows see (at most as
+// many as the unit has tokens), copy zeros for one that is not finite, and
+// note it; the rows that do see it add its term at the end.
 #pragma once
 
 #include "prefix_attn.cuh"
@@ -30,15 +42,22 @@ constexpr float kTcGrow = 8.f;        // log2 growth of a row's maximum that mov
 
 template <int HD, int MT>
 struct TcLayout {
-  static constexpr int kThreads = MT == 1 ? 384 : 512;
-  static constexpr int kProducer = 4 * MT;                 // first producer warp
-  static constexpr int kMma = kProducer + 4;               // the issuing warp
+  static constexpr int kProducer = 8 * MT;                 // first producer warp
+  static constexpr int kProducers = 3;
+  static constexpr int kMma = kProducer + kProducers;      // the issuing warp
+  static constexpr int kThreads = 32 * (kMma + 1);
+  // With MT = 2 a thread is launched with 96 registers; the softmax warps draw
+  // on what the last four warps give back: 640 x 96 = 512 x 104 + 128 x 64.
+  static constexpr int kSoftRegs = 104, kRestRegs = 64;
+  static constexpr int kLaunchRegs = MT == 2 ? (512 * kSoftRegs + 128 * kRestRegs) / kThreads : 0;
   static constexpr int kTile = kTcKeys * HD * 2;           // bytes of a K, V or Q tile
   static constexpr int kStages = HD == 64 ? 8 : MT == 1 ? 6 : 5;
-  static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 1;
-  static constexpr int kSmem = MT * kTile + kStages * kTile + 2 * kTcKeys * 4 + kBars * 8 + 16;
+  static constexpr int kMaxBuffers = MT == 1 ? 2 : 1;      // see the softmax warps
+  static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 1 + 1;
+  static constexpr int kSmem = MT * kTile + kStages * kTile + kMaxBuffers * MT * 2 * kTcRows * 4 + kBars * 8 + 8 * 4 + 16;
   static constexpr int kPoly = 3;                          // eighths of the exponentials on the FMA units
   static constexpr uint32_t kScores = 0, kOut = 256;       // tensor memory columns
+  static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 };
 
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
@@ -105,10 +124,6 @@ __host__ __device__ constexpr uint32_t tc_idesc(int M, int N, bool b_mn_major) {
          ((uint32_t)(M >> 4) << 24);
 }
 
-#define LS_TMEM32(r)                                                                                          \
-  r[0], r[1], r[2], r[3], r[4], r[5], r[6], r[7], r[8], r[9], r[10], r[11], r[12], r[13], r[14], r[15], r[16], \
-      r[17], r[18], r[19], r[20], r[21], r[22], r[23], r[24], r[25], r[26], r[27], r[28], r[29], r[30], r[31]
-
 // 32 lanes x 32 consecutive columns a warp.
 __device__ __forceinline__ void tmem_ld_x32(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -131,7 +146,6 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-#undef LS_TMEM32
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -156,29 +170,41 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// Maxima that are NaN when an operand is.
+__device__ __forceinline__ float max2_nan(float a, float b) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 
 // 2^x of a pair on the FMA units, for 16-bit weights: x = n + f with n = round(x)
 // (added to 1.5 * 2^23 it sits in the low mantissa bits), |f| <= 1/2, 2^f by the
 // cubic that minimises the largest relative error there (Remez exchange: 7.5e-5,
-// a fiftieth of bf16's half unit, a seventh of f16's), n added to the exponent.
-// Below 2^-126 the result stays about 2^-127 instead of 0.
+// a fiftieth of bf16's half unit, a seventh of f16's), times 2^n put together
+// from its exponent bits: 0 from n = -127 on down, so a masked score weighs
+// nothing. NaN is not passed on; the caller's row maximum does that.
 __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
   constexpr float kMagic = 12582912.f;
   const float2 v = unpair(x);
-  x = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  x = pair(fmaxf(v.x, -127.f), fmaxf(v.y, -127.f));
   const uint64_t t = add2(x, pair(kMagic, kMagic));
   const uint64_t f = fma2(add2(t, pair(-kMagic, -kMagic)), pair(-1.f, -1.f), x);
   uint64_t y = fma2(f, pair(0.055171669f, 0.055171669f), pair(0.24261112f, 0.24261112f));
   y = fma2(y, f, pair(0.69326099f, 0.69326099f));
   y = fma2(y, f, pair(0.99992807f, 0.99992807f));
-  const float2 n = unpair(t), r = unpair(y);
-  return pair(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(n.x) << 23)),
-              __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
+  const float2 n = unpair(t);
+  return mul2(y, pair(__uint_as_float((__float_as_uint(n.x) << 23) + 0x3f800000u),
+                      __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u)));
 }
 
 // A whole warp's wait: all lanes agree on the outcome, so none leaves the others in a collective.
@@ -191,9 +217,51 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void producers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
-// grid: 1-D over (row tile fastest, kv head, part): CTAs that run together read the same keys.
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void cp_async16_to(uint32_t dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+// The weight of own position `pos` for a row whose reference is m, by the formula.
+template <int HD, typename C>
+__device__ __noinline__ float weight_of(const C* q, const C* k, float m, float scale_log2) {
+  float s = 0.f;
+  for (int i = 0; i < HD; ++i) s += (float)q[i] * (float)k[i];
+  const float base = (m == -INFINITY ? 0.f : m * scale_log2) - weight_bias(C());
+  return exp2_fast(s * scale_log2 - base);
+}
+
+// Whether 8 packed 16-bit values hold a NaN or infinity (exponent bits all set).
+template <typename C>
+__device__ __forceinline__ bool not_finite8(const uint4& v) {
+  constexpr uint32_t kExp = std::is_same<C, __half>::value ? 0x7C00u : 0x7F80u;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bad |= (w[i] & kExp) == kExp || ((w[i] >> 16) & kExp) == kExp;
+  return bad;
+}
+
+// grid: 1-D over (row tile fastest, kv head, part, request if `own`): CTAs that run together read the same keys.
 template <int HD, typename C, int MT>
 __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kernel(PrefixAttnArgs a) {
   using L = TcLayout<HD, MT>;
@@ -203,36 +271,74 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* s_q = smem;
   unsigned char* s_ring = smem + MT * L::kTile;
-  int* s_slot = reinterpret_cast<int*>(s_ring + ST * L::kTile);      // [2][kTcKeys]
-  const uint32_t bars = smem_u32(s_slot + 2 * kTcKeys);
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_slot + 2 * kTcKeys + 2 * L::kBars);
+  float* s_max = reinterpret_cast<float*>(s_ring + ST * L::kTile);   // [kMaxBuffers][MT][half][row]
+  const uint32_t bars = smem_u32(s_max + L::kMaxBuffers * MT * 2 * kTcRows);
+  uint32_t* s_bad = reinterpret_cast<uint32_t*>(s_max + L::kMaxBuffers * MT * 2 * kTcRows) + 2 * L::kBars;   // [8] bits
+  uint32_t* s_tmem = s_bad + 8;
   const uint32_t full0 = bars, empty0 = full0 + 8 * ST, s_full = empty0 + 8 * ST, p_full = s_full + 16,
-                 pv_done = p_full + 16, q_full = pv_done + 16;
+                 pv_done = p_full + 16, q_full = pv_done + 16, noted = q_full + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
 
+  // the unit: its rows, and its keys as prefix positions [ka0, ka1) and own positions [0, kb1)
   const int G = a.nh / a.nkv;
-  const int tile = blockIdx.x % a.prefix_tiles;
-  const int g = (blockIdx.x / a.prefix_tiles) % a.nkv;
-  const int part = blockIdx.x / a.prefix_tiles / a.nkv;
-  const int rows = a.n_tokens * G;                 // rows of the kv head
+  unsigned u = blockIdx.x;
+  const int tile = (int)(u % (unsigned)a.prefix_tiles);
+  u /= (unsigned)a.prefix_tiles;
+  const int g = (int)(u % (unsigned)a.nkv);
+  u /= (unsigned)a.nkv;
+  const unsigned n_parts = max(1, a.prefix_parts);
+  const int part = (int)(u % n_parts), req = (int)(u / n_parts);
+  int start = 0, n_new = a.n_tokens, len = 0;
+  if (a.own) {
+    const bool ok = request_range(a, req, start, n_new, len);
+    if (tile == 0 && part == 0) {
+      // tokens of no request, and those of one that is out of bounds, get zeros
+      auto clear = [&](int t0, int t1) {
+        t0 = max(0, t0);
+        t1 = min(a.n_tokens, t1);
+        for (int i = threadIdx.x; i < (t1 - t0) * G * CH; i += blockDim.x) {
+          const int t = t0 + i / (G * CH), c = i % (G * CH);
+          *reinterpret_cast<uint4*>(static_cast<C*>(a.out) + (long)t * a.out_stride + (long)g * G * HD + c * 8) =
+              make_uint4(0, 0, 0, 0);
+        }
+      };
+      if (a.direct) {
+        if (req == 0) clear(0, a.token_start[0]);
+        if (req == a.n_requests - 1) clear(a.token_start[a.n_requests], a.n_tokens);
+        if (!ok) clear(a.token_start[req], a.token_start[req + 1]);
+      }
+    }
+    if (!ok) return;
+  }
+  const int rows = n_new * G;                      // rows of the kv head
   const int row0 = tile * (MT * kTcRows);
-  const int k0 = part * a.prefix_chunk, k1 = min(a.prefix_len, k0 + a.prefix_chunk);
-  const int n = (k1 - k0 + kTcKeys - 1) / kTcKeys; // key tiles, at least one
+  if (row0 >= rows) return;
+  const int seen0 = len - n_new + 1;               // own positions the request's first new token sees
+  const int ka0 = part * a.prefix_chunk, ka1 = min(a.prefix_len, ka0 + a.prefix_chunk);
+  const int last_row = min(rows, row0 + MT * kTcRows) - 1;
+  const int see_first = seen0 + row0 / G;          // own positions every row sees, and some row sees
+  const int kb1 = a.own && part == (int)n_parts - 1 ? max(0, min(len, seen0 + last_row / G)) : 0;
+  const int na = (max(0, ka1 - ka0) + kTcKeys - 1) / kTcKeys;
+  const int n = na + (kb1 + kTcKeys - 1) / kTcKeys;    // key tiles
+  const int* own_table = a.block_table + req * a.table_stride;
 
-  // softmax warps with rows of their own; the others have nothing to do
+  // softmax warps of a row tile's half with rows of their own; the others have nothing to do
   auto live_warps = [&](int t) { return max(0, min(4, (rows - row0 - t * kTcRows + 31) / 32)); };
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; ++s) {
-      mbar_init(full0 + 8 * s, 128);
+      mbar_init(full0 + 8 * s, 32);
       mbar_init(empty0 + 8 * s, 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(s_full + 8 * b, 1);
       // with MT = 2 a buffer belongs to a row tile; one without rows is never used
-      mbar_init(p_full + 8 * b, max(1, live_warps(MT == 2 ? b : 0)));
+      mbar_init(p_full + 8 * b, max(1, 2 * live_warps(MT == 2 ? b : 0)));
       mbar_init(pv_done + 8 * b, 1);
     }
-    mbar_init(q_full, 4 * MT);
+    mbar_init(q_full, 8 * MT);
+    mbar_init(noted, L::kProducers);
+    for (int i = 0; i < 8; ++i) s_bad[i] = 0;
     fence_barrier_init();
   }
   if (warp == L::kMma) {
@@ -244,22 +350,21 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
   const int tiles_here = MT == 2 && live_warps(1) > 0 ? 2 : 1;   // row tiles with rows
-  pdl_launch_dependents();
 
   if (warp < L::kProducer) {
     // ---------------------------------------------------------------- softmax
-    if (MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    const int t = warp >> 2, quarter = warp & 3;
+    if (MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftRegs));
+    const int t = MT == 2 ? warp >> 3 : 0, half = (warp >> 2) & 1, quarter = warp & 3;
     // the row tile's queries, swizzled; rows past the last are zeros
     {
       unsigned char* dst = s_q + t * L::kTile;
       const C* q = static_cast<const C*>(a.q);
-      for (int i = threadIdx.x & 127; i < kTcRows * CH; i += 128) {
+      for (int i = threadIdx.x & 255; i < kTcRows * CH; i += 256) {
         const int r = i / CH, c = i % CH, rr = row0 + t * kTcRows + r;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (rr < rows) {
           const int tok = rr / G, h = g * G + rr - tok * G;
-          v = *reinterpret_cast<const uint4*>(q + (long)tok * a.q_stride + (long)h * HD + c * 8);
+          v = *reinterpret_cast<const uint4*>(q + (long)(start + tok) * a.q_stride + (long)h * HD + c * 8);
         }
         *reinterpret_cast<uint4*>(dst + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
       }
@@ -269,50 +374,66 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
     }
     const int r = quarter * 32 + lane, rr = row0 + t * kTcRows + r;
     if (quarter < live_warps(t)) {
+      const int pair_bar = 1 + t * 4 + quarter;      // the two warps of 32 rows
       const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-      const uint32_t out = lanes + L::kOut + t * 128;
+      const uint32_t out = lanes + L::kOut + t * 128 + half * (HD / 2);
+      // own positions this row sees, within the unit's
+      const int see = rr < rows ? min(kb1, seen0 + rr / G) : kb1;
+      const int see_least = __reduce_min_sync(0xffffffffu, see);
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int j = 0; j < n && ok; ++j) {
+      // After a wait that timed out the warp waits no more, but goes on through
+      // the barriers that it shares with its other half.
+      for (int j = 0; j < n; ++j) {
         const int b = MT == 1 ? j & 1 : t;
         const uint32_t ph = (MT == 1 ? j >> 1 : j) & 1;
-        ok = warp_wait(s_full + 8 * b, ph, a.status, kDevTimeoutAcc);
-        if (!ok) break;
+        // keys of this tile that the row sees, counted from this thread's first
+        int left = (j < na ? ka1 - ka0 - j * kTcKeys : see - (j - na) * kTcKeys) - half * 64;
+        const bool cut = j < na ? j == na - 1 : see_least - (j - na) * kTcKeys < kTcKeys;
+        ok = ok && warp_wait(s_full + 8 * b, ph, a.status, kDevTimeoutAcc);
         tc_fence_after();
         const uint32_t sc = lanes + L::kScores + b * 128;
-        uint32_t s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_x32(sc + 32 * c, s + 32 * c);
+        uint32_t s[64];
+        tmem_ld_x32(sc + half * 64, s);
+        tmem_ld_x32(sc + half * 64 + 32, s + 32);
         tmem_ld_wait();
-        if (j == n - 1) {                          // keys past the range
-          const int left = k1 - k0 - j * kTcKeys;
+        if (cut) {
 #pragma unroll
-          for (int i = 0; i < 128; ++i)
+          for (int i = 0; i < 64; ++i)
             if (i >= left) s[i] = 0xff800000u;     // -inf
         }
         float mx[4] = {m, m, m, m};
 #pragma unroll
-        for (int i = 0; i < 128; i += 2)
-          mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        // m and top are raw scores; their distance counts after the scale
-        const bool move = m == -INFINITY ? top != -INFINITY : (top - m) * a.scale_log2 > kTcGrow;
+        for (int i = 0; i < 64; i += 2)
+          mx[(i >> 1) & 3] = max3_nan(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        float top = max2_nan(max2_nan(mx[0], mx[1]), max2_nan(mx[2], mx[3]));
+        // The other half's maximum. The barrier also tells that both have read
+        // their scores, which P is written over. One buffer does for MT = 2: the
+        // next tile's scores come only after both have finished this one.
+        float* row_max = s_max + ((MT == 1 ? j & 1 : t) * 2) * kTcRows + r;
+        row_max[half * kTcRows] = top;
+        tc_fence_before();
+        asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+        tc_fence_after();
+        top = max2_nan(top, row_max[(half ^ 1) * kTcRows]);
+        // m and top are raw scores; their distance counts after the scale. A NaN
+        // score makes the reference NaN, and with it the whole row
+        const bool move = m == -INFINITY ? top != -INFINITY : !((top - m) * a.scale_log2 <= kTcGrow);
         if (__any_sync(0xffffffffu, move)) {
-          const float keep = move && m != -INFINITY ? exp2_fast((m - top) * a.scale_log2) : 1.f;
+          const float keep = move && m > -INFINITY ? exp2_fast((m - top) * a.scale_log2) : 1.f;
           if (move) m = top;
           l *= keep;
           if (j > 0) {
-            ok = warp_wait(pv_done + 8 * t, (j - 1) & 1, a.status, kDevTimeoutAcc);
-            if (!ok) break;
+            ok = ok && warp_wait(pv_done + 8 * t, (j - 1) & 1, a.status, kDevTimeoutAcc);
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-              uint32_t v[32];
-              tmem_ld_x32(out + c, v);
+            for (int c = 0; c < HD / 2; c += 16) {
+              uint32_t v[16];
+              tmem_ld_x16(out + c, v);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * keep);
-              tmem_st_x32(out + c, v);
+              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * keep);
+              tmem_st_x16(out + c, v);
             }
           }
         }
@@ -321,9 +442,9 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
         // function units, which do 4 of these a cycle and SM quarter
         const uint64_t scale = pair(a.scale_log2, a.scale_log2), minus = pair(-base, -base);
         uint64_t sum[2] = {0, 0};
-        uint32_t p[64];
+        uint32_t p[32];
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
+        for (int i = 0; i < 32; ++i) {
           const uint64_t x = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, minus);
           uint64_t w;
           if ((i * L::kPoly) % 8 < L::kPoly) {
@@ -335,9 +456,9 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
           sum[i & 1] = add2(sum[i & 1], w);
           const float2 v = unpair(w);
           p[i] = pack2(v.x, v.y, C());
-          if (i == 31) tmem_st_x32(sc, p);
+          if (i == 15) tmem_st_x16(sc + half * 32, p);
         }
-        tmem_st_x32(sc + 32, p + 32);
+        tmem_st_x16(sc + half * 32 + 16, p + 16);
         const float2 total = unpair(add2(sum[0], sum[1]));
         l += total.x + total.y;
         tmem_st_wait();
@@ -345,141 +466,193 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + 8 * b);
       }
-      if (ok) ok = warp_wait(pv_done + 8 * t, (n - 1) & 1, a.status, kDevTimeoutAcc);
+      // join the two halves' sums; a wait that timed out leaves zeros
+      bool have = n > 0 && ok;
+      if (have) have = warp_wait(pv_done + 8 * t, (n - 1) & 1, a.status, kDevTimeoutAcc);
+      if (a.own) have = warp_wait(noted, 0, a.status, kDevTimeoutAcc) && have;
       tc_fence_after();
-      long at = 0;
-      if (rr < rows) {
-        const int tok = rr / G;
-        at = ((long)part * a.n_tokens + tok) * a.nh + g * G + rr - tok * G;
-        a.part_ml[at] = ok ? make_float2(m * a.scale_log2, l) : make_float2(-INFINITY, 0.f);
-      }
+      float* row_sum = s_max + ((MT == 1 ? n & 1 : t) * 2) * kTcRows + r;
+      row_sum[half * kTcRows] = l;
+      asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
+      l = row_sum[0] + row_sum[kTcRows];
+      const int tok = start + rr / G, h = g * G + rr % G;
+      const float inv = !have ? 0.f : !a.direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      const long at = ((long)part * a.n_tokens + tok) * a.nh + h;
+      if (!a.direct && rr < rows && half == 0)
+        a.part_ml[at] = have ? make_float2(m * a.scale_log2, l) : make_float2(-INFINITY, 0.f);
 #pragma unroll 1
-      for (int c = 0; c < HD; c += 32) {
-        uint32_t v[32];
-        tmem_ld_x32(out + c, v);
+      for (int c = 0; c < HD / 2; c += 16) {
+        uint32_t v[16];
+        tmem_ld_x16(out + c, v);
         tmem_ld_wait();
-        if (rr < rows) {
+        if (rr >= rows) continue;
+        float f[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(a.part_o + at * HD + c + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        for (int i = 0; i < 16; ++i) f[i] = have ? __uint_as_float(v[i]) * inv : 0.f;
+        const int d = half * (HD / 2) + c;
+        if (a.own && have) {                       // terms left out of the products
+          for (int w = 0; w < 8; ++w)
+            for (uint32_t bits = s_bad[w]; bits; bits &= bits - 1) {
+              const int pos = see_first + w * 32 + __ffs(bits) - 1;
+              if (pos >= see) continue;
+              const long slot = ((long)own_table[pos >> a.page_shift] << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
+              const C* k = static_cast<const C*>(a.k_pool) + slot * a.slot_stride + (long)g * HD;
+              const C* v = static_cast<const C*>(a.v_pool) + slot * a.slot_stride + (long)g * HD + d;
+              const float p = weight_of<HD, C>(static_cast<const C*>(a.q) + (long)tok * a.q_stride + (long)h * HD, k, m,
+                                               a.scale_log2) * inv;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) f[i] += p * (float)v[i];
+            }
+        }
+        if (a.direct) {
+          C* dst = static_cast<C*>(a.out) + (long)tok * a.out_stride + (long)h * HD + d;
+          store8(dst, *reinterpret_cast<float(*)[8]>(f));
+          store8(dst + 8, *reinterpret_cast<float(*)[8]>(f + 8));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; i += 4)
+            store4(a.part_o + at * HD + d + i, make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]));
         }
       }
       tc_fence_before();
     }
-  } else if (warp < L::kMma) {
+  } else if (MT == 2) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kRestRegs));
+  }
+  if (warp >= L::kProducer && warp < L::kMma) {
     // --------------------------------------------------------------- producer
-    if (MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    const int tid = threadIdx.x - 32 * L::kProducer;
-    constexpr int RPI = 128 / CH;                  // rows copied at a time by the 4 warps
-    const int c = tid % CH, r0 = tid / CH;
+    constexpr int RPI = 32 / CH;                   // rows copied at a time
+    const int c = lane % CH, hi = lane / CH;
     const C* kp = static_cast<const C*>(a.k_pool) + (long)g * HD + c * 8;
     const C* vp = static_cast<const C*>(a.v_pool) + (long)g * HD + c * 8;
     const int mask = (1 << a.page_shift) - 1;
-    // the block of key `tid` of tile j: loaded a tile ahead, looked at when its turn comes
-    auto block_of = [&](int j) {
-      const int pos = k0 + j * kTcKeys + tid;
-      return pos < k1 ? a.prefix_table[pos >> a.page_shift] : 0;
-    };
-    int next = block_of(0);
-    bool ok = true;
-    // copy i (2 j: K, 2 j + 1: V) goes to stage i % ST; the barrier counts each
-    // thread's part in when it has landed, so the producers run a ring ahead
-    int issued = 0;
-    // after a wait that timed out the warp copies no more but stays in the barriers
-    for (int j = 0; j < n; ++j) {
-      int* slots = s_slot + (j & 1) * kTcKeys;
-      const int pos = k0 + j * kTcKeys + tid;
-      const long sl = ((long)next << a.page_shift) + (pos & mask);
-      const bool fits = next >= 0 && sl < a.n_slots;
-      if (!fits && pos < k1) atomicCAS(a.status, kDevOk, kDevBadIndex);
-      slots[tid] = fits && pos < k1 ? (int)sl : -1;   // -1: filled with zeros
-      if (j + 1 < n) next = block_of(j + 1);
-      producers_sync();
-#pragma unroll 1
-      for (int kv = 0; kv < 2 && ok; ++kv) {
-        const int st = issued % ST;
-        if (issued >= ST) ok = warp_wait(empty0 + 8 * st, (issued / ST - 1) & 1, a.status, kDevTimeoutEmpty);
-        if (!ok) break;
-        unsigned char* dst = s_ring + st * L::kTile + (c >> 3) * kBlock;
-        const C* src = kv ? vp : kp;
+    const uint32_t dst0 = smem_u32(s_ring) + (c >> 3) * kBlock + hi * 128;
+    // Copy i (2 j: K of tile j, 2 j + 1: its V) goes to stage i % ST and is the
+    // work of warp i % 3; the barrier counts each thread's part in when it has
+    // landed, so the producers run a ring ahead. Lane l knows the slots of rows
+    // l, l + 32, l + 64, l + 96; their blocks are loaded a copy ahead.
+    int next[4];
+    auto look_up = [&](int i) {
+      const int j = i >> 1;
+      const bool own = j >= na;
+      const int* table = own ? own_table : a.prefix_table;
+      const int pos = (own ? (j - na) * kTcKeys : ka0 + j * kTcKeys) + lane, end = i >= 2 * n ? 0 : own ? kb1 : ka1;
 #pragma unroll
-        for (int i = 0; i < kTcKeys / RPI; ++i) {
-          const int r = r0 + i * RPI;
-          const int slot = slots[r];
-          cp_async16(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4), src + (long)max(slot, 0) * a.slot_stride, slot >= 0);
-        }
-        cp_async_arrive(full0 + 8 * st);
-        ++issued;
+      for (int q = 0; q < 4; ++q) next[q] = pos + 32 * q < end ? table[(pos + 32 * q) >> a.page_shift] : 0;
+    };
+    const int first = warp - L::kProducer;
+    look_up(first);
+    for (int i = first; i < 2 * n; i += L::kProducers) {
+      const int j = i >> 1, st = i % ST;
+      const bool own = j >= na, is_v = i & 1;
+      const int pos = (own ? (j - na) * kTcKeys : ka0 + j * kTcKeys) + lane, end = own ? kb1 : ka1;
+      int slot[4];                                 // -1: filled with zeros
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int at = pos + 32 * q;
+        const long sl = ((long)next[q] << a.page_shift) + (at & mask);
+        const bool fits = next[q] >= 0 && sl < a.n_slots;
+        if (!fits && at < end) atomicCAS(a.status, kDevOk, kDevBadIndex);
+        slot[q] = fits && at < end ? (int)sl : -1;
       }
+      look_up(i + L::kProducers);
+      if (own && is_v) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int at = pos + 32 * q;
+          if (slot[q] >= 0 && at >= see_first) {   // a row that only some of the unit's rows see
+            const C* row = static_cast<const C*>(a.v_pool) + (long)slot[q] * a.slot_stride + (long)g * HD;
+            bool bad = false;
+            for (int x = 0; x < HD; x += 8) bad |= not_finite8<C>(*reinterpret_cast<const uint4*>(row + x));
+            if (bad) {
+              atomicOr(s_bad + ((at - see_first) >> 5), 1u << ((at - see_first) & 31));
+              slot[q] = -1;
+            }
+          }
+        }
+        __syncwarp();
+      }
+      if (i >= ST && !warp_wait(empty0 + 8 * st, (i / ST - 1) & 1, a.status, kDevTimeoutEmpty)) break;
+      const uint32_t dst = dst0 + st * L::kTile;
+      const C* src = is_v ? vp : kp;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int x = 0; x < 32 / RPI; ++x) {
+          const int row_slot = __shfl_sync(0xffffffffu, slot[q], x * RPI + hi);
+          const int r = x * RPI + hi;              // the swizzle goes by the row modulo 8
+          cp_async16_to(dst + (32 * q + x * RPI) * 128 + (((c & 7) ^ (r & 7)) << 4),
+                        src + (long)max(row_slot, 0) * a.slot_stride, row_slot >= 0);
+        }
+      cp_async_arrive(full0 + 8 * st);
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(noted);
     cp_async_commit();
     cp_async_wait<0>();
-  } else {
+  } else if (warp == L::kMma) {
     // ------------------------------------------------------------------- issue
-    if (MT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == L::kMma) {
-      constexpr uint32_t idesc_s = tc_idesc<C>(kTcRows, kTcKeys, false);
-      constexpr uint32_t idesc_o = tc_idesc<C>(kTcRows, HD, true);
-      const uint32_t leader = elect_one();
-      const uint32_t ring_k = umma_lo(smem_u32(s_ring), 0), ring_v = umma_lo(smem_u32(s_ring), kBlock),
-                     q0 = umma_lo(smem_u32(s_q), 0);
-      auto wait_full = [&](int i) {
-        const bool ok = warp_wait(full0 + 8 * (i % ST), (i / ST) & 1, a.status, kDevTimeoutFull);
-        fence_proxy_async();                       // copies came by the generic proxy; the products read by the async one
-        tc_fence_after();
-        return ok;
-      };
-      auto release = [&](int i) {                  // copy i's stage, if another copy will want it
-        if (i + ST < 2 * n) tc_commit_if(leader, empty0 + 8 * (i % ST));
-      };
-      auto scores = [&](int t, int b, int j) {     // S[b] = Q[t] K[j]^T
-        const uint32_t k = ring_k + ((2 * j % ST) * L::kTile >> 4), q = q0 + (t * L::kTile >> 4);
+    constexpr uint32_t idesc_s = tc_idesc<C>(kTcRows, kTcKeys, false);
+    constexpr uint32_t idesc_o = tc_idesc<C>(kTcRows, HD, true);
+    const uint32_t leader = elect_one();
+    const uint32_t ring_k = umma_lo(smem_u32(s_ring), 0), ring_v = umma_lo(smem_u32(s_ring), kBlock),
+                   q0 = umma_lo(smem_u32(s_q), 0);
+    auto wait_full = [&](int i) {
+      const bool ok = warp_wait(full0 + 8 * (i % ST), (i / ST) & 1, a.status, kDevTimeoutFull);
+      fence_proxy_async();                         // copies came by the generic proxy; the products read by the async one
+      tc_fence_after();
+      return ok;
+    };
+    auto release = [&](int i) {                    // copy i's stage, if another copy will want it
+      if (i + ST < 2 * n) tc_commit_if(leader, empty0 + 8 * (i % ST));
+    };
+    auto scores = [&](int t, int b, int j) {       // S[b] = Q[t] K[j]^T
+      const uint32_t k = ring_k + ((2 * j % ST) * L::kTile >> 4), q = q0 + (t * L::kTile >> 4);
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-          const uint32_t off = ((i >> 2) * kBlock + (i & 3) * 32) >> 4;
-          tc_mma_ss(leader, tmem + L::kScores + b * 128, q + off, k + off, kUmmaHi, idesc_s, i != 0);
-        }
-        tc_commit_if(leader, s_full + 8 * b);
-      };
-      auto outputs = [&](int t, int b, int j) {    // O[t] += P[b] V[j]
-        const uint32_t v = ring_v + (((2 * j + 1) % ST) * L::kTile >> 4);
-#pragma unroll
-        for (int i = 0; i < kTcKeys / 16; ++i)
-          tc_mma_ts(leader, tmem + L::kOut + t * 128, tmem + L::kScores + b * 128 + i * 8, v + (i * 2048 >> 4), kUmmaHi,
-                    idesc_o, i != 0 ? 1u : (uint32_t)(j != 0));
-        tc_commit_if(leader, pv_done + 8 * t);
-      };
-      bool ok = warp_wait(q_full, 0, a.status, kDevTimeoutFull) && wait_full(0);
-      if (ok) {
-        for (int t = 0; t < tiles_here; ++t) scores(t, t, 0);
-        release(0);
+      for (int i = 0; i < HD / 16; ++i) {
+        const uint32_t off = ((i >> 2) * kBlock + (i & 3) * 32) >> 4;
+        tc_mma_ss(leader, tmem + L::kScores + b * 128, q + off, k + off, kUmmaHi, idesc_s, i != 0);
       }
-      for (int j = 0; j < n && ok; ++j) {
-        const bool more = j + 1 < n;
-        if (MT == 1) {
-          // the buffer's P was consumed by the product issued before this one
-          if (more) {
-            if (!(ok = wait_full(2 * j + 2))) break;
-            scores(0, (j + 1) & 1, j + 1);
-            release(2 * j + 2);
-          }
-          ok = wait_full(2 * j + 1) && warp_wait(p_full + 8 * (j & 1), (j >> 1) & 1, a.status, kDevTimeoutAcc);
-          if (!ok) break;
+      tc_commit_if(leader, s_full + 8 * b);
+    };
+    auto outputs = [&](int t, int b, int j) {      // O[t] += P[b] V[j]
+      const uint32_t v = ring_v + (((2 * j + 1) % ST) * L::kTile >> 4);
+#pragma unroll
+      for (int i = 0; i < kTcKeys / 16; ++i)
+        tc_mma_ts(leader, tmem + L::kOut + t * 128, tmem + L::kScores + b * 128 + i * 8, v + (i * 2048 >> 4), kUmmaHi,
+                  idesc_o, i != 0 ? 1u : (uint32_t)(j != 0));
+      tc_commit_if(leader, pv_done + 8 * t);
+    };
+    bool ok = n > 0 && warp_wait(q_full, 0, a.status, kDevTimeoutFull) && wait_full(0);
+    if (ok) {
+      for (int t = 0; t < tiles_here; ++t) scores(t, t, 0);
+      release(0);
+    }
+    for (int j = 0; j < n && ok; ++j) {
+      const bool more = j + 1 < n;
+      if (MT == 1) {
+        // the buffer's P was consumed by the product issued before this one
+        if (more) {
+          if (!(ok = wait_full(2 * j + 2))) break;
+          scores(0, (j + 1) & 1, j + 1);
+          release(2 * j + 2);
+        }
+        ok = wait_full(2 * j + 1) && warp_wait(p_full + 8 * (j & 1), (j >> 1) & 1, a.status, kDevTimeoutAcc);
+        if (!ok) break;
+        tc_fence_after();
+        outputs(0, j & 1, j);
+        release(2 * j + 1);
+      } else {
+        if (!(ok = wait_full(2 * j + 1))) break;
+        for (int t = 0; t < tiles_here; ++t) {
+          if (!(ok = warp_wait(p_full + 8 * t, j & 1, a.status, kDevTimeoutAcc))) break;
           tc_fence_after();
-          outputs(0, j & 1, j);
-          release(2 * j + 1);
-        } else {
-          if (!(ok = wait_full(2 * j + 1))) break;
-          for (int t = 0; t < tiles_here; ++t) {
-            if (!(ok = warp_wait(p_full + 8 * t, j & 1, a.status, kDevTimeoutAcc))) break;
-            tc_fence_after();
-            outputs(t, t, j);
-            if (t + 1 == tiles_here) release(2 * j + 1);
-            if (more) {
-              if (t == 0 && !(ok = wait_full(2 * j + 2))) break;
-              scores(t, t, j + 1);
-              if (t + 1 == tiles_here) release(2 * j + 2);
-            }
+          outputs(t, t, j);
+          if (t + 1 == tiles_here) release(2 * j + 1);
+          if (more) {
+            if (t == 0 && !(ok = wait_full(2 * j + 2))) break;
+            scores(t, t, j + 1);
+            if (t + 1 == tiles_here) release(2 * j + 2);
           }
         }
       }

@@ -175,7 +175,8 @@ void run_qk_norm_rope(const ls_qk_norm_args& p, cudaStream_t stream) {
 // ------------------------------------------------------------ prefix attention
 // How a call is cut into units: a function of its sizes and types alone.
 struct PrefixPlan {
-  int tc_tiles;     // 128-row tiles a CTA of the tcgen05 kernel takes; 0: the unit kernel does the prefix
+  int tc_tiles;     // 128-row tiles a CTA of the tcgen05 kernel takes; 0: the unit kernel does everything
+  bool own;         // it takes one request's rows and also does that request's own positions
   int prefix_parts, prefix_chunk, suffix_parts, suffix_chunk, prefix_tiles, suffix_tiles;
   size_t o_bytes, ml_bytes, total;
 };
@@ -199,17 +200,29 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
   PrefixPlan p{};
   const int G = nh / nkv;
   const long rows = (long)n_tokens * G;
-  p.tc_tiles = split_q || rows <= 16 || prefix_len == 0 ? 0 : rows > kTcRows ? 2 : 1;
-  p.suffix_tiles = cdiv((long)std::min(max_new, n_tokens) * G, 16);
-  if (p.tc_tiles) {
-    p.prefix_tiles = cdiv(rows, kTcRows * p.tc_tiles);
-    cut((long)p.prefix_tiles * nkv, prefix_len, sms, kTcKeys, kTcKeys, p.prefix_parts, p.prefix_chunk);
+  const long most_new = std::min(max_new, n_tokens);
+  // Requests that bring whole tiles of rows on average do not need each other
+  // to fill one: their own positions then follow the prefix in the same unit.
+  p.own = !split_q && rows >= (long)kTcRows * n_requests;
+  p.suffix_tiles = cdiv(most_new * G, 16);
+  if (p.own) {
+    p.tc_tiles = most_new * G > kTcRows ? 2 : 1;
+    p.prefix_tiles = cdiv(most_new * G, kTcRows * p.tc_tiles);
+    const long units = (rows / (kTcRows * p.tc_tiles) + 1) * nkv;
+    cut(units, prefix_len, sms, 2 * kTcKeys, kTcKeys, p.prefix_parts, p.prefix_chunk);
   } else {
-    p.prefix_tiles = cdiv(rows, 16);
-    cut((long)p.prefix_tiles * nkv, prefix_len, 2L * sms, 256, 64, p.prefix_parts, p.prefix_chunk);
+    p.tc_tiles = split_q || rows <= 16 || prefix_len == 0 ? 0 : rows > kTcRows ? 2 : 1;
+    if (p.tc_tiles) {
+      p.prefix_tiles = cdiv(rows, kTcRows * p.tc_tiles);
+      cut((long)p.prefix_tiles * nkv, prefix_len, sms, kTcKeys, kTcKeys, p.prefix_parts, p.prefix_chunk);
+    } else {
+      p.prefix_tiles = cdiv(rows, 16);
+      cut((long)p.prefix_tiles * nkv, prefix_len, 2L * sms, 256, 64, p.prefix_parts, p.prefix_chunk);
+    }
+    cut((long)p.suffix_tiles * nkv * n_requests, max_len, 8L * sms, 256, 64, p.suffix_parts, p.suffix_chunk);
   }
-  cut((long)p.suffix_tiles * nkv * n_requests, max_len, 8L * sms, 256, 64, p.suffix_parts, p.suffix_chunk);
-  const size_t part_rows = (size_t)(p.prefix_parts + p.suffix_parts) * n_tokens * nh;
+  const bool direct = p.own && p.prefix_parts <= 1;   // whole results, no parts to keep
+  const size_t part_rows = direct ? 0 : (size_t)(p.prefix_parts + p.suffix_parts) * n_tokens * nh;
   p.o_bytes = round256(part_rows * hd * sizeof(float));
   p.ml_bytes = round256(part_rows * sizeof(float2));
   p.total = p.o_bytes + p.ml_bytes;
@@ -220,7 +233,18 @@ template <int HD, typename C, int MT>
 void launch_tc(const PrefixAttnArgs& a, cudaStream_t stream) {
   const size_t smem = TcLayout<HD, MT>::kSmem;
   allow_smem<prefix_tc_kernel<HD, C, MT>>(smem);
-  launch(prefix_tc_kernel<HD, C, MT>, dim3((unsigned)(a.prefix_tiles * a.nkv * a.prefix_parts)),
+  // the register hand-over inside the kernel waits for good if the launch holds less than it shares out
+  static const int regs = [] {
+    cudaFuncAttributes attr = {};
+    CK(cudaFuncGetAttributes(&attr, prefix_tc_kernel<HD, C, MT>));
+    return attr.numRegs;
+  }();
+  constexpr int kNeed = TcLayout<HD, MT>::kLaunchRegs;
+  REQUIRE(regs >= kNeed, LS_ECUDA,
+          "prefix attention: built with " + std::to_string(regs) + " registers a thread, fewer than it shares out");
+  const long units = (long)a.prefix_tiles * a.nkv * std::max(1, a.prefix_parts) * (a.own ? a.n_requests : 1);
+  REQUIRE(units <= INT32_MAX, LS_EINVAL, "prefix attention: too many units for one launch");
+  launch(prefix_tc_kernel<HD, C, MT>, dim3((unsigned)units),
          dim3(TcLayout<HD, MT>::kThreads), smem, stream, false, a);
 }
 
@@ -230,6 +254,7 @@ void launch_prefix(PrefixAttnArgs a, int tc_tiles, cudaStream_t stream) {
     if (tc_tiles == 1) launch_tc<HD, C, 1>(a, stream);
     if (tc_tiles == 2) launch_tc<HD, C, 2>(a, stream);
   }
+  if (a.direct) return;
   a.prefix_units = tc_tiles == 0;
   const long units = (a.prefix_units ? (long)a.prefix_parts * a.prefix_tiles * a.nkv : 0) +
                      (long)a.suffix_parts * a.suffix_tiles * a.nkv * a.n_requests;
@@ -319,6 +344,8 @@ void run_prefix_attention(const ls_prefix_attention_args& p, cudaStream_t stream
   a.suffix_chunk = plan.suffix_chunk;
   a.prefix_tiles = plan.prefix_tiles;
   a.suffix_tiles = plan.suffix_tiles;
+  a.own = plan.own;
+  a.direct = plan.own && plan.prefix_parts <= 1;
   a.status = p.status;
   if (p.q_type == LS_BF16) launch_prefix<bf16, bf16, 1>(a, p.head_dim, plan.tc_tiles, stream);
   else if (p.q_type == LS_F16) launch_prefix<__half, __half, 1>(a, p.head_dim, plan.tc_tiles, stream);

@@ -181,6 +181,43 @@ def test_tokens_that_see_nothing_and_padding_get_zeros():
     status.check()
 
 
+@pytest.mark.parametrize("kind,cache", ALL)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("counts,lens,prefix,nh,nkv", [
+    ([64], [64], 300, 2, 1),                      # one tile of 128 rows
+    ([64, 64], [64, 190], 0, 4, 2),               # no prefix
+    ([200], [200], 9000, 2, 1),                   # few rows, long prefix: several key ranges
+    ([300, 1, 40], [300, 1, 129], 513, 9, 3),     # requests of one and of several tiles
+    ([130, 140], [128, 100], 0, 4, 4),            # more new tokens than positions: the first see nothing
+    ([256, 257], [256, 513], 127, 1, 1),
+])
+def test_prompts_behind_a_prefix(counts, lens, prefix, nh, nkv, hd, kind, cache):
+    c = make(counts, lens, prefix, 16, nh, nkv, hd, kind, cache, seed=sum(counts) + prefix, pad=3, fill=float("nan"))
+    out = call(c, 16)
+    near(out, c, 16, kind, cache)
+    assert not bool(out[-3:].any())
+
+
+@pytest.mark.parametrize("kind,cache", [("bf16", "bf16"), ("f16", "f16")])
+def test_nan_in_the_prefix_reaches_every_row_and_only_its_dimensions(kind, cache):
+    """A NaN key spoils all rows of its kv head; an infinite value only its own dimension."""
+    for counts, lens, nh in (([1] * 30, [4] * 30, 2), ([1, 1], [4, 4], 2), ([100, 120], [100, 120], 4)):
+        c = make(counts, lens, 700, 16, nh, 2, 64, kind, cache, seed=12)
+        k, v, table = c[1], c[2], c[3]
+        slots = table.long().repeat_interleave(16) * 16 + torch.arange(16).repeat(len(table))
+        for pos in (3, 130, 255, 699):
+            bad = (c[0], k.clone(), v.clone(), *c[3:])
+            bad[1][slots[pos], 1] = float("nan")
+            bad[2][slots[pos], 0, 5] = float("inf")
+            out = call(bad, 16).float()
+            G = nh // 2
+            assert bool(torch.isnan(out[:, G:]).all())
+            assert bool(torch.isinf(out[:, :G, 5]).all())
+            rest = torch.ones(64, dtype=torch.bool)
+            rest[5] = False
+            assert bool(torch.isfinite(out[:, :G][..., rest.cuda()]).all())
+
+
 @pytest.mark.parametrize("kind,cache", [("bf16", "bf16"), ("f32", "f16")])
 def test_strides_scale_and_bounds(kind, cache):
     """q inside packed rows, pools interleaved, a wide table, generous bounds, another scale."""
@@ -240,6 +277,20 @@ def test_what_only_the_gpu_sees_is_skipped_and_reported(fault):
         assert torch.equal(out[[0, 3]], good[[0, 3]])       # the other requests are whole
     if fault in ("length", "tokens"):
         assert not bool(out[1:3].any())
+
+
+def test_a_bad_request_among_prompts_gets_zeros():
+    from loopspec_b200 import _lib
+    from loopspec_b200.status import DeviceStatus
+    c = make([150, 200, 170], [150, 260, 170], 300, 16, 4, 4, 64, "bf16", "bf16", seed=2)
+    good = call(c, 16)
+    c[6][1] = 5000
+    status = DeviceStatus("cuda")
+    out = call(c, 16, status=status)
+    with pytest.raises(_lib.EngineError):
+        status.check()
+    assert torch.equal(out[:150], good[:150]) and torch.equal(out[350:], good[350:])
+    assert not bool(out[150:350].any())
 
 
 def test_slots_past_32_bit_offsets():
