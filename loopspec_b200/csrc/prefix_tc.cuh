@@ -55,7 +55,7 @@ struct TcLayout {
   static constexpr int kMaxBuffers = MT == 1 ? 2 : 1;      // see the softmax warps
   static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 1 + 1;
   static constexpr int kSmem = MT * kTile + kStages * kTile + kMaxBuffers * MT * 2 * kTcRows * 4 + kBars * 8 + 8 * 4 + 16;
-  static constexpr int kPoly = 3;                          // eighths of the exponentials on the FMA units
+  static constexpr int kPoly = 2;                          // eighths of the exponentials on the FMA units
   static constexpr uint32_t kScores = 0, kOut = 256;       // tensor memory columns
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 };
@@ -207,9 +207,13 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
                       __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u)));
 }
 
-// A whole warp's wait: all lanes agree on the outcome, so none leaves the others in a collective.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* err, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+// Wait unless an earlier wait timed out. A warp whose wait times out does not
+// leave its loop: it waits no more and goes on over what is there, so that no
+// lane and no warp is missing from a collective or a barrier of the others; the
+// status word tells. (A vote on the outcome would cost 31 cycles a wait, a
+// barrier that is ready 13.)
+__device__ __forceinline__ void wait_on(bool& ok, uint32_t bar, uint32_t parity, int* err, int code) {
+  if (ok && !mbar_try_wait(bar, parity)) ok = mbar_wait(bar, parity, err, code);
 }
 
 // Arrive on `bar` once this thread's cp.async copies so far have landed.
@@ -382,15 +386,13 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
       const int see_least = __reduce_min_sync(0xffffffffu, see);
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      // After a wait that timed out the warp waits no more, but goes on through
-      // the barriers that it shares with its other half.
       for (int j = 0; j < n; ++j) {
         const int b = MT == 1 ? j & 1 : t;
         const uint32_t ph = (MT == 1 ? j >> 1 : j) & 1;
         // keys of this tile that the row sees, counted from this thread's first
         int left = (j < na ? ka1 - ka0 - j * kTcKeys : see - (j - na) * kTcKeys) - half * 64;
         const bool cut = j < na ? j == na - 1 : see_least - (j - na) * kTcKeys < kTcKeys;
-        ok = ok && warp_wait(s_full + 8 * b, ph, a.status, kDevTimeoutAcc);
+        wait_on(ok, s_full + 8 * b, ph, a.status, kDevTimeoutAcc);
         tc_fence_after();
         const uint32_t sc = lanes + L::kScores + b * 128;
         uint32_t s[64];
@@ -424,7 +426,7 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
           if (move) m = top;
           l *= keep;
           if (j > 0) {
-            ok = ok && warp_wait(pv_done + 8 * t, (j - 1) & 1, a.status, kDevTimeoutAcc);
+            wait_on(ok, pv_done + 8 * t, (j - 1) & 1, a.status, kDevTimeoutAcc);
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < HD / 2; c += 16) {
@@ -467,9 +469,9 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
         if (lane == 0) mbar_arrive(p_full + 8 * b);
       }
       // join the two halves' sums; a wait that timed out leaves zeros
-      bool have = n > 0 && ok;
-      if (have) have = warp_wait(pv_done + 8 * t, (n - 1) & 1, a.status, kDevTimeoutAcc);
-      if (a.own) have = warp_wait(noted, 0, a.status, kDevTimeoutAcc) && have;
+      if (n > 0) wait_on(ok, pv_done + 8 * t, (n - 1) & 1, a.status, kDevTimeoutAcc);
+      if (a.own) wait_on(ok, noted, 0, a.status, kDevTimeoutAcc);
+      const bool have = n > 0 && ok;
       tc_fence_after();
       float* row_sum = s_max + ((MT == 1 ? n & 1 : t) * 2) * kTcRows + r;
       row_sum[half * kTcRows] = l;
@@ -541,6 +543,7 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
       for (int q = 0; q < 4; ++q) next[q] = pos + 32 * q < end ? table[(pos + 32 * q) >> a.page_shift] : 0;
     };
     const int first = warp - L::kProducer;
+    bool ok = true;
     look_up(first);
     for (int i = first; i < 2 * n; i += L::kProducers) {
       const int j = i >> 1, st = i % ST;
@@ -572,7 +575,7 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
         }
         __syncwarp();
       }
-      if (i >= ST && !warp_wait(empty0 + 8 * st, (i / ST - 1) & 1, a.status, kDevTimeoutEmpty)) break;
+      if (i >= ST) wait_on(ok, empty0 + 8 * st, (i / ST - 1) & 1, a.status, kDevTimeoutEmpty);
       const uint32_t dst = dst0 + st * L::kTile;
       const C* src = is_v ? vp : kp;
 #pragma unroll
@@ -597,11 +600,10 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
     const uint32_t leader = elect_one();
     const uint32_t ring_k = umma_lo(smem_u32(s_ring), 0), ring_v = umma_lo(smem_u32(s_ring), kBlock),
                    q0 = umma_lo(smem_u32(s_q), 0);
+    bool ok = n > 0;
     auto wait_full = [&](int i) {
-      const bool ok = warp_wait(full0 + 8 * (i % ST), (i / ST) & 1, a.status, kDevTimeoutFull);
+      wait_on(ok, full0 + 8 * (i % ST), (i / ST) & 1, a.status, kDevTimeoutFull);
       fence_proxy_async();                         // copies came by the generic proxy; the products read by the async one
-      tc_fence_after();
-      return ok;
     };
     auto release = [&](int i) {                    // copy i's stage, if another copy will want it
       if (i + ST < 2 * n) tc_commit_if(leader, empty0 + 8 * (i % ST));
@@ -623,37 +625,32 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
                   idesc_o, i != 0 ? 1u : (uint32_t)(j != 0));
       tc_commit_if(leader, pv_done + 8 * t);
     };
-    bool ok = n > 0 && warp_wait(q_full, 0, a.status, kDevTimeoutFull) && wait_full(0);
-    if (ok) {
+    if (n > 0) {
+      wait_on(ok, q_full, 0, a.status, kDevTimeoutFull);
+      wait_full(0);
+      tc_fence_after();
       for (int t = 0; t < tiles_here; ++t) scores(t, t, 0);
       release(0);
     }
-    for (int j = 0; j < n && ok; ++j) {
+    for (int j = 0; j < n; ++j) {
       const bool more = j + 1 < n;
-      if (MT == 1) {
+      if (more) wait_full(2 * j + 2);
+      if (MT == 1 && more) {
         // the buffer's P was consumed by the product issued before this one
-        if (more) {
-          if (!(ok = wait_full(2 * j + 2))) break;
-          scores(0, (j + 1) & 1, j + 1);
-          release(2 * j + 2);
-        }
-        ok = wait_full(2 * j + 1) && warp_wait(p_full + 8 * (j & 1), (j >> 1) & 1, a.status, kDevTimeoutAcc);
-        if (!ok) break;
         tc_fence_after();
-        outputs(0, j & 1, j);
-        release(2 * j + 1);
-      } else {
-        if (!(ok = wait_full(2 * j + 1))) break;
-        for (int t = 0; t < tiles_here; ++t) {
-          if (!(ok = warp_wait(p_full + 8 * t, j & 1, a.status, kDevTimeoutAcc))) break;
-          tc_fence_after();
-          outputs(t, t, j);
-          if (t + 1 == tiles_here) release(2 * j + 1);
-          if (more) {
-            if (t == 0 && !(ok = wait_full(2 * j + 2))) break;
-            scores(t, t, j + 1);
-            if (t + 1 == tiles_here) release(2 * j + 2);
-          }
+        scores(0, (j + 1) & 1, j + 1);
+        release(2 * j + 2);
+      }
+      wait_full(2 * j + 1);
+      for (int t = 0; t < tiles_here; ++t) {
+        const int b = MT == 1 ? j & 1 : t;
+        wait_on(ok, p_full + 8 * b, (MT == 1 ? j >> 1 : j) & 1, a.status, kDevTimeoutAcc);
+        tc_fence_after();
+        outputs(t, b, j);
+        if (t + 1 == tiles_here) release(2 * j + 1);
+        if (MT == 2 && more) {
+          scores(t, t, j + 1);
+          if (t + 1 == tiles_here) release(2 * j + 2);
         }
       }
     }
