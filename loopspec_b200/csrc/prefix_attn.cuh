@@ -484,45 +484,62 @@ __device__ __forceinline__ void store4(__half* p, float4 v) {
 }
 
 constexpr int kJoinThreads = 128;
+constexpr int kJoinBatch = 8;
 
-// Join the parts of each row: HD/4 threads a row, 4 columns each. grid: rows
-// of (t, h) over kJoinThreads/(HD/4) a CTA. Tokens past token_start[R] and
-// those of a request that was skipped get zeros, as do rows that see nothing.
+// Join the parts of each row: HD/4 threads a row, 4 columns each. grid: (token,
+// heads over kJoinThreads/(HD/4)). Tokens past token_start[R] and those of a
+// request that was skipped get zeros, as do rows that see nothing. Bound: the
+// latency of two loads (lengths; parts, all at once) after the parts are there.
 template <int HD, typename Q>
 __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArgs a) {
   constexpr int TPR = HD / 4;
-  pdl_wait();
-  const long row = (long)blockIdx.x * (kJoinThreads / TPR) + threadIdx.x / TPR;
-  if (row >= (long)a.n_tokens * a.nh) return;
-  const int c = (threadIdx.x % TPR) * 4;
-  const int t = (int)(row / a.nh), h = (int)(row - (long)t * a.nh);
-  // the token's request: the last i with token_start[i] <= t
-  int lo = 0, hi = a.n_requests;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.token_start[mid] <= t) lo = mid;
-    else hi = mid;
+  const int t = blockIdx.x;
+  // whether a valid request holds the token: written by nobody ahead of this kernel
+  bool mine = false;
+  for (int i = threadIdx.x; i < a.n_requests; i += kJoinThreads) {
+    const int start = a.token_start[i], end = a.token_start[i + 1], len = a.lens[i];
+    mine |= t >= start && t < end && start >= 0 && end - start <= a.max_new && end <= a.n_tokens && len >= 0 &&
+            len <= a.max_len;
   }
-  const int start = a.token_start[lo], n = a.token_start[lo + 1] - start, len = a.lens[lo];
-  const bool ok = start >= 0 && n >= 0 && n <= a.max_new && start <= a.n_tokens - n && len >= 0 &&
-                  len <= a.max_len && t >= start && t < start + n;
+  const bool ok = __syncthreads_or(mine);
+  pdl_wait();
+  const int h = blockIdx.y * (kJoinThreads / TPR) + threadIdx.x / TPR;
+  if (h >= a.nh) return;
+  const int c = (threadIdx.x % TPR) * 4;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (ok) {
     const int parts = a.prefix_parts + a.suffix_parts;
-    const long stride = (long)a.n_tokens * a.nh;
-    float mm = -INFINITY;
-    for (int p = 0; p < parts; ++p) mm = fmaxf(mm, a.part_ml[p * stride + row].x);
-    const float base = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f;
-    for (int p = 0; p < parts; ++p) {
-      const float2 ml = a.part_ml[p * stride + row];
-      const float w = exp2_fast(ml.x - base);
-      const float4 v = *reinterpret_cast<const float4*>(a.part_o + (p * stride + row) * HD + c);
-      ll += ml.y * w;
-      acc.x += v.x * w;
-      acc.y += v.y * w;
-      acc.z += v.z * w;
-      acc.w += v.w * w;
+    const long stride = (long)a.n_tokens * a.nh, row = (long)t * a.nh + h;
+    float mm = -INFINITY, ll = 0.f;
+    for (int p0 = 0; p0 < parts; p0 += kJoinBatch) {
+      float2 ml[kJoinBatch];
+      float4 v[kJoinBatch];
+#pragma unroll
+      for (int p = 0; p < kJoinBatch; ++p) {
+        const bool in = p0 + p < parts;
+        const long at = (in ? p0 + p : p0) * stride + row;
+        ml[p] = __ldcg(a.part_ml + at);
+        v[p] = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * HD + c));
+        if (!in) ml[p].x = -INFINITY;
+      }
+      float top = mm;
+#pragma unroll
+      for (int p = 0; p < kJoinBatch; ++p) top = fmaxf(top, ml[p].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float keep = exp2_fast(mm - base);
+      mm = top;
+      ll *= keep;
+      acc = make_float4(acc.x * keep, acc.y * keep, acc.z * keep, acc.w * keep);
+#pragma unroll
+      for (int p = 0; p < kJoinBatch; ++p) {
+        const float w = exp2_fast(ml[p].x - base);
+        if (p0 + p >= parts) break;
+        ll += ml[p].y * w;
+        acc.x += v[p].x * w;
+        acc.y += v[p].y * w;
+        acc.z += v[p].z * w;
+        acc.w += v[p].w * w;
+      }
     }
     const float inv = ll == 0.f ? 0.f : 1.f / ll;
     acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);

@@ -363,14 +363,20 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
     {
       unsigned char* dst = s_q + t * L::kTile;
       const C* q = static_cast<const C*>(a.q);
-      for (int i = threadIdx.x & 255; i < kTcRows * CH; i += 256) {
-        const int r = i / CH, c = i % CH, rr = row0 + t * kTcRows + r;
-        uint4 v = make_uint4(0, 0, 0, 0);
+      uint4 v[CH / 2];                               // all of them on their way at once
+#pragma unroll
+      for (int k = 0; k < CH / 2; ++k) {
+        const int i = (threadIdx.x & 255) + 256 * k, r = i / CH, c = i % CH, rr = row0 + t * kTcRows + r;
+        v[k] = make_uint4(0, 0, 0, 0);
         if (rr < rows) {
           const int tok = rr / G, h = g * G + rr - tok * G;
-          v = *reinterpret_cast<const uint4*>(q + (long)(start + tok) * a.q_stride + (long)h * HD + c * 8);
+          v[k] = *reinterpret_cast<const uint4*>(q + (long)(start + tok) * a.q_stride + (long)h * HD + c * 8);
         }
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+      }
+#pragma unroll
+      for (int k = 0; k < CH / 2; ++k) {
+        const int i = (threadIdx.x & 255) + 256 * k, r = i / CH, c = i % CH;
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
       }
       fence_proxy_async();
       __syncwarp();
@@ -482,17 +488,25 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
       const long at = ((long)part * a.n_tokens + tok) * a.nh + h;
       if (!a.direct && rr < rows && half == 0)
         a.part_ml[at] = have ? make_float2(m * a.scale_log2, l) : make_float2(-INFINITY, 0.f);
+      // Parts leave by a patch of the row tile's queries, which are done with:
+      // a warp's rows by CW columns, 16-byte chunks swizzled, so that it stores
+      // whole rows of 4 CW bytes (a thread storing its own row by itself
+      // touches 32 lines with every instruction: 8000 cycles for the tile).
+      constexpr int CW = HD / 4, CPR = CW / 4;
+      unsigned char* patch = s_q + t * L::kTile + (half * 4 + quarter) * (32 * CW * 4);
+      auto place = [&](int row, int chunk) {
+        return reinterpret_cast<float4*>(patch + row * (CW * 4) + ((chunk ^ (CPR == 8 ? row & 7 : (row >> 1) & 3)) << 4));
+      };
 #pragma unroll 1
       for (int c = 0; c < HD / 2; c += 16) {
         uint32_t v[16];
         tmem_ld_x16(out + c, v);
         tmem_ld_wait();
-        if (rr >= rows) continue;
         float f[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[i] = have ? __uint_as_float(v[i]) * inv : 0.f;
         const int d = half * (HD / 2) + c;
-        if (a.own && have) {                       // terms left out of the products
+        if (a.own && have && rr < rows) {            // terms left out of the products
           for (int w = 0; w < 8; ++w)
             for (uint32_t bits = s_bad[w]; bits; bits &= bits - 1) {
               const int pos = see_first + w * 32 + __ffs(bits) - 1;
@@ -507,14 +521,25 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
             }
         }
         if (a.direct) {
-          C* dst = static_cast<C*>(a.out) + (long)tok * a.out_stride + (long)h * HD + d;
-          store8(dst, *reinterpret_cast<float(*)[8]>(f));
-          store8(dst + 8, *reinterpret_cast<float(*)[8]>(f + 8));
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            store4(a.part_o + at * HD + d + i, make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]));
+          if (rr < rows) {
+            C* dst = static_cast<C*>(a.out) + (long)tok * a.out_stride + (long)h * HD + d;
+            store8(dst, *reinterpret_cast<float(*)[8]>(f));
+            store8(dst + 8, *reinterpret_cast<float(*)[8]>(f + 8));
+          }
+          continue;
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *place(lane, (c % CW) / 4 + i) = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+        if ((c + 16) % CW) continue;
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < CPR; ++k) {
+          const int row = k * (32 / CPR) + lane / CPR, chunk = lane % CPR;
+          const long to = __shfl_sync(0xffffffffu, at, row);
+          if (row0 + t * kTcRows + quarter * 32 + row < rows)
+            store4(a.part_o + to * HD + half * (HD / 2) + c + 16 - CW + chunk * 4, *place(row, chunk));
+        }
+        __syncwarp();
       }
       tc_fence_before();
     }

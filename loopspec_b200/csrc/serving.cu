@@ -266,8 +266,8 @@ void launch_prefix(PrefixAttnArgs a, int tc_tiles, cudaStream_t stream) {
            tc_tiles != 0, a);
   }
   const int per = kJoinThreads / (HD / 4);
-  launch(prefix_join_kernel<HD, Q>, dim3((unsigned)cdiv((long)a.n_tokens * a.nh, per)), dim3(kJoinThreads), 0,
-         stream, true, a);
+  launch(prefix_join_kernel<HD, Q>, dim3((unsigned)a.n_tokens, (unsigned)cdiv(a.nh, per)), dim3(kJoinThreads), 0,
+         stream, tc_tiles != 0 || units > 0, a);   // early only behind kernels of this call
 }
 
 template <typename Q, typename C, int TERMS>
