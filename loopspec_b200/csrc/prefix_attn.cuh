@@ -12,13 +12,21 @@
 // token), each request's own positions are another, and a last pass joins
 // them.
 //
-// This file: the unit kernel. A unit is (row tile of 16, kv head, key range)
-// of the prefix or of one request. Four warps split the range's keys, 16 at a
-// time, each through its own ring of cp.async stages (no CTA barrier in the
-// loop), S = q K^T and O += P V on mma.sync m16n8k16 with fp32 accumulators;
-// the G query heads of a kv head and the request's tokens are the rows, so a
-// K/V tile is used by all of them. The warps join in shared memory, and the
-// unit writes its (m, l, o) in fp32.
+// This file: the stream kernel, for few query rows a kv head, and the joining
+// pass. A unit is (row tile, kv head, key range) of the prefix or of one
+// request; the G query heads of a kv head and the request's tokens are the
+// rows, so a K/V tile is used by all of them. Each warp works by itself through
+// its units, 16 keys at a time, as one stream, while the next tiles, of this
+// unit or the next one, are on their way into the warp's ring by cp.async (a
+// CTA for each unit, with its lookups, loads and joins one after the other,
+// took 8500 cycles a unit beside the 1500 a tile).
+// The products run on mma.sync m16n8k16, fp32 accumulators, with the keys as
+// M: S^T = K q^T (16 keys by 8 rows) and O^T += V^T P^T. A decode step has one
+// to eight rows a kv head; as N they cost half the products and registers that
+// they cost as M. A row tile is 8 RT rows, whose products share the fragments
+// of K and V. A unit's (m, l, o) goes out in
+// fp32; O is rescaled only when a row's maximum has grown by more than 2^8 since
+// its reference was set (the reference cancels in o / l).
 //
 // Types: bf16 or f16 K/V. q of the cache's type enters the product exactly.
 // fp32 q enters as a sum of TERMS values of the cache's type, each the
@@ -55,6 +63,7 @@ struct PrefixAttnArgs {
   int n_requests, n_tokens, max_new, max_len;
   int page_shift;
   int nh, nkv;
+  uint32_t g_magic;         // ceil(2^32 / (nh / nkv)), see div_by
   float scale_log2;         // scale * log2(e): scores in powers of two
   void* out;
   long out_stride;
@@ -62,9 +71,9 @@ struct PrefixAttnArgs {
   float* part_o;
   float2* part_ml;
   int prefix_parts, prefix_chunk;    // key ranges of the prefix, positions each
-  int suffix_parts, suffix_chunk;
-  int prefix_tiles, suffix_tiles;    // row tiles of 16 (prefix: of its own kernel's rows)
-  bool prefix_units;                 // the unit kernel also does the prefix
+  int suffix_parts, suffix_chunk;    // ... of max_len own positions
+  int prefix_tiles, suffix_tiles;    // row tiles, of their kernels' rows
+  bool prefix_units, suffix_units;   // what a launch of the stream kernel does
   bool own, direct;                  // tcgen05 kernel: rows of one request and its own positions; whole results
   int* status;
 };
@@ -72,28 +81,21 @@ struct PrefixAttnArgs {
 constexpr int kUnitThreads = 128;
 constexpr int kUnitKeys = 16;      // keys of a warp's stage
 constexpr int kUnitWarps = kUnitThreads / 32;
-// Stages of a warp's ring and CTAs an SM: 16-bit queries of 128 take 166
-// registers a thread, so a third CTA fits beside two when the rings shrink to
-// two stages (one copy in flight a warp, 12 warps); fp32 queries hold two or
-// three terms of q and leave room for two CTAs with three stages.
-template <int HD, int TERMS>
-__host__ __device__ constexpr int unit_stages() { return HD == 128 && TERMS == 1 ? 2 : 3; }
-template <int HD, int TERMS>
-__host__ __device__ constexpr int unit_ctas() { return HD == 128 ? (TERMS == 1 ? 3 : 2) : TERMS == 3 ? 3 : 4; }
+// CTAs an SM by the registers that q (TERMS x RT) and O (RT) take, and the
+// stages of a warp's ring that this leaves shared memory for.
+template <int HD, int TERMS, int RT>
+__host__ __device__ constexpr int unit_ctas() {
+  return HD == 128 ? (TERMS * RT <= 3 && RT <= 2 ? 3 : 2) : (TERMS * RT <= 4 && RT <= 2 ? 4 : 3);
+}
+template <int HD, int TERMS, int RT>
+__host__ __device__ constexpr int unit_stages() { return unit_ctas<HD, TERMS, RT>() >= (HD == 128 ? 3 : 4) ? 2 : 3; }
 
 template <int HD>
 __host__ __device__ constexpr int unit_row_bytes() { return HD * 2 + 16; }   // padded: fragment reads hit distinct banks
 template <int HD>
 __host__ __device__ constexpr int unit_stage_bytes() { return 2 * kUnitKeys * unit_row_bytes<HD>(); }
-template <int HD, int TERMS>
-constexpr size_t unit_smem_bytes() { return (size_t)kUnitWarps * unit_stages<HD, TERMS>() * unit_stage_bytes<HD>(); }
-
-// Joining the warps reuses the rings: kUnitWarps x 16 rows of HD floats, padded
-// so that the 8 rows a warp stores at once lie in different banks.
-template <int HD>
-__host__ __device__ constexpr int unit_join_row() { return HD + 8; }
-static_assert(unit_smem_bytes<64, 1>() >= sizeof(float) * kUnitWarps * 16 * unit_join_row<64>(), "join buffer");
-static_assert(unit_smem_bytes<128, 1>() >= sizeof(float) * kUnitWarps * 16 * unit_join_row<128>(), "join buffer");
+template <int HD, int TERMS, int RT>
+constexpr size_t unit_smem_bytes() { return (size_t)kUnitWarps * unit_stages<HD, TERMS, RT>() * unit_stage_bytes<HD>(); }
 
 // Two fp32 values as a packed pair of the cache's type, lower index in the low half.
 __device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) { return pack_bf16(a, b); }
@@ -144,6 +146,20 @@ __device__ __forceinline__ float exp2_fast(float x) {   // ex2.approx: 2 ulp; ex
   return y;
 }
 
+// The transpose of an 8 x 8 tile of 16-bit values, two a lane.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+  return d;
+}
+
+// r / G by a multiplication: `magic` is ceil(2^32 / G), the quotient at most one too large for r < 2^31.
+__device__ __forceinline__ int div_by(int r, int G, uint32_t magic) {
+  if (G == 1) return r;
+  const int q = (int)__umulhi((uint32_t)r, magic);
+  return q * G > r ? q - 1 : q;
+}
+
 // A request's token range and own length; false (and the status word) when they are out of bounds.
 __device__ __forceinline__ bool request_range(const PrefixAttnArgs& a, int i, int& start, int& n, int& len) {
   start = a.token_start[i];
@@ -165,6 +181,8 @@ __device__ __forceinline__ float2 load2(const __half* p) {
   return unpack2(*reinterpret_cast<const uint32_t*>(p), __half());
 }
 
+constexpr float kGrow = 8.f;   // log2 growth of a row's maximum that moves its reference
+
 // Whether a warp's 16 V rows in shared memory hold a NaN or infinity (exponent bits all set).
 template <int HD, typename C>
 __device__ __forceinline__ bool any_not_finite(const unsigned char* vb, int lane) {
@@ -177,302 +195,383 @@ __device__ __forceinline__ bool any_not_finite(const unsigned char* vb, int lane
   return __any_sync(0xffffffffu, found);
 }
 
-// O += P V over one stage without the tensor cores, each row adding only the positions it sees.
-template <int HD, typename C>
-__device__ __forceinline__ void add_by_weight(float (&o)[HD / 8][4], const float (&p)[2][4], const unsigned char* vb,
-                                           int key, int k1, const int (&see)[2], int lane) {
-  const int tig = lane & 3;
+// O^T += V^T P^T over one stage without the tensor cores, each row adding only the positions it sees.
+template <int HD, typename C, int RT>
+__device__ __forceinline__ void add_by_weight(float (&o)[RT][HD / 16][4], const float (&p)[RT][4],
+                                              const unsigned char* vb, int key, int k1, const int (&see)[RT][2],
+                                              int lane) {
+  const int gid = lane >> 2, tig = lane & 3;
 #pragma unroll 1
   for (int k = 0; k < kUnitKeys; ++k) {
-    const int from = (lane & ~3) | ((k & 7) >> 1);
+    const int from = (k & 7) * 4 + tig;
+    const C* row = reinterpret_cast<const C*>(vb + k * unit_row_bytes<HD>());
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float even = k < 8 ? p[0][2 * e] : p[1][2 * e], odd = k < 8 ? p[0][2 * e + 1] : p[1][2 * e + 1];
-      const float w = __shfl_sync(0xffffffffu, k & 1 ? odd : even, from);
-      if (key + k >= k1 || key + k >= see[e]) continue;
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int i = 0; i < HD / 8; ++i) {
-        const float2 v = unpack2(
-            *reinterpret_cast<const uint32_t*>(vb + k * unit_row_bytes<HD>() + (i * 8 + tig * 2) * 2), C());
-        o[i][2 * e] += w * v.x;
-        o[i][2 * e + 1] += w * v.y;
+      for (int e = 0; e < 2; ++e) {
+        const float w = __shfl_sync(0xffffffffu, k < 8 ? p[rt][e] : p[rt][2 + e], from);
+        if (key + k >= k1 || key + k >= see[rt][e]) continue;
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          o[rt][i][e] += w * (float)row[i * 16 + gid];
+          o[rt][i][2 + e] += w * (float)row[i * 16 + 8 + gid];
+        }
       }
-    }
   }
 }
 
-// grid: 1-D over prefix units (part, row tile, kv head), then suffix units
-// (part, row tile, kv head, request).
-template <int HD, typename Q, typename C, int TERMS>
-__global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS>()) prefix_unit_kernel(PrefixAttnArgs a) {
-  constexpr int ST = unit_stages<HD, TERMS>();
+constexpr int kBatchRequests = 256;    // looked up at a time; 32 x 8 for the search
+
+// Units of a batch of requests: their lengths, and where each one's units begin.
+struct UnitMap {
+  int first[kBatchRequests + 1];
+  int start[kBatchRequests], n[kBatchRequests], len[kBatchRequests];
+  int warp_sum[kUnitWarps];
+};
+
+// grid: any number of CTAs. Units with work are numbered one after the other --
+// the prefix's, then request by request: row tile, key range, kv head fastest --
+// and warp w of W takes units w, w + W, ...: a request's length decides how many
+// it has, so every CTA sums them up first (up to kBatchRequests at a time).
+template <int HD, typename Q, typename C, int TERMS, int RT>
+__global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) prefix_stream_kernel(PrefixAttnArgs a) {
+  constexpr int ST = unit_stages<HD, TERMS, RT>();
+  constexpr int ROWS = 8 * RT;                   // rows of a tile
   constexpr int RB = unit_row_bytes<HD>();
   constexpr int KS = HD / 16;
-  constexpr int NT = HD / 8;
+  constexpr int MT = HD / 16;                    // 16-dimension tiles of O^T
   constexpr int CH = HD / 8;                     // 16-byte chunks of a K/V row
   constexpr int LR = 32 / CH;                    // rows a warp copies at a time
+  constexpr unsigned kAll = 0xffffffffu;
   extern __shared__ __align__(16) unsigned char s_ring[];
-  __shared__ float s_ml[kUnitWarps][16][2];
+  __shared__ UnitMap s_map;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
   const int G = a.nh / a.nkv;
   const int mask = (1 << a.page_shift) - 1;
   pdl_launch_dependents();
-  // A prefix kernel ahead of this one runs on beside it; this grid is not done
-  // before that one is, which every way out of it below waits for
-
-  // the unit
-  unsigned u = blockIdx.x;
-  const unsigned n_prefix = a.prefix_units ? (unsigned)(a.prefix_parts * a.prefix_tiles * a.nkv) : 0;
-  const bool suffix = u >= n_prefix;
-  if (suffix) u -= n_prefix;
-  const unsigned parts = suffix ? a.suffix_parts : a.prefix_parts, tiles = suffix ? a.suffix_tiles : a.prefix_tiles;
-  const int part = (int)(u % parts);
-  u /= parts;
-  const int tile = (int)(u % tiles);
-  u /= tiles;
-  const int g = (int)(u % (unsigned)a.nkv), req = (int)(u / (unsigned)a.nkv);   // req 0 for the prefix
-  const int* table = suffix ? a.block_table + req * a.table_stride : a.prefix_table;
-  const int bound = suffix ? a.max_len : a.prefix_len;                          // positions the table covers
-  const int chunk = suffix ? a.suffix_chunk : a.prefix_chunk;
-  const int k0 = part * chunk;
-  const int first = k0 + warp * kUnitKeys, step = kUnitWarps * kUnitKeys;
-  // the block of key `key + lane`: loaded a step ahead of its copy, the first
-  // ones beside the request's length
-  auto block_of = [&](int key) {
-    return lane < kUnitKeys && key + lane < bound ? table[(key + lane) >> a.page_shift] : 0;
-  };
-  int block[ST - 1];
-#pragma unroll
-  for (int s = 0; s < ST - 1; ++s) block[s] = block_of(first + s * step);
-  int ahead = block_of(first + (ST - 1) * step);
-  int start = 0, n = a.n_tokens, len = a.prefix_len;
-  if (suffix && !request_range(a, req, start, n, len)) return pdl_wait();
-  const int rows = n * G;
-  if (tile * 16 >= rows) return pdl_wait();
-  const int seen0 = suffix ? len - n + 1 : len;                   // positions the first token sees
-  const int seen_by_all = seen0 + (suffix ? tile * 16 / G : 0);   // ... every row of the tile
-  const int k1 = min(len, k0 + chunk);
-  const int slot_part = suffix ? a.prefix_parts + part : part;
-
   unsigned char* ring = s_ring + (size_t)warp * ST * unit_stage_bytes<HD>();
-  const C* kp = static_cast<const C*>(a.k_pool) + (long)g * HD;
-  const C* vp = static_cast<const C*>(a.v_pool) + (long)g * HD;
-  // stage s <- keys [key, key + 16): rows past the range or with a bad block
-  // are filled with zeros, so what the pool holds there never enters a product
-  auto issue = [&](int key, int block, int s) {
-    unsigned char* dst = ring + s * unit_stage_bytes<HD>();
-    int slot = -1;
-    if (lane < kUnitKeys && key + lane < k1) {
-      const long sl = ((long)block << a.page_shift) + ((key + lane) & mask);
-      if (block < 0 || sl >= a.n_slots) atomicCAS(a.status, kDevOk, kDevBadIndex);
-      else slot = (int)sl;
-    }
-#pragma unroll
-    for (int i = 0; i < kUnitKeys / LR; ++i) {
-      const int r = i * LR + lane / CH, c = lane % CH;
-      const int sl = __shfl_sync(0xffffffffu, slot, r);
-      const long off = (long)max(sl, 0) * a.slot_stride + c * 8;
-      cp_async16(dst + r * RB + c * 16, kp + off, sl >= 0);
-      cp_async16(dst + (kUnitKeys + r) * RB + c * 16, vp + off, sl >= 0);
-    }
-  };
+  const int W = gridDim.x * kUnitWarps, w = warp * gridDim.x + blockIdx.x;
 
-  float o[NT][4];
+  for (int req0 = 0; req0 < (a.suffix_units ? a.n_requests : 1); req0 += kBatchRequests) {
+    const int n_prefix = a.prefix_units && req0 == 0 ? a.prefix_parts * a.prefix_tiles * a.nkv : 0;
+    const int n_req = a.suffix_units ? min(kBatchRequests, a.n_requests - req0) : 0;
+    int n_units = n_prefix;
+    if (n_req) {
+      __syncthreads();                           // the last batch's map is done with
+      constexpr int PER = kBatchRequests / kUnitThreads;
+      int count[PER], sum = 0;
 #pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      for (int k = 0; k < PER; ++k) {
+        const int i = threadIdx.x * PER + k;
+        count[k] = 0;
+        int start, n, len;
+        if (i < n_req && request_range(a, req0 + i, start, n, len)) {
+          s_map.start[i] = start;
+          s_map.n[i] = n;
+          s_map.len[i] = len;
+          count[k] = (n * G + ROWS - 1) / ROWS * ((len + a.suffix_chunk - 1) / a.suffix_chunk) * a.nkv;
+        }
+        sum += count[k];
+      }
+      int upto = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kAll, upto, o);
+        if (lane >= o) upto += v;
+      }
+      if (lane == 31) s_map.warp_sum[warp] = upto;
+      __syncthreads();
+      int at = n_prefix + upto - sum;
+#pragma unroll
+      for (int v = 0; v < kUnitWarps; ++v) {
+        if (v < warp) at += s_map.warp_sum[v];
+        n_units += s_map.warp_sum[v];
+      }
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        s_map.first[threadIdx.x * PER + k] = at;
+        at += count[k];
+      }
+      if (threadIdx.x == kUnitThreads - 1) s_map.first[kBatchRequests] = at;
+      __syncthreads();
+    }
+    struct Unit {
+      int req, g, tile, part, start, n, len, k0, k1;   // req -1: the prefix; keys [k0, k1), at least one
+    };
+    auto unit_of = [&](int u) {
+      Unit x;
+      int tiles = a.prefix_tiles;
+      x.req = -1;
+      x.start = 0;
+      x.n = a.n_tokens;
+      x.len = a.prefix_len;
+      int chunk = a.prefix_chunk;
+      if (u >= n_prefix) {
+        // the last request whose first unit is <= u: one of 32 eights, one of 8
+        int i = (__popc(__ballot_sync(kAll, s_map.first[lane * 8] <= u)) - 1) * 8;
+        i += __popc(__ballot_sync(kAll, lane < 8 && s_map.first[i + (lane & 7)] <= u)) - 1;
+        u -= s_map.first[i];
+        x.req = req0 + i;
+        x.start = s_map.start[i];
+        x.n = s_map.n[i];
+        x.len = s_map.len[i];
+        chunk = a.suffix_chunk;
+        tiles = (x.n * G + ROWS - 1) / ROWS;
+      }
+      const int v = u / a.nkv;
+      x.g = u - v * a.nkv;
+      x.part = v / tiles;
+      x.tile = v - x.part * tiles;
+      x.k0 = x.part * chunk;
+      x.k1 = min(x.len, x.k0 + chunk);
+      // what some row of the tile sees (a range that nobody sees gives the part of no weight)
+      if (x.req >= 0)
+        x.k1 = max(x.k0 + 1, min(x.k1, x.len - x.n + 1 + div_by(min(x.n * G, (x.tile + 1) * ROWS) - 1, G, a.g_magic)));
+      return x;
+    };
 
+    // the next tile to copy: its table, head, key; the blocks of its keys are
+    // loaded (`ahead`, a key a lane) when the tile before it is copied
+    int p_unit = w;
+    const int* p_table = a.prefix_table;
+    int p_g = 0, p_key = 0, p_k1 = 0, ahead = 0, to = 0;
+    auto look = [&]() { ahead = lane < kUnitKeys && p_key + lane < p_k1 ? p_table[(p_key + lane) >> a.page_shift] : 0; };
+    auto open = [&]() {
+      p_k1 = 0;
+      if (p_unit < n_units) {
+        const Unit x = unit_of(p_unit);
+        p_unit += W;
+        p_g = x.g;
+        p_key = x.k0;
+        p_k1 = x.k1;
+        p_table = x.req >= 0 ? a.block_table + x.req * a.table_stride : a.prefix_table;
+        look();
+      }
+    };
+    // copy it into stage `to`: rows past the range or with a bad block are
+    // filled with zeros, so what the pool holds there never enters a product
+    auto push = [&]() {
+      if (p_k1 > 0) {
+        unsigned char* dst = ring + to * unit_stage_bytes<HD>();
+        int slot = -1;
+        if (lane < kUnitKeys && p_key + lane < p_k1) {
+          const long sl = ((long)ahead << a.page_shift) + ((p_key + lane) & mask);
+          if (ahead < 0 || sl >= a.n_slots) atomicCAS(a.status, kDevOk, kDevBadIndex);
+          else slot = (int)sl;
+        }
+        const int c = lane % CH;
+        const char* kp = static_cast<const char*>(a.k_pool) + ((long)p_g * HD + c * 8) * 2;
+        const long to_v = static_cast<const char*>(a.v_pool) - static_cast<const char*>(a.k_pool);
+        const int row_bytes = (int)(a.slot_stride * 2);
 #pragma unroll
-  for (int s = 0; s < ST - 1; ++s) {
-    if (first + s * step < k1) issue(first + s * step, block[s], s);
-    cp_async_commit();
+        for (int i = 0; i < kUnitKeys / LR; ++i) {
+          const int r = i * LR + lane / CH;
+          const int sl = __shfl_sync(kAll, slot, r);
+          const char* src = kp + (long)max(sl, 0) * row_bytes;
+          cp_async16(dst + r * RB + c * 16, src, sl >= 0);
+          cp_async16(dst + (kUnitKeys + r) * RB + c * 16, src + to_v, sl >= 0);
+        }
+        p_key += kUnitKeys;
+        if (p_key < p_k1) look();
+        else open();
+        if (++to == ST) to = 0;
+      }
+      cp_async_commit();
+    };
+    open();
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) push();
+
+    int at = 0;                                  // the stage of the next tile to use
+    for (int c_unit = w; c_unit < n_units; c_unit += W) {
+      const Unit x = unit_of(c_unit);
+      const bool suffix = x.req >= 0;
+      const int g = x.g, tile = x.tile, part = x.part, start = x.start, n = x.n, len = x.len, k0 = x.k0, k1 = x.k1;
+      const int rows = n * G;
+      const int seen0 = suffix ? len - n + 1 : len;                   // positions the first token sees
+      const int seen_by_all = seen0 + (suffix ? div_by(tile * ROWS, G, a.g_magic) : 0);   // ... every row of the tile
+
+      // q of row gid of each eight as the second operand
+      uint32_t qf[TERMS][RT][KS][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int r = tile * ROWS + rt * 8 + gid;
+        const Q* src = nullptr;
+        if (r < rows) {
+          const int j = div_by(r, G, a.g_magic);
+          src = static_cast<const Q*>(a.q) + (long)(start + j) * a.q_stride + (long)(g * G + r - j * G) * HD + tig * 2;
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if constexpr (TERMS == 1) {          // q is of the cache's type: as it is
+              qf[0][rt][ks][x] = src ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 * x) : 0;
+            } else {
+              const float2 v = src ? load2(src + ks * 16 + 8 * x) : make_float2(0.f, 0.f);
+              uint32_t term[TERMS];
+              split2<TERMS, C>(v.x, v.y, term);
+#pragma unroll
+              for (int i = 0; i < TERMS; ++i) qf[i][rt][ks][x] = term[i];
+            }
+          }
+      }
+      // the scores and outputs of this thread belong to rows 2 tig and 2 tig + 1
+      // of each eight: the number of positions they see
+      int see[RT][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = tile * ROWS + rt * 8 + tig * 2 + e;
+          see[rt][e] = r >= rows ? 0 : suffix ? seen0 + div_by(r, G, a.g_magic) : len;
+        }
+      float o[RT][MT][4], m[RT][2], l[RT][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        m[rt][0] = m[rt][1] = -INFINITY;
+        l[rt][0] = l[rt][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) o[rt][i][0] = o[rt][i][1] = o[rt][i][2] = o[rt][i][3] = 0.f;
+      }
+
+      for (int key = k0; key < k1; key += kUnitKeys) {
+        push();
+        cp_async_wait<ST - 1>();
+        __syncwarp();
+        const unsigned char* kb = ring + at * unit_stage_bytes<HD>();
+        const unsigned char* vb = kb + kUnitKeys * RB;
+        // S^T: chains of products that wait for one another cost ~20 cycles a
+        // link, so each term (or half of the head) has accumulators of its own
+        constexpr int CHAINS = TERMS == 1 && RT < 4 ? 2 : TERMS;
+        float acc[CHAINS][RT][4];
+#pragma unroll
+        for (int i = 0; i < CHAINS; ++i)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) acc[i][rt][0] = acc[i][rt][1] = acc[i][rt][2] = acc[i][rt][3] = 0.f;
+        // lane l names row l % 8 of matrix l / 8: (keys, keys + 8) x (dims, dims + 8)
+        const unsigned char* kr = kb + ((lane & 7) + ((lane >> 3) & 1) * 8) * RB + (lane >> 4) * 16;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t kf[4];
+          ldmatrix_x4(kf, kr + ks * 32);
+#pragma unroll
+          for (int i = 0; i < TERMS; ++i)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+              mma16816(acc[TERMS == 1 ? ks % CHAINS : i][rt], kf, qf[i][rt][ks][0], qf[i][rt][ks][1], C());
+        }
+        // Scores in powers of two; masked ones leave by selection, whatever they
+        // hold. c[0], c[1]: key gid, rows 2 tig and 2 tig + 1; c[2], c[3]: key gid + 8.
+        float sc[RT][4], mx[RT][2];
+        const bool cut = key + kUnitKeys > min(k1, seen_by_all);
+        bool move = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = acc[CHAINS - 1][rt][e];    // smallest terms first
+#pragma unroll
+            for (int i = CHAINS - 2; i >= 0; --i) v += acc[i][rt][e];
+            sc[rt][e] = v * a.scale_log2;
+            if (cut) {
+              const int pos = key + gid + (e >> 1) * 8;
+              if (pos >= k1 || pos >= see[rt][e & 1]) sc[rt][e] = -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v = fmaxf(sc[rt][e], sc[rt][2 + e]);
+            v = fmaxf(v, __shfl_xor_sync(kAll, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(kAll, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(kAll, v, 16));
+            mx[rt][e] = v;
+            move |= m[rt][e] == -INFINITY ? v != -INFINITY : v - m[rt][e] > kGrow;
+          }
+        }
+        if (__any_sync(kAll, move)) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const bool grown = m[rt][e] == -INFINITY || mx[rt][e] - m[rt][e] > kGrow;
+              const float keep = grown && m[rt][e] != -INFINITY ? exp2_fast(m[rt][e] - mx[rt][e]) : 1.f;
+              if (grown) m[rt][e] = mx[rt][e];
+              l[rt][e] *= keep;
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                o[rt][i][e] *= keep;
+                o[rt][i][2 + e] *= keep;
+              }
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float base = (m[rt][e & 1] == -INFINITY ? 0.f : m[rt][e & 1]) - weight_bias(C());
+            sc[rt][e] = exp2_fast(sc[rt][e] - base);
+            l[rt][e & 1] += sc[rt][e];
+          }
+        // A weight of 0 times a NaN or infinity is NaN: where some rows of the
+        // tile must not see a position that others see, a value that is not
+        // finite is kept out of the product, and added one weight at a time
+        if (key + kUnitKeys > seen_by_all && any_not_finite<HD, C>(vb, lane)) {
+          add_by_weight<HD, C, RT>(o, sc, vb, key, k1, see, lane);
+        } else {
+          uint32_t pf[TERMS][RT][2];             // P^T as the second operand: rows become columns
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              uint32_t term[TERMS];
+              split2<TERMS, C>(sc[rt][2 * x], sc[rt][2 * x + 1], term);
+#pragma unroll
+              for (int i = 0; i < TERMS; ++i) pf[i][rt][x] = transpose8x8(term[i]);
+            }
+          const unsigned char* vr = vb + ((lane & 7) + (lane >> 4) * 8) * RB + ((lane >> 3) & 1) * 16;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            uint32_t vf[4];
+            ldmatrix_x4_trans(vf, vr + i * 32);
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x)
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt) mma16816(o[rt][i], vf, pf[x][rt][0], pf[x][rt][1], C());
+          }
+        }
+        __syncwarp();   // the stage is refilled by the next turn's copy
+        if (++at == ST) at = 0;
+      }
+
+      // the unit's part; the eight lanes of a row store 32 bytes side by side
+      const long base = (long)(suffix ? a.prefix_parts + part : part) * a.n_tokens * a.nh;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[rt][e];
+          sum += __shfl_xor_sync(kAll, sum, 4);
+          sum += __shfl_xor_sync(kAll, sum, 8);
+          sum += __shfl_xor_sync(kAll, sum, 16);
+          const int r = tile * ROWS + rt * 8 + tig * 2 + e;
+          if (r >= rows) continue;
+          const int j = div_by(r, G, a.g_magic);
+          const long row = base + (long)(start + j) * a.nh + g * G + r - j * G;
+          if (gid == 0) a.part_ml[row] = make_float2(m[rt][e], sum);
+          float* dst = a.part_o + row * HD + gid;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            dst[i * 16] = o[rt][i][e];
+            dst[i * 16 + 8] = o[rt][i][2 + e];
+          }
+        }
+    }
+    cp_async_wait<0>();
   }
-
-  // this thread's two rows: token, head, and the number of positions it sees
-  long row_at[2];                                // t * nh + h, or -1
-  int see[2];
-  uint32_t qf[TERMS][KS][4];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const int r = tile * 16 + gid + 8 * e;
-    row_at[e] = -1;
-    see[e] = 0;
-    const Q* src = nullptr;
-    if (r < rows) {
-      const int j = r / G, t = start + j, h = g * G + (r - j * G);
-      row_at[e] = (long)t * a.nh + h;
-      see[e] = suffix ? seen0 + j : len;
-      src = static_cast<const Q*>(a.q) + (long)t * a.q_stride + (long)h * HD;
-    }
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        const float2 x = src ? load2(src + ks * 16 + tig * 2 + 8 * f) : make_float2(0.f, 0.f);
-        uint32_t term[TERMS];
-        split2<TERMS, C>(x.x, x.y, term);
-#pragma unroll
-        for (int i = 0; i < TERMS; ++i) qf[i][ks][e + 2 * f] = term[i];
-      }
-    }
-  }
-
-  int s = 0;
-  for (int key = first; key < k1; key += step) {
-    const int next = key + (ST - 1) * step;
-    int sn = s + ST - 1;
-    if (sn >= ST) sn -= ST;
-    if (next < k1) issue(next, ahead, sn);
-    cp_async_commit();
-    ahead = block_of(next + step);
-    cp_async_wait<ST - 1>();
-    __syncwarp();
-    const unsigned char* kb = ring + s * unit_stage_bytes<HD>();
-    const unsigned char* vb = kb + kUnitKeys * RB;
-    // chains of products that wait for one another cost ~20 cycles a link:
-    // each term (or half of the head) has accumulators of its own
-    constexpr int CHAINS = TERMS == 1 ? 2 : TERMS;
-    float acc[CHAINS][2][4];
-#pragma unroll
-    for (int i = 0; i < CHAINS; ++i)
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) acc[i][nt][0] = acc[i][nt][1] = acc[i][nt][2] = acc[i][nt][3] = 0.f;
-    // K fragments of both key octets: lane l names row l % 8 of matrix l / 8
-    const int kr = (lane & 7) + ((lane >> 4) << 3), kc = ((lane >> 3) & 1) * 8;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      uint32_t kf[4];
-      ldmatrix_x4(kf, kb + kr * RB + (ks * 16 + kc) * 2);
-#pragma unroll
-      for (int i = 0; i < TERMS; ++i) {
-        const int ch = TERMS == 1 ? ks & 1 : i;
-        mma16816(acc[ch][0], qf[i][ks], kf[0], kf[1], C());
-        mma16816(acc[ch][1], qf[i][ks], kf[2], kf[3], C());
-      }
-    }
-    float sc[2][4];
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sc[nt][e] = acc[CHAINS - 1][nt][e];        // smallest terms first
-#pragma unroll
-        for (int i = CHAINS - 2; i >= 0; --i) sc[nt][e] += acc[i][nt][e];
-      }
-    // scores in powers of two; masked ones leave by selection, whatever they hold
-    float mx[2] = {m[0], m[1]};
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int pos = key + nt * 8 + tig * 2 + (e & 1);
-        const bool in = pos < k1 && pos < see[e >> 1];
-        sc[nt][e] = in ? sc[nt][e] * a.scale_log2 : -INFINITY;
-        mx[e >> 1] = fmaxf(mx[e >> 1], sc[nt][e]);
-      }
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-      mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-      const float base = mx[e] == -INFINITY ? 0.f : mx[e];
-      const float keep = exp2_fast(m[e] - base);
-      m[e] = mx[e];
-      mx[e] = base - weight_bias(C());
-      l[e] *= keep;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        o[i][2 * e] *= keep;
-        o[i][2 * e + 1] *= keep;
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sc[nt][e] = exp2_fast(sc[nt][e] - mx[e >> 1]);
-        l[e >> 1] += sc[nt][e];
-      }
-    uint32_t pf[TERMS][4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      uint32_t term[TERMS];
-      split2<TERMS, C>(sc[e >> 1][2 * (e & 1)], sc[e >> 1][2 * (e & 1) + 1], term);
-#pragma unroll
-      for (int i = 0; i < TERMS; ++i) pf[i][e] = term[i];
-    }
-    // A weight of 0 times a NaN or infinity is NaN: where some rows of the tile
-    // must not see a position that others see, a value that is not finite is
-    // kept out of the product, and added one weight at a time
-    if (key + kUnitKeys > seen_by_all && any_not_finite<HD, C>(vb, lane)) {
-      add_by_weight<HD, C>(o, sc, vb, key, k1, see, lane);
-    } else {
-    const int vr = (lane & 7) + ((lane >> 3) & 1) * 8;
-#pragma unroll
-    for (int np = 0; np < NT / 2; ++np) {
-      uint32_t vf[4];
-      ldmatrix_x4_trans(vf, vb + vr * RB + (np * 16 + (lane >> 4) * 8) * 2);
-#pragma unroll
-      for (int i = 0; i < TERMS; ++i) {
-        mma16816(o[2 * np], pf[i], vf[0], vf[1], C());
-        mma16816(o[2 * np + 1], pf[i], vf[2], vf[3], C());
-      }
-    }
-    }
-    __syncwarp();   // the stage is refilled by the next turn's copy
-    if (++s == ST) s = 0;
-  }
-  cp_async_wait<0>();
-
-  // join the warps
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
-    l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-    if (tig == 0) {
-      s_ml[warp][gid + 8 * e][0] = m[e];
-      s_ml[warp][gid + 8 * e][1] = l[e];
-    }
-  }
-  __syncthreads();   // also: every warp is done with its ring
-  float* s_o = reinterpret_cast<float*>(s_ring);
-#pragma unroll
-  for (int i = 0; i < NT; ++i)
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      *reinterpret_cast<float2*>(s_o + ((warp * 16 + gid + 8 * e) * unit_join_row<HD>() + i * 8 + tig * 2)) =
-          make_float2(o[i][2 * e], o[i][2 * e + 1]);
-  __syncthreads();
-  constexpr int TPR = kUnitThreads / 16;         // threads of a row
-  const int r = threadIdx.x / TPR, c0 = (threadIdx.x % TPR) * (HD / TPR);
+  // a prefix kernel ahead of this one runs on beside it; this grid is not done before that one is
   pdl_wait();
-  if (tile * 16 + r >= rows) return;
-  float mm = -INFINITY;
-#pragma unroll
-  for (int w = 0; w < kUnitWarps; ++w) mm = fmaxf(mm, s_ml[w][r][0]);
-  const float base = mm == -INFINITY ? 0.f : mm;
-  float ll = 0.f, wt[kUnitWarps];
-#pragma unroll
-  for (int w = 0; w < kUnitWarps; ++w) {
-    wt[w] = exp2_fast(s_ml[w][r][0] - base);
-    ll += s_ml[w][r][1] * wt[w];
-  }
-  const int rr = tile * 16 + r, j = rr / G;
-  const long at = (long)slot_part * a.n_tokens * a.nh + (long)(start + j) * a.nh + g * G + (rr - j * G);
-  if (c0 == 0) a.part_ml[at] = make_float2(mm, ll);
-#pragma unroll
-  for (int c = 0; c < HD / TPR; c += 4) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < kUnitWarps; ++w) {
-      const float4 v = *reinterpret_cast<const float4*>(s_o + (w * 16 + r) * unit_join_row<HD>() + c0 + c);
-      acc.x += v.x * wt[w];
-      acc.y += v.y * wt[w];
-      acc.z += v.z * wt[w];
-      acc.w += v.w * wt[w];
-    }
-    *reinterpret_cast<float4*>(a.part_o + at * HD + c0 + c) = acc;
-  }
 }
 
 __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
@@ -486,41 +585,53 @@ __device__ __forceinline__ void store4(__half* p, float4 v) {
 constexpr int kJoinThreads = 128;
 constexpr int kJoinBatch = 8;
 
-// Join the parts of each row: HD/4 threads a row, 4 columns each. grid: (token,
-// heads over kJoinThreads/(HD/4)). Tokens past token_start[R] and those of a
-// request that was skipped get zeros, as do rows that see nothing. Bound: the
-// latency of two loads (lengths; parts, all at once) after the parts are there.
-template <int HD, typename Q>
+// Join the parts of each row: HD/4 threads a group, 4 columns each. With SPLIT
+// (more than kJoinBatch parts) the groups of a CTA share one row's parts, else
+// each has a row of its own. grid: (token, heads over the rows of a CTA).
+// Tokens past token_start[R] and those of a request that was skipped get zeros,
+// as do rows that see nothing. Bound: the latency of two loads (lengths; parts,
+// all at once) after the parts are there.
+template <int HD, typename Q, bool SPLIT>
 __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArgs a) {
-  constexpr int TPR = HD / 4;
+  constexpr int TPR = HD / 4, GROUPS = kJoinThreads / TPR;
+  __shared__ float4 s_acc[SPLIT ? GROUPS : 1][TPR];
+  __shared__ float2 s_ml[GROUPS];
+  __shared__ int s_len;
   const int t = blockIdx.x;
   // whether a valid request holds the token: written by nobody ahead of this kernel
   bool mine = false;
   for (int i = threadIdx.x; i < a.n_requests; i += kJoinThreads) {
     const int start = a.token_start[i], end = a.token_start[i + 1], len = a.lens[i];
-    mine |= t >= start && t < end && start >= 0 && end - start <= a.max_new && end <= a.n_tokens && len >= 0 &&
-            len <= a.max_len;
+    if (t >= start && t < end && start >= 0 && end - start <= a.max_new && end <= a.n_tokens && len >= 0 &&
+        len <= a.max_len) {
+      mine = true;
+      s_len = len;
+    }
   }
   const bool ok = __syncthreads_or(mine);
   pdl_wait();
-  const int h = blockIdx.y * (kJoinThreads / TPR) + threadIdx.x / TPR;
-  if (h >= a.nh) return;
-  const int c = (threadIdx.x % TPR) * 4;
+  const int group = threadIdx.x / TPR, c = (threadIdx.x % TPR) * 4;
+  const int h = SPLIT ? blockIdx.y : blockIdx.y * GROUPS + group;
+  if (!SPLIT && h >= a.nh) return;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float mm = -INFINITY, ll = 0.f;
   if (ok) {
-    const int parts = a.prefix_parts + a.suffix_parts;
+    // own positions past the length have no parts
+    const int parts = a.prefix_parts + (a.suffix_parts ? (s_len + a.suffix_chunk - 1) / a.suffix_chunk : 0);
     const long stride = (long)a.n_tokens * a.nh, row = (long)t * a.nh + h;
-    float mm = -INFINITY, ll = 0.f;
-    for (int p0 = 0; p0 < parts; p0 += kJoinBatch) {
+    constexpr int STEP = SPLIT ? GROUPS : 1;
+    for (int p0 = SPLIT ? group : 0; p0 < parts; p0 += STEP * kJoinBatch) {
       float2 ml[kJoinBatch];
       float4 v[kJoinBatch];
 #pragma unroll
       for (int p = 0; p < kJoinBatch; ++p) {
-        const bool in = p0 + p < parts;
-        const long at = (in ? p0 + p : p0) * stride + row;
-        ml[p] = __ldcg(a.part_ml + at);
-        v[p] = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * HD + c));
-        if (!in) ml[p].x = -INFINITY;
+        ml[p] = make_float2(-INFINITY, 0.f);
+        v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p0 + p * STEP < parts) {
+          const long at = (p0 + p * STEP) * stride + row;
+          ml[p] = __ldcg(a.part_ml + at);
+          v[p] = __ldcg(reinterpret_cast<const float4*>(a.part_o + at * HD + c));
+        }
       }
       float top = mm;
 #pragma unroll
@@ -533,7 +644,6 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
 #pragma unroll
       for (int p = 0; p < kJoinBatch; ++p) {
         const float w = exp2_fast(ml[p].x - base);
-        if (p0 + p >= parts) break;
         ll += ml[p].y * w;
         acc.x += v[p].x * w;
         acc.y += v[p].y * w;
@@ -541,9 +651,30 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
         acc.w += v[p].w * w;
       }
     }
-    const float inv = ll == 0.f ? 0.f : 1.f / ll;
-    acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   }
+  if (SPLIT) {
+    s_acc[group][threadIdx.x % TPR] = acc;
+    if (c == 0) s_ml[group] = make_float2(mm, ll);
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int i = 1; i < GROUPS; ++i) mm = fmaxf(mm, s_ml[i].x);
+    const float base = mm == -INFINITY ? 0.f : mm;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    ll = 0.f;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) {
+      const float w = exp2_fast(s_ml[i].x - base);
+      const float4 v = s_acc[i][threadIdx.x % TPR];
+      ll += s_ml[i].y * w;
+      acc.x += v.x * w;
+      acc.y += v.y * w;
+      acc.z += v.z * w;
+      acc.w += v.w * w;
+    }
+  }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   store4(static_cast<Q*>(a.out) + (long)t * a.out_stride + (long)h * HD + c, acc);
 }
 

@@ -38,7 +38,6 @@ namespace ls {
 
 constexpr int kTcKeys = 128;          // keys of a tile
 constexpr int kTcRows = 128;          // rows of a tile
-constexpr float kTcGrow = 8.f;        // log2 growth of a row's maximum that moves its reference
 
 template <int HD, int MT>
 struct TcLayout {
@@ -426,7 +425,7 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
         top = max2_nan(top, row_max[(half ^ 1) * kTcRows]);
         // m and top are raw scores; their distance counts after the scale. A NaN
         // score makes the reference NaN, and with it the whole row
-        const bool move = m == -INFINITY ? top != -INFINITY : !((top - m) * a.scale_log2 <= kTcGrow);
+        const bool move = m == -INFINITY ? top != -INFINITY : !((top - m) * a.scale_log2 <= kGrow);
         if (__any_sync(0xffffffffu, move)) {
           const float keep = move && m > -INFINITY ? exp2_fast((m - top) * a.scale_log2) : 1.f;
           if (move) m = top;

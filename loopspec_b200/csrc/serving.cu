@@ -175,11 +175,14 @@ void run_qk_norm_rope(const ls_qk_norm_args& p, cudaStream_t stream) {
 // ------------------------------------------------------------ prefix attention
 // How a call is cut into units: a function of its sizes and types alone.
 struct PrefixPlan {
-  int tc_tiles;     // 128-row tiles a CTA of the tcgen05 kernel takes; 0: the unit kernel does everything
+  int tc_tiles;     // 128-row tiles a CTA of the tcgen05 kernel takes; 0: the stream kernel does everything
   bool own;         // it takes one request's rows and also does that request's own positions
   int prefix_parts, prefix_chunk, suffix_parts, suffix_chunk, prefix_tiles, suffix_tiles;
+  int prefix_rt, suffix_rt;   // eights of rows in a tile of the stream kernel
   size_t o_bytes, ml_bytes, total;
 };
+
+constexpr int kMaxParts = 64;   // of the prefix, and of a request's own positions
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -189,11 +192,15 @@ void cut(long units, int len, long resident, int least, int grain, int& parts, i
   parts = chunk = 0;
   if (len == 0) return;
   const long want = std::max(1L, resident / std::max(1L, units));
-  const int most = std::max(1, len / least);
-  parts = (int)std::min<long>(want, most);
+  const int most = std::max(1, cdiv(len, least));
+  parts = (int)std::min<long>(std::min<long>(want, most), kMaxParts);
   chunk = cdiv(cdiv(len, parts), grain) * grain;
   parts = cdiv(len, chunk);
 }
+
+// Eights of rows in a row tile of the stream kernel: the rows there are, up to
+// what q and O leave registers for.
+int tile_eights(long rows) { return rows <= 8 ? 1 : 2; }
 
 PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int prefix_len, int max_new,
                      int max_len, bool split_q, int sms) {
@@ -204,7 +211,9 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
   // Requests that bring whole tiles of rows on average do not need each other
   // to fill one: their own positions then follow the prefix in the same unit.
   p.own = !split_q && rows >= (long)kTcRows * n_requests;
-  p.suffix_tiles = cdiv(most_new * G, 16);
+  p.suffix_rt = tile_eights(most_new * G);
+  p.suffix_tiles = cdiv(most_new * G, 8 * p.suffix_rt);
+  const long warps = 12L * sms;   // of the stream kernel, about
   if (p.own) {
     p.tc_tiles = most_new * G > kTcRows ? 2 : 1;
     p.prefix_tiles = cdiv(most_new * G, kTcRows * p.tc_tiles);
@@ -216,10 +225,13 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
       p.prefix_tiles = cdiv(rows, kTcRows * p.tc_tiles);
       cut((long)p.prefix_tiles * nkv, prefix_len, sms, kTcKeys, kTcKeys, p.prefix_parts, p.prefix_chunk);
     } else {
-      p.prefix_tiles = cdiv(rows, 16);
-      cut((long)p.prefix_tiles * nkv, prefix_len, 2L * sms, 256, 64, p.prefix_parts, p.prefix_chunk);
+      // one launch for both if it reads the prefix no more than four times (from L2)
+      p.prefix_rt = rows <= 32 ? p.suffix_rt : tile_eights(rows);
+      p.prefix_tiles = cdiv(rows, 8 * p.prefix_rt);
+      cut((long)p.prefix_tiles * nkv, prefix_len, warps, 64, 16, p.prefix_parts, p.prefix_chunk);
     }
-    cut((long)p.suffix_tiles * nkv * n_requests, max_len, 8L * sms, 256, 64, p.suffix_parts, p.suffix_chunk);
+    // lengths are spread below max_len: two ranges a warp even that out
+    cut((long)p.suffix_tiles * nkv * n_requests, max_len, 2 * warps, 64, 16, p.suffix_parts, p.suffix_chunk);
   }
   const bool direct = p.own && p.prefix_parts <= 1;   // whole results, no parts to keep
   const size_t part_rows = direct ? 0 : (size_t)(p.prefix_parts + p.suffix_parts) * n_tokens * nh;
@@ -248,32 +260,57 @@ void launch_tc(const PrefixAttnArgs& a, cudaStream_t stream) {
          dim3(TcLayout<HD, MT>::kThreads), smem, stream, false, a);
 }
 
+// The stream kernel over the prefix, the requests' own positions or both.
+// `behind`: a kernel of this call is ahead of it.
+template <int HD, typename Q, typename C, int TERMS, int RT>
+void launch_stream(PrefixAttnArgs a, bool prefix, bool suffix, bool behind, cudaStream_t stream) {
+  const long units = (prefix ? (long)a.prefix_parts * a.prefix_tiles * a.nkv : 0) +
+                     (suffix ? (long)a.suffix_parts * a.suffix_tiles * a.nkv * a.n_requests : 0);
+  REQUIRE(units <= INT32_MAX / 2, LS_EINVAL, "prefix attention: too many units for one launch");   // and a stride past the last
+  a.prefix_units = prefix;
+  a.suffix_units = suffix;
+  const size_t smem = unit_smem_bytes<HD, TERMS, RT>();
+  allow_smem<prefix_stream_kernel<HD, Q, C, TERMS, RT>>(smem);
+  const long ctas = std::min<long>((long)unit_ctas<HD, TERMS, RT>() * sm_count(), cdiv(units, kUnitWarps));
+  launch(prefix_stream_kernel<HD, Q, C, TERMS, RT>, dim3((unsigned)ctas), dim3(kUnitThreads), smem, stream, behind, a);
+}
+
 template <int HD, typename Q, typename C, int TERMS>
-void launch_prefix(PrefixAttnArgs a, int tc_tiles, cudaStream_t stream) {
+void launch_stream(const PrefixAttnArgs& a, int rt, bool prefix, bool suffix, bool behind, cudaStream_t stream) {
+  if (rt == 1) return launch_stream<HD, Q, C, TERMS, 1>(a, prefix, suffix, behind, stream);
+  launch_stream<HD, Q, C, TERMS, 2>(a, prefix, suffix, behind, stream);
+}
+
+template <int HD, typename Q, typename C, int TERMS>
+void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& plan, cudaStream_t stream) {
   if constexpr (TERMS == 1) {
-    if (tc_tiles == 1) launch_tc<HD, C, 1>(a, stream);
-    if (tc_tiles == 2) launch_tc<HD, C, 2>(a, stream);
+    if (plan.tc_tiles == 1) launch_tc<HD, C, 1>(a, stream);
+    if (plan.tc_tiles == 2) launch_tc<HD, C, 2>(a, stream);
   }
   if (a.direct) return;
-  a.prefix_units = tc_tiles == 0;
-  const long units = (a.prefix_units ? (long)a.prefix_parts * a.prefix_tiles * a.nkv : 0) +
-                     (long)a.suffix_parts * a.suffix_tiles * a.nkv * a.n_requests;
-  REQUIRE(units <= INT32_MAX, LS_EINVAL, "prefix attention: too many units for one launch");
-  if (units > 0) {
-    const size_t smem = unit_smem_bytes<HD, TERMS>();
-    allow_smem<prefix_unit_kernel<HD, Q, C, TERMS>>(smem);
-    launch(prefix_unit_kernel<HD, Q, C, TERMS>, dim3((unsigned)units), dim3(kUnitThreads), smem, stream,
-           tc_tiles != 0, a);
+  const bool prefix = plan.tc_tiles == 0 && a.prefix_parts > 0, suffix = a.suffix_parts > 0 && a.suffix_tiles > 0;
+  bool behind = plan.tc_tiles != 0;
+  if (prefix && suffix && plan.prefix_rt == plan.suffix_rt) {
+    launch_stream<HD, Q, C, TERMS>(a, plan.prefix_rt, true, true, false, stream);
+    behind = true;
+  } else {
+    if (prefix) launch_stream<HD, Q, C, TERMS>(a, plan.prefix_rt, true, false, false, stream);
+    behind = behind || prefix;
+    if (suffix) launch_stream<HD, Q, C, TERMS>(a, plan.suffix_rt, false, true, behind, stream);
+    behind = behind || suffix;
   }
-  const int per = kJoinThreads / (HD / 4);
-  launch(prefix_join_kernel<HD, Q>, dim3((unsigned)a.n_tokens, (unsigned)cdiv(a.nh, per)), dim3(kJoinThreads), 0,
-         stream, tc_tiles != 0 || units > 0, a);   // early only behind kernels of this call
+  // early only behind kernels of this call: it reads the lengths before it waits
+  constexpr int kGroups = kJoinThreads / (HD / 4);
+  const dim3 rows((unsigned)a.n_tokens, (unsigned)a.nh), groups((unsigned)a.n_tokens, (unsigned)cdiv(a.nh, kGroups));
+  if (a.prefix_parts + a.suffix_parts > kJoinBatch)
+    launch(prefix_join_kernel<HD, Q, true>, rows, dim3(kJoinThreads), 0, stream, behind, a);
+  else launch(prefix_join_kernel<HD, Q, false>, groups, dim3(kJoinThreads), 0, stream, behind, a);
 }
 
 template <typename Q, typename C, int TERMS>
-void launch_prefix(const PrefixAttnArgs& a, int hd, int tc_tiles, cudaStream_t stream) {
-  if (hd == 64) launch_prefix<64, Q, C, TERMS>(a, tc_tiles, stream);
-  else launch_prefix<128, Q, C, TERMS>(a, tc_tiles, stream);
+void launch_prefix(const PrefixAttnArgs& a, int hd, const PrefixPlan& plan, cudaStream_t stream) {
+  if (hd == 64) launch_prefix<64, Q, C, TERMS>(a, plan, stream);
+  else launch_prefix<128, Q, C, TERMS>(a, plan, stream);
 }
 
 void check_prefix_sizes(int n_tokens, int n_requests, int nh, int nkv, int hd, int prefix_len, int max_new,
@@ -284,6 +321,8 @@ void check_prefix_sizes(int n_tokens, int n_requests, int nh, int nkv, int hd, i
   REQUIRE(hd == 64 || hd == 128, LS_EINVAL, "prefix attention: head_dim must be 64 or 128");
   REQUIRE((int64_t)n_tokens * nh <= INT32_MAX, LS_EINVAL, "prefix attention: too many query rows");
 }
+
+bool nh_fits(int n_heads) { return n_heads <= 65535; }   // a grid dimension
 
 void run_prefix_attention(const ls_prefix_attention_args& p, cudaStream_t stream) {
   check_prefix_sizes(p.n_tokens, p.n_requests, p.n_heads, p.n_kv_heads, p.head_dim, p.prefix_len, p.max_new,
@@ -298,6 +337,7 @@ void run_prefix_attention(const ls_prefix_attention_args& p, cudaStream_t stream
   REQUIRE(p.q_stride >= qd && p.out_stride >= qd && p.slot_stride >= kd &&
               p.table_stride >= cdiv(p.max_len, p.page_size),
           LS_EINVAL, "prefix attention: a stride is smaller than its row");
+  REQUIRE(p.slot_stride <= 1 << 29 && nh_fits(p.n_heads), LS_EINVAL, "prefix attention: slot_stride or n_heads too large");
   if (p.n_tokens == 0) return;
   REQUIRE(p.q && p.k_pool && p.v_pool && p.lens && p.token_start && p.out && p.workspace && p.status &&
               (p.prefix_table || p.prefix_len == 0) && (p.block_table || p.max_len == 0),
@@ -333,6 +373,8 @@ void run_prefix_attention(const ls_prefix_attention_args& p, cudaStream_t stream
   a.page_shift = shift;
   a.nh = p.n_heads;
   a.nkv = p.n_kv_heads;
+  const uint32_t group = (uint32_t)(p.n_heads / p.n_kv_heads);
+  a.g_magic = (uint32_t)(((1ull << 32) + group - 1) / group);
   a.scale_log2 = (float)((double)p.scale * 1.4426950408889634);
   a.out = p.out;
   a.out_stride = (long)p.out_stride;
@@ -347,10 +389,10 @@ void run_prefix_attention(const ls_prefix_attention_args& p, cudaStream_t stream
   a.own = plan.own;
   a.direct = plan.own && plan.prefix_parts <= 1;
   a.status = p.status;
-  if (p.q_type == LS_BF16) launch_prefix<bf16, bf16, 1>(a, p.head_dim, plan.tc_tiles, stream);
-  else if (p.q_type == LS_F16) launch_prefix<__half, __half, 1>(a, p.head_dim, plan.tc_tiles, stream);
-  else if (p.cache_type == LS_BF16) launch_prefix<float, bf16, 3>(a, p.head_dim, plan.tc_tiles, stream);
-  else launch_prefix<float, __half, 2>(a, p.head_dim, plan.tc_tiles, stream);
+  if (p.q_type == LS_BF16) launch_prefix<bf16, bf16, 1>(a, p.head_dim, plan, stream);
+  else if (p.q_type == LS_F16) launch_prefix<__half, __half, 1>(a, p.head_dim, plan, stream);
+  else if (p.cache_type == LS_BF16) launch_prefix<float, bf16, 3>(a, p.head_dim, plan, stream);
+  else launch_prefix<float, __half, 2>(a, p.head_dim, plan, stream);
 }
 
 }  // namespace
