@@ -179,6 +179,7 @@ struct PrefixPlan {
   bool own;         // it takes one request's rows and also does that request's own positions
   int prefix_parts, prefix_chunk, suffix_parts, suffix_chunk, prefix_tiles, suffix_tiles;
   int prefix_rt, suffix_rt;   // eights of rows in a tile of the stream kernel
+  int stream_sms;             // SMs the stream kernel is launched for
   size_t o_bytes, ml_bytes, total;
 };
 
@@ -202,6 +203,36 @@ void cut(long units, int len, long resident, int least, int grain, int& parts, i
 // what q and O leave registers for.
 int tile_eights(long rows) { return rows <= 8 ? 1 : 2; }
 
+// How many key ranges the tcgen05 kernel cuts the prefix into, and the SMs left
+// to the stream kernel, which does the requests' own positions beside it: a
+// tcgen05 CTA fills an SM, so the two share the GPU by SMs. Measured costs in
+// cycles: a CTA spends 16000 around its key tiles (lookups, first copies, parts
+// out) and 3400 a tile (two row tiles; one: 2000); the stream kernel 6000 on
+// every SM and 350 a tile of 16 keys. Fewer, longer CTAs waste less on the
+// former (33 requests of 5 drafts behind 5001 positions: 5 ranges beside the
+// stream take 44000 cycles, 10 ranges and then the stream 50000).
+void share(PrefixPlan& p, int prefix_len, double stream_cycles, int sms, int units) {
+  const int tiles = cdiv(prefix_len, kTcKeys);
+  const double per_tile = p.tc_tiles == 2 ? 3400 : 2000;
+  auto ranged = [&](int parts) { return 16000 + per_tile * cdiv(tiles, parts); };
+  const int most = std::max(1, std::min({sms / units, tiles, kMaxParts}));
+  double best = 0;
+  for (int parts = 1; parts <= most; ++parts) {
+    const int ctas = units * cdiv(tiles, cdiv(tiles, parts));
+    const double after = ranged(parts) * cdiv(ctas, sms) + stream_cycles / sms;
+    // lengths are only bounded: never stretch the prefix far for the sake of the rest
+    const double beside = ctas < sms && ranged(parts) <= 1.6 * ranged(most)
+                              ? std::max(ranged(parts), stream_cycles / (sms - ctas)) : after;
+    const double cycles = std::min(after, beside);
+    if (best == 0 || cycles < best) {
+      best = cycles;
+      p.prefix_chunk = cdiv(tiles, parts) * kTcKeys;
+      p.stream_sms = beside < after ? sms - ctas : sms;
+    }
+  }
+  p.prefix_parts = cdiv(prefix_len, p.prefix_chunk);
+}
+
 PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int prefix_len, int max_new,
                      int max_len, bool split_q, int sms) {
   PrefixPlan p{};
@@ -213,7 +244,7 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
   p.own = !split_q && rows >= (long)kTcRows * n_requests;
   p.suffix_rt = tile_eights(most_new * G);
   p.suffix_tiles = cdiv(most_new * G, 8 * p.suffix_rt);
-  const long warps = 12L * sms;   // of the stream kernel, about
+  p.stream_sms = sms;
   if (p.own) {
     p.tc_tiles = most_new * G > kTcRows ? 2 : 1;
     p.prefix_tiles = cdiv(most_new * G, kTcRows * p.tc_tiles);
@@ -223,15 +254,17 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
     p.tc_tiles = split_q || rows <= 16 || prefix_len == 0 ? 0 : rows > kTcRows ? 2 : 1;
     if (p.tc_tiles) {
       p.prefix_tiles = cdiv(rows, kTcRows * p.tc_tiles);
-      cut((long)p.prefix_tiles * nkv, prefix_len, sms, kTcKeys, kTcKeys, p.prefix_parts, p.prefix_chunk);
+      const double own_tiles = (double)n_requests * nkv * cdiv(cdiv(rows, n_requests), 8 * p.suffix_rt) * max_len / 16 / 2;
+      const long units = (long)p.prefix_tiles * nkv;
+      share(p, prefix_len, max_len ? 350 * own_tiles + 6000. * sms : 0, sms, (int)std::min<long>(units, 1 << 20));
     } else {
       // one launch for both if it reads the prefix no more than four times (from L2)
       p.prefix_rt = rows <= 32 ? p.suffix_rt : tile_eights(rows);
       p.prefix_tiles = cdiv(rows, 8 * p.prefix_rt);
-      cut((long)p.prefix_tiles * nkv, prefix_len, warps, 64, 16, p.prefix_parts, p.prefix_chunk);
+      cut((long)p.prefix_tiles * nkv, prefix_len, 12L * sms, 64, 16, p.prefix_parts, p.prefix_chunk);
     }
-    // lengths are spread below max_len: two ranges a warp even that out
-    cut((long)p.suffix_tiles * nkv * n_requests, max_len, 2 * warps, 64, 16, p.suffix_parts, p.suffix_chunk);
+    // lengths are spread below max_len: two ranges a warp (12 an SM) even that out
+    cut((long)p.suffix_tiles * nkv * n_requests, max_len, 24L * p.stream_sms, 64, 16, p.suffix_parts, p.suffix_chunk);
   }
   const bool direct = p.own && p.prefix_parts <= 1;   // whole results, no parts to keep
   const size_t part_rows = direct ? 0 : (size_t)(p.prefix_parts + p.suffix_parts) * n_tokens * nh;
@@ -263,7 +296,7 @@ void launch_tc(const PrefixAttnArgs& a, cudaStream_t stream) {
 // The stream kernel over the prefix, the requests' own positions or both.
 // `behind`: a kernel of this call is ahead of it.
 template <int HD, typename Q, typename C, int TERMS, int RT>
-void launch_stream(PrefixAttnArgs a, bool prefix, bool suffix, bool behind, cudaStream_t stream) {
+void launch_stream(PrefixAttnArgs a, bool prefix, bool suffix, bool behind, int sms, cudaStream_t stream) {
   const long units = (prefix ? (long)a.prefix_parts * a.prefix_tiles * a.nkv : 0) +
                      (suffix ? (long)a.suffix_parts * a.suffix_tiles * a.nkv * a.n_requests : 0);
   REQUIRE(units <= INT32_MAX / 2, LS_EINVAL, "prefix attention: too many units for one launch");   // and a stride past the last
@@ -271,14 +304,14 @@ void launch_stream(PrefixAttnArgs a, bool prefix, bool suffix, bool behind, cuda
   a.suffix_units = suffix;
   const size_t smem = unit_smem_bytes<HD, TERMS, RT>();
   allow_smem<prefix_stream_kernel<HD, Q, C, TERMS, RT>>(smem);
-  const long ctas = std::min<long>((long)unit_ctas<HD, TERMS, RT>() * sm_count(), cdiv(units, kUnitWarps));
+  const long ctas = std::min<long>((long)unit_ctas<HD, TERMS, RT>() * sms, cdiv(units, kUnitWarps));
   launch(prefix_stream_kernel<HD, Q, C, TERMS, RT>, dim3((unsigned)ctas), dim3(kUnitThreads), smem, stream, behind, a);
 }
 
 template <int HD, typename Q, typename C, int TERMS>
-void launch_stream(const PrefixAttnArgs& a, int rt, bool prefix, bool suffix, bool behind, cudaStream_t stream) {
-  if (rt == 1) return launch_stream<HD, Q, C, TERMS, 1>(a, prefix, suffix, behind, stream);
-  launch_stream<HD, Q, C, TERMS, 2>(a, prefix, suffix, behind, stream);
+void launch_stream(const PrefixAttnArgs& a, int rt, bool prefix, bool suffix, bool behind, int sms, cudaStream_t stream) {
+  if (rt == 1) launch_stream<HD, Q, C, TERMS, 1>(a, prefix, suffix, behind, sms, stream);
+  else launch_stream<HD, Q, C, TERMS, 2>(a, prefix, suffix, behind, sms, stream);
 }
 
 template <int HD, typename Q, typename C, int TERMS>
@@ -291,18 +324,19 @@ void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& plan, cudaStream_t
   const bool prefix = plan.tc_tiles == 0 && a.prefix_parts > 0, suffix = a.suffix_parts > 0 && a.suffix_tiles > 0;
   bool behind = plan.tc_tiles != 0;
   if (prefix && suffix && plan.prefix_rt == plan.suffix_rt) {
-    launch_stream<HD, Q, C, TERMS>(a, plan.prefix_rt, true, true, false, stream);
+    launch_stream<HD, Q, C, TERMS>(a, plan.prefix_rt, true, true, false, plan.stream_sms, stream);
     behind = true;
   } else {
-    if (prefix) launch_stream<HD, Q, C, TERMS>(a, plan.prefix_rt, true, false, false, stream);
+    if (prefix) launch_stream<HD, Q, C, TERMS>(a, plan.prefix_rt, true, false, false, plan.stream_sms, stream);
     behind = behind || prefix;
-    if (suffix) launch_stream<HD, Q, C, TERMS>(a, plan.suffix_rt, false, true, behind, stream);
+    if (suffix) launch_stream<HD, Q, C, TERMS>(a, plan.suffix_rt, false, true, behind, plan.stream_sms, stream);
     behind = behind || suffix;
   }
   // early only behind kernels of this call: it reads the lengths before it waits
   constexpr int kGroups = kJoinThreads / (HD / 4);
   const dim3 rows((unsigned)a.n_tokens, (unsigned)a.nh), groups((unsigned)a.n_tokens, (unsigned)cdiv(a.nh, kGroups));
-  if (a.prefix_parts + a.suffix_parts > kJoinBatch)
+  // a row's parts are shared out where there are too few rows to keep the GPU busy
+  if (a.prefix_parts + a.suffix_parts > kJoinBatch && (long)groups.x * groups.y < 4L * sm_count())
     launch(prefix_join_kernel<HD, Q, true>, rows, dim3(kJoinThreads), 0, stream, behind, a);
   else launch(prefix_join_kernel<HD, Q, false>, groups, dim3(kJoinThreads), 0, stream, behind, a);
 }
