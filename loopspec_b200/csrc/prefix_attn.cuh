@@ -583,7 +583,7 @@ __device__ __forceinline__ void store4(__half* p, float4 v) {
 }
 
 constexpr int kJoinThreads = 128;
-constexpr int kJoinBatch = 8;
+constexpr int kJoinBatch = 4;
 
 // Join the parts of each row: HD/4 threads a group, 4 columns each. With SPLIT
 // (more than kJoinBatch parts) the groups of a CTA share one row's parts, else

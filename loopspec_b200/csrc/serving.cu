@@ -336,7 +336,7 @@ void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& plan, cudaStream_t
   constexpr int kGroups = kJoinThreads / (HD / 4);
   const dim3 rows((unsigned)a.n_tokens, (unsigned)a.nh), groups((unsigned)a.n_tokens, (unsigned)cdiv(a.nh, kGroups));
   // a row's parts are shared out where there are too few rows to keep the GPU busy
-  if (a.prefix_parts + a.suffix_parts > kJoinBatch && (long)groups.x * groups.y < 4L * sm_count())
+  if (a.prefix_parts + a.suffix_parts > kJoinBatch && (long)groups.x * groups.y < 16L * sm_count())
     launch(prefix_join_kernel<HD, Q, true>, rows, dim3(kJoinThreads), 0, stream, behind, a);
   else launch(prefix_join_kernel<HD, Q, false>, groups, dim3(kJoinThreads), 0, stream, behind, a);
 }
