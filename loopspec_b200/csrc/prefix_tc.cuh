@@ -1,14 +1,16 @@
-// Shared-prefix attention on the 5th-generation tensor cores, for 16-bit
-// queries (the formulas are in prefix_attn.cuh).
+// Shared-prefix attention on the 5th-generation tensor cores, for many query
+// rows a kv head (the formulas and types are in prefix_attn.cuh; the terms of
+// an fp32 q are tiles beside each other in shared memory, those of P columns
+// beside each other in tensor memory, and the products add up).
 //
 // A unit is (MT row tiles of 128, kv head, key range). Either the rows are
 // query heads of any requests and the keys a range of the prefix (they are the
 // same for all; the result is a part to be joined), or, where requests bring
 // whole tiles of rows (prompts), the rows are one request's and the keys a
-// range of the prefix, the last range followed by the request's own positions;
-// with one range that is the whole result, which is normalised and stored.
+// range of the prefix followed by the request's own positions; with one range
+// that is the whole result, which is normalised and stored.
 // One CTA a unit:
-//   3 producer warps gather K and V rows, a tile of 128 keys each in turn,
+//   2 or 3 producer warps gather K and V rows, a tile of 128 keys each in turn,
 //     through the block table with 16-byte cp.async into a ring of
 //     128-byte-swizzled tiles;
 //   one warp issues S = Q K^T and O += P V (tcgen05.mma, M = 128): K is the
@@ -39,23 +41,32 @@ namespace ls {
 constexpr int kTcKeys = 128;          // keys of a tile
 constexpr int kTcRows = 128;          // rows of a tile
 
-template <int HD, int MT>
+template <int HD, int TERMS, int MT>
 struct TcLayout {
+  static_assert(TERMS == 1 || MT == 1, "the terms of q and P take the second row tile's room");
+  static constexpr int kTile = kTcKeys * HD * 2;           // bytes of a K, V or Q tile
   static constexpr int kProducer = 8 * MT;                 // first producer warp
-  static constexpr int kProducers = 3;
+  static constexpr int kStages = HD == 64 ? 8 : TERMS == 3 ? 4 : TERMS * MT == 2 ? 5 : 6;
+  // A producer waits for a stage by the parity of its turn, which is only right
+  // while the turn before that one is over. Copy i waits for copy i - ST to be
+  // used; its warp has seen copy i - P - ST used, and copies are used in order
+  // but for neighbours (K of a tile before V of the one ahead), so copy
+  // i - 2 ST is over for certain if ST >= P + 2.
+  static constexpr int kProducers = kStages >= 5 ? 3 : 2;
+  static_assert(kStages >= kProducers + 2, "a stage's turns would be mistaken for one another");
   static constexpr int kMma = kProducer + kProducers;      // the issuing warp
   static constexpr int kThreads = 32 * (kMma + 1);
   // With MT = 2 a thread is launched with 96 registers; the softmax warps draw
   // on what the last four warps give back: 640 x 96 = 512 x 104 + 128 x 64.
   static constexpr int kSoftRegs = 104, kRestRegs = 64;
   static constexpr int kLaunchRegs = MT == 2 ? (512 * kSoftRegs + 128 * kRestRegs) / kThreads : 0;
-  static constexpr int kTile = kTcKeys * HD * 2;           // bytes of a K, V or Q tile
-  static constexpr int kStages = HD == 64 ? 8 : MT == 1 ? 6 : 5;
   static constexpr int kMaxBuffers = MT == 1 ? 2 : 1;      // see the softmax warps
   static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 1 + 1;
-  static constexpr int kSmem = MT * kTile + kStages * kTile + kMaxBuffers * MT * 2 * kTcRows * 4 + kBars * 8 + 8 * 4 + 16;
-  static constexpr int kPoly = 2;                          // eighths of the exponentials on the FMA units
-  static constexpr uint32_t kScores = 0, kOut = 256;       // tensor memory columns
+  static constexpr int kQTiles = MT * TERMS;
+  static constexpr int kSmem = kQTiles * kTile + kStages * kTile + kMaxBuffers * MT * 2 * kTcRows * 4 + kBars * 8 + 8 * 4 + 16;
+  static constexpr int kPoly = TERMS == 1 ? 2 : 0;         // eighths of the exponentials on the FMA units
+  // tensor memory columns: two buffers of scores, each with room for P's terms (64 each) over them, then O
+  static constexpr uint32_t kScores = 0, kBuffer = TERMS == 3 ? 192 : 128, kOut = 2 * kBuffer;
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -206,13 +217,22 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
                       __uint_as_float((__float_as_uint(n.y) << 23) + 0x3f800000u)));
 }
 
+// Polls of one wait before it gives up: a poll that finds nothing suspends for
+// microseconds, the longest wait of a sound run is a few hundred.
+constexpr uint32_t kTcWaitLimit = 1u << 20;
+
 // Wait unless an earlier wait timed out. A warp whose wait times out does not
 // leave its loop: it waits no more and goes on over what is there, so that no
 // lane and no warp is missing from a collective or a barrier of the others; the
 // status word tells. (A vote on the outcome would cost 31 cycles a wait, a
 // barrier that is ready 13.)
 __device__ __forceinline__ void wait_on(bool& ok, uint32_t bar, uint32_t parity, int* err, int code) {
-  if (ok && !mbar_try_wait(bar, parity)) ok = mbar_wait(bar, parity, err, code);
+  if (ok && !mbar_try_wait(bar, parity)) {
+    uint32_t i = 0;
+    while (i < kTcWaitLimit && !mbar_try_wait(bar, parity)) ++i;
+    ok = i < kTcWaitLimit;
+    if (!ok) atomicCAS(err, kDevOk, code);
+  }
 }
 
 // Arrive on `bar` once this thread's cp.async copies so far have landed.
@@ -245,8 +265,8 @@ __device__ __forceinline__ void cp_async16_to(uint32_t dst, const void* src, boo
 }
 
 // The weight of own position `pos` for a row whose reference is m, by the formula.
-template <int HD, typename C>
-__device__ __noinline__ float weight_of(const C* q, const C* k, float m, float scale_log2) {
+template <int HD, typename Q, typename C>
+__device__ __noinline__ float weight_of(const Q* q, const C* k, float m, float scale_log2) {
   float s = 0.f;
   for (int i = 0; i < HD; ++i) s += (float)q[i] * (float)k[i];
   const float base = (m == -INFINITY ? 0.f : m * scale_log2) - weight_bias(C());
@@ -265,15 +285,15 @@ __device__ __forceinline__ bool not_finite8(const uint4& v) {
 }
 
 // grid: 1-D over (row tile fastest, kv head, part, request if `own`): CTAs that run together read the same keys.
-template <int HD, typename C, int MT>
-__global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kernel(PrefixAttnArgs a) {
-  using L = TcLayout<HD, MT>;
+template <int HD, typename Q, typename C, int TERMS, int MT>
+__global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_tc_kernel(PrefixAttnArgs a) {
+  using L = TcLayout<HD, TERMS, MT>;
   constexpr int ST = L::kStages;
   constexpr int CH = HD / 8;                       // 16-byte chunks of a row
   constexpr uint32_t kBlock = kTcRows * 128;       // bytes of 64 columns of a tile
   extern __shared__ __align__(1024) unsigned char smem[];
   unsigned char* s_q = smem;
-  unsigned char* s_ring = smem + MT * L::kTile;
+  unsigned char* s_ring = smem + L::kQTiles * L::kTile;
   float* s_max = reinterpret_cast<float*>(s_ring + ST * L::kTile);   // [kMaxBuffers][MT][half][row]
   const uint32_t bars = smem_u32(s_max + L::kMaxBuffers * MT * 2 * kTcRows);
   uint32_t* s_bad = reinterpret_cast<uint32_t*>(s_max + L::kMaxBuffers * MT * 2 * kTcRows) + 2 * L::kBars;   // [8] bits
@@ -283,7 +303,7 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
 
-  // the unit: its rows, and its keys as prefix positions [ka0, ka1) and own positions [0, kb1)
+  // the unit: its rows, and its keys as prefix positions [ka0, ka1) and own positions [kb0, kb1)
   const int G = a.nh / a.nkv;
   unsigned u = blockIdx.x;
   const int tile = (int)(u % (unsigned)a.prefix_tiles);
@@ -300,10 +320,9 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
       auto clear = [&](int t0, int t1) {
         t0 = max(0, t0);
         t1 = min(a.n_tokens, t1);
-        for (int i = threadIdx.x; i < (t1 - t0) * G * CH; i += blockDim.x) {
-          const int t = t0 + i / (G * CH), c = i % (G * CH);
-          *reinterpret_cast<uint4*>(static_cast<C*>(a.out) + (long)t * a.out_stride + (long)g * G * HD + c * 8) =
-              make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < (t1 - t0) * G * (HD / 4); i += blockDim.x) {
+          const int t = t0 + i / (G * (HD / 4)), c = i % (G * (HD / 4));
+          store4(static_cast<Q*>(a.out) + (long)t * a.out_stride + (long)g * G * HD + c * 4, make_float4(0.f, 0.f, 0.f, 0.f));
         }
       };
       if (a.direct) {
@@ -318,12 +337,16 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
   const int row0 = tile * (MT * kTcRows);
   if (row0 >= rows) return;
   const int seen0 = len - n_new + 1;               // own positions the request's first new token sees
-  const int ka0 = part * a.prefix_chunk, ka1 = min(a.prefix_len, ka0 + a.prefix_chunk);
+  // A part is a run of key tiles: of the prefix's, followed by the request's own if `own`.
+  const int j0 = part * (a.prefix_chunk / kTcKeys), j1 = j0 + a.prefix_chunk / kTcKeys;
+  const int n_shared = (a.prefix_len + kTcKeys - 1) / kTcKeys;
+  const int ka0 = min(a.prefix_len, j0 * kTcKeys), ka1 = min(a.prefix_len, j1 * kTcKeys);
   const int last_row = min(rows, row0 + MT * kTcRows) - 1;
   const int see_first = seen0 + row0 / G;          // own positions every row sees, and some row sees
-  const int kb1 = a.own && part == (int)n_parts - 1 ? max(0, min(len, seen0 + last_row / G)) : 0;
-  const int na = (max(0, ka1 - ka0) + kTcKeys - 1) / kTcKeys;
-  const int n = na + (kb1 + kTcKeys - 1) / kTcKeys;    // key tiles
+  const int kb0 = max(0, j0 - n_shared) * kTcKeys;
+  const int kb1 = a.own ? min(max(0, j1 - n_shared) * kTcKeys, min(len, seen0 + last_row / G)) : 0;
+  const int na = (ka1 - ka0 + kTcKeys - 1) / kTcKeys;
+  const int n = na + (max(0, kb1 - kb0) + kTcKeys - 1) / kTcKeys;    // key tiles
   const int* own_table = a.block_table + req * a.table_stride;
 
   // softmax warps of a row tile's half with rows of their own; the others have nothing to do
@@ -361,21 +384,33 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
     // the row tile's queries, swizzled; rows past the last are zeros
     {
       unsigned char* dst = s_q + t * L::kTile;
-      const C* q = static_cast<const C*>(a.q);
-      uint4 v[CH / 2];                               // all of them on their way at once
+      const Q* q = static_cast<const Q*>(a.q);
+      Raw8<Q> v[CH / 2];                             // all of them on their way at once
 #pragma unroll
       for (int k = 0; k < CH / 2; ++k) {
         const int i = (threadIdx.x & 255) + 256 * k, r = i / CH, c = i % CH, rr = row0 + t * kTcRows + r;
-        v[k] = make_uint4(0, 0, 0, 0);
+        v[k] = Raw8<Q>();
         if (rr < rows) {
           const int tok = rr / G, h = g * G + rr - tok * G;
-          v[k] = *reinterpret_cast<const uint4*>(q + (long)(start + tok) * a.q_stride + (long)h * HD + c * 8);
+          v[k].load(q + (long)(start + tok) * a.q_stride + (long)h * HD + c * 8);
         }
       }
 #pragma unroll
       for (int k = 0; k < CH / 2; ++k) {
         const int i = (threadIdx.x & 255) + 256 * k, r = i / CH, c = i % CH;
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[k];
+        unsigned char* to = dst + (c >> 3) * kBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        if constexpr (TERMS == 1) {                  // q is of the cache's type: as it is
+          *reinterpret_cast<uint4*>(to) = v[k].v[0];
+        } else {
+          float f[8];
+          v[k].get(f);
+          uint32_t term[4][TERMS];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) split2<TERMS, C>(f[2 * x], f[2 * x + 1], term[x]);
+#pragma unroll
+          for (int x = 0; x < TERMS; ++x)
+            *reinterpret_cast<uint4*>(to + x * L::kTile) = make_uint4(term[0][x], term[1][x], term[2][x], term[3][x]);
+        }
       }
       fence_proxy_async();
       __syncwarp();
@@ -395,11 +430,11 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
         const int b = MT == 1 ? j & 1 : t;
         const uint32_t ph = (MT == 1 ? j >> 1 : j) & 1;
         // keys of this tile that the row sees, counted from this thread's first
-        int left = (j < na ? ka1 - ka0 - j * kTcKeys : see - (j - na) * kTcKeys) - half * 64;
-        const bool cut = j < na ? j == na - 1 : see_least - (j - na) * kTcKeys < kTcKeys;
+        int left = (j < na ? ka1 - ka0 - j * kTcKeys : see - kb0 - (j - na) * kTcKeys) - half * 64;
+        const bool cut = j < na ? j == na - 1 : see_least - kb0 - (j - na) * kTcKeys < kTcKeys;
         wait_on(ok, s_full + 8 * b, ph, a.status, kDevTimeoutAcc);
         tc_fence_after();
-        const uint32_t sc = lanes + L::kScores + b * 128;
+        const uint32_t sc = lanes + L::kScores + b * L::kBuffer;
         uint32_t s[64];
         tmem_ld_x32(sc + half * 64, s);
         tmem_ld_x32(sc + half * 64 + 32, s + 32);
@@ -449,23 +484,29 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
         // function units, which do 4 of these a cycle and SM quarter
         const uint64_t scale = pair(a.scale_log2, a.scale_log2), minus = pair(-base, -base);
         uint64_t sum[2] = {0, 0};
-        uint32_t p[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const uint64_t x = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, minus);
-          uint64_t w;
-          if ((i * L::kPoly) % 8 < L::kPoly) {
-            w = exp2_poly(x);
-          } else {
-            const float2 v = unpair(x);
-            w = pair(exp2_fast(v.x), exp2_fast(v.y));
+        for (int i0 = 0; i0 < 32; i0 += 16) {
+          uint32_t p[TERMS][16];
+#pragma unroll
+          for (int i = i0; i < i0 + 16; ++i) {
+            const uint64_t x = fma2(pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, minus);
+            uint64_t w;
+            if ((i * L::kPoly) % 8 < L::kPoly) {
+              w = exp2_poly(x);
+            } else {
+              const float2 v = unpair(x);
+              w = pair(exp2_fast(v.x), exp2_fast(v.y));
+            }
+            sum[i & 1] = add2(sum[i & 1], w);
+            const float2 v = unpair(w);
+            uint32_t term[TERMS];
+            split2<TERMS, C>(v.x, v.y, term);
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x) p[x][i - i0] = term[x];
           }
-          sum[i & 1] = add2(sum[i & 1], w);
-          const float2 v = unpair(w);
-          p[i] = pack2(v.x, v.y, C());
-          if (i == 15) tmem_st_x16(sc + half * 32, p);
+#pragma unroll
+          for (int x = 0; x < TERMS; ++x) tmem_st_x16(sc + x * 64 + half * 32 + i0, p[x]);
         }
-        tmem_st_x16(sc + half * 32 + 16, p + 16);
         const float2 total = unpair(add2(sum[0], sum[1]));
         l += total.x + total.y;
         tmem_st_wait();
@@ -513,15 +554,15 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
               const long slot = ((long)own_table[pos >> a.page_shift] << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
               const C* k = static_cast<const C*>(a.k_pool) + slot * a.slot_stride + (long)g * HD;
               const C* v = static_cast<const C*>(a.v_pool) + slot * a.slot_stride + (long)g * HD + d;
-              const float p = weight_of<HD, C>(static_cast<const C*>(a.q) + (long)tok * a.q_stride + (long)h * HD, k, m,
-                                               a.scale_log2) * inv;
+              const float p = weight_of<HD, Q, C>(static_cast<const Q*>(a.q) + (long)tok * a.q_stride + (long)h * HD, k, m,
+                                                  a.scale_log2) * inv;
 #pragma unroll
               for (int i = 0; i < 16; ++i) f[i] += p * (float)v[i];
             }
         }
         if (a.direct) {
           if (rr < rows) {
-            C* dst = static_cast<C*>(a.out) + (long)tok * a.out_stride + (long)h * HD + d;
+            Q* dst = static_cast<Q*>(a.out) + (long)tok * a.out_stride + (long)h * HD + d;
             store8(dst, *reinterpret_cast<float(*)[8]>(f));
             store8(dst + 8, *reinterpret_cast<float(*)[8]>(f + 8));
           }
@@ -554,7 +595,7 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
     const int mask = (1 << a.page_shift) - 1;
     const uint32_t dst0 = smem_u32(s_ring) + (c >> 3) * kBlock + hi * 128;
     // Copy i (2 j: K of tile j, 2 j + 1: its V) goes to stage i % ST and is the
-    // work of warp i % 3; the barrier counts each thread's part in when it has
+    // work of warp i % kProducers; the barrier counts each thread's part in when it has
     // landed, so the producers run a ring ahead. Lane l knows the slots of rows
     // l, l + 32, l + 64, l + 96; their blocks are loaded a copy ahead.
     int next[4];
@@ -562,7 +603,7 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
       const int j = i >> 1;
       const bool own = j >= na;
       const int* table = own ? own_table : a.prefix_table;
-      const int pos = (own ? (j - na) * kTcKeys : ka0 + j * kTcKeys) + lane, end = i >= 2 * n ? 0 : own ? kb1 : ka1;
+      const int pos = (own ? kb0 + (j - na) * kTcKeys : ka0 + j * kTcKeys) + lane, end = i >= 2 * n ? 0 : own ? kb1 : ka1;
 #pragma unroll
       for (int q = 0; q < 4; ++q) next[q] = pos + 32 * q < end ? table[(pos + 32 * q) >> a.page_shift] : 0;
     };
@@ -572,7 +613,7 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
     for (int i = first; i < 2 * n; i += L::kProducers) {
       const int j = i >> 1, st = i % ST;
       const bool own = j >= na, is_v = i & 1;
-      const int pos = (own ? (j - na) * kTcKeys : ka0 + j * kTcKeys) + lane, end = own ? kb1 : ka1;
+      const int pos = (own ? kb0 + (j - na) * kTcKeys : ka0 + j * kTcKeys) + lane, end = own ? kb1 : ka1;
       int slot[4];                                 // -1: filled with zeros
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -632,21 +673,26 @@ __global__ void __launch_bounds__(TcLayout<HD, MT>::kThreads, 1) prefix_tc_kerne
     auto release = [&](int i) {                    // copy i's stage, if another copy will want it
       if (i + ST < 2 * n) tc_commit_if(leader, empty0 + 8 * (i % ST));
     };
-    auto scores = [&](int t, int b, int j) {       // S[b] = Q[t] K[j]^T
+    auto scores = [&](int t, int b, int j) {       // S[b] = Q[t] K[j]^T, smallest terms first
       const uint32_t k = ring_k + ((2 * j % ST) * L::kTile >> 4), q = q0 + (t * L::kTile >> 4);
 #pragma unroll
-      for (int i = 0; i < HD / 16; ++i) {
-        const uint32_t off = ((i >> 2) * kBlock + (i & 3) * 32) >> 4;
-        tc_mma_ss(leader, tmem + L::kScores + b * 128, q + off, k + off, kUmmaHi, idesc_s, i != 0);
-      }
+      for (int x = TERMS - 1; x >= 0; --x)
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          const uint32_t off = ((i >> 2) * kBlock + (i & 3) * 32) >> 4;
+          tc_mma_ss(leader, tmem + L::kScores + b * L::kBuffer, q + (x * L::kTile >> 4) + off, k + off, kUmmaHi, idesc_s,
+                    i != 0 || x != TERMS - 1);
+        }
       tc_commit_if(leader, s_full + 8 * b);
     };
     auto outputs = [&](int t, int b, int j) {      // O[t] += P[b] V[j]
       const uint32_t v = ring_v + (((2 * j + 1) % ST) * L::kTile >> 4);
 #pragma unroll
-      for (int i = 0; i < kTcKeys / 16; ++i)
-        tc_mma_ts(leader, tmem + L::kOut + t * 128, tmem + L::kScores + b * 128 + i * 8, v + (i * 2048 >> 4), kUmmaHi,
-                  idesc_o, i != 0 ? 1u : (uint32_t)(j != 0));
+      for (int x = TERMS - 1; x >= 0; --x)
+#pragma unroll
+        for (int i = 0; i < kTcKeys / 16; ++i)
+          tc_mma_ts(leader, tmem + L::kOut + t * 128, tmem + L::kScores + b * L::kBuffer + x * 64 + i * 8,
+                    v + (i * 2048 >> 4), kUmmaHi, idesc_o, i != 0 || x != TERMS - 1 ? 1u : (uint32_t)(j != 0));
       tc_commit_if(leader, pv_done + 8 * t);
     };
     if (n > 0) {

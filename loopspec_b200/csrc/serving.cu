@@ -183,38 +183,44 @@ struct PrefixPlan {
   size_t o_bytes, ml_bytes, total;
 };
 
-constexpr int kMaxParts = 64;   // of the prefix, and of a request's own positions
+constexpr int kMaxParts = 64;   // of a request's own positions, and of what the tcgen05 kernel does
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Key ranges of `len` positions for `units` row tiles: as many as keep
 // `resident` units on the GPU, none under `least` positions.
-void cut(long units, int len, long resident, int least, int grain, int& parts, int& chunk) {
+void cut(long units, int len, long resident, int least, int grain, int most, int& parts, int& chunk) {
   parts = chunk = 0;
   if (len == 0) return;
   const long want = std::max(1L, resident / std::max(1L, units));
-  const int most = std::max(1, cdiv(len, least));
-  parts = (int)std::min<long>(std::min<long>(want, most), kMaxParts);
+  parts = (int)std::min<long>(want, std::min(most, std::max(1, cdiv(len, least))));
   chunk = cdiv(cdiv(len, parts), grain) * grain;
   parts = cdiv(len, chunk);
 }
 
-// Eights of rows in a row tile of the stream kernel: the rows there are, up to
-// what q and O leave registers for.
-int tile_eights(long rows) { return rows <= 8 ? 1 : 2; }
+// Measured costs, in cycles of an SM. A CTA of the tcgen05 kernel fills one and
+// spends kAround besides its key tiles (lookups, first copies, results out).
+// The stream kernel spends kStreamAround on every SM.
+constexpr double kAround = 16000, kStreamAround = 6000, kJoinAround = 6000;
 
-// How many key ranges the tcgen05 kernel cuts the prefix into, and the SMs left
-// to the stream kernel, which does the requests' own positions beside it: a
-// tcgen05 CTA fills an SM, so the two share the GPU by SMs. Measured costs in
-// cycles: a CTA spends 16000 around its key tiles (lookups, first copies, parts
-// out) and 3400 a tile (two row tiles; one: 2000); the stream kernel 6000 on
-// every SM and 350 a tile of 16 keys. Fewer, longer CTAs waste less on the
-// former (33 requests of 5 drafts behind 5001 positions: 5 ranges beside the
-// stream take 44000 cycles, 10 ranges and then the stream 50000).
-void share(PrefixPlan& p, int prefix_len, double stream_cycles, int sms, int units) {
+double tc_tile_cycles(int hd, int terms, int tc_tiles) {
+  const double products = (hd == 128 ? 1030. : 520.) * terms * tc_tiles;   // both, at the tensor cores' rate
+  const double softmax = terms > 1 ? 2000 : tc_tiles == 2 ? (hd == 128 ? 3400 : 3000) : 1800;
+  return std::max(products * 1.1, softmax);
+}
+
+// ... and this a tile of 16 keys by 8 or 16 rows
+double stream_tile_cycles(int terms, int rt) { return (terms == 1 ? 300 : 450) * rt; }
+
+// How many key ranges the tcgen05 kernel cuts the shared prefix into, and the
+// SMs left to the stream kernel, which does the requests' own positions beside
+// it: the two share the GPU by SMs. Fewer, longer CTAs waste less around their
+// tiles (33 requests of 5 drafts behind 5001 positions: 5 ranges beside the
+// stream take 44000 cycles, 10 ranges and then the stream 50000). Returns the
+// cycles it expects.
+double share(PrefixPlan& p, int prefix_len, double tile_cycles, double stream_cycles, int sms, int units) {
   const int tiles = cdiv(prefix_len, kTcKeys);
-  const double per_tile = p.tc_tiles == 2 ? 3400 : 2000;
-  auto ranged = [&](int parts) { return 16000 + per_tile * cdiv(tiles, parts); };
+  auto ranged = [&](int parts) { return kAround + tile_cycles * cdiv(tiles, parts); };
   const int most = std::max(1, std::min({sms / units, tiles, kMaxParts}));
   double best = 0;
   for (int parts = 1; parts <= most; ++parts) {
@@ -231,40 +237,64 @@ void share(PrefixPlan& p, int prefix_len, double stream_cycles, int sms, int uni
     }
   }
   p.prefix_parts = cdiv(prefix_len, p.prefix_chunk);
+  return best;
 }
 
+// Eights of rows in a row tile of the stream kernel: the rows there are, up to
+// what q and O leave registers for.
+int tile_eights(long rows) { return rows <= 8 ? 1 : 2; }
+
+// terms: 1 for 16-bit q, else those of an fp32 q (see prefix_attn.cuh).
 PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int prefix_len, int max_new,
-                     int max_len, bool split_q, int sms) {
+                     int max_len, int terms, int sms) {
   PrefixPlan p{};
   const int G = nh / nkv;
   const long rows = (long)n_tokens * G;
-  const long most_new = std::min(max_new, n_tokens);
-  // Requests that bring whole tiles of rows on average do not need each other
-  // to fill one: their own positions then follow the prefix in the same unit.
-  p.own = !split_q && rows >= (long)kTcRows * n_requests;
-  p.suffix_rt = tile_eights(most_new * G);
-  p.suffix_tiles = cdiv(most_new * G, 8 * p.suffix_rt);
+  const long most_rows = (long)std::min(max_new, n_tokens) * G, mean_rows = cdiv(rows, n_requests);
+
+  // one way: the prefix for all rows together, the requests' own positions by the stream kernel
+  p.suffix_rt = tile_eights(most_rows);
+  p.suffix_tiles = cdiv(most_rows, 8 * p.suffix_rt);
   p.stream_sms = sms;
-  if (p.own) {
-    p.tc_tiles = most_new * G > kTcRows ? 2 : 1;
-    p.prefix_tiles = cdiv(most_new * G, kTcRows * p.tc_tiles);
-    const long units = (rows / (kTcRows * p.tc_tiles) + 1) * nkv;
-    cut(units, prefix_len, sms, 2 * kTcKeys, kTcKeys, p.prefix_parts, p.prefix_chunk);
+  const double own_tiles = (double)n_requests * nkv * cdiv(mean_rows, 8 * p.suffix_rt) * max_len / 16 / 2;
+  const double stream_cycles = max_len ? stream_tile_cycles(terms, p.suffix_rt) * own_tiles + kStreamAround * sms : 0;
+  double cycles = stream_cycles / sms + kJoinAround;
+  if (rows > 16 && prefix_len > 0) {
+    p.tc_tiles = terms > 1 || rows <= kTcRows ? 1 : 2;
+    p.prefix_tiles = cdiv(rows, kTcRows * p.tc_tiles);
+    const int units = (int)std::min<long>((long)p.prefix_tiles * nkv, 1 << 20);
+    cycles = share(p, prefix_len, tc_tile_cycles(hd, terms, p.tc_tiles), stream_cycles, sms, units) + kJoinAround;
   } else {
-    p.tc_tiles = split_q || rows <= 16 || prefix_len == 0 ? 0 : rows > kTcRows ? 2 : 1;
-    if (p.tc_tiles) {
-      p.prefix_tiles = cdiv(rows, kTcRows * p.tc_tiles);
-      const double own_tiles = (double)n_requests * nkv * cdiv(cdiv(rows, n_requests), 8 * p.suffix_rt) * max_len / 16 / 2;
-      const long units = (long)p.prefix_tiles * nkv;
-      share(p, prefix_len, max_len ? 350 * own_tiles + 6000. * sms : 0, sms, (int)std::min<long>(units, 1 << 20));
-    } else {
-      // one launch for both if it reads the prefix no more than four times (from L2)
-      p.prefix_rt = rows <= 32 ? p.suffix_rt : tile_eights(rows);
-      p.prefix_tiles = cdiv(rows, 8 * p.prefix_rt);
-      cut((long)p.prefix_tiles * nkv, prefix_len, 12L * sms, 64, 16, p.prefix_parts, p.prefix_chunk);
+    // one launch for both if it reads the prefix no more than twice (from L2)
+    p.prefix_rt = p.suffix_rt;
+    p.prefix_tiles = cdiv(rows, 8 * p.prefix_rt);
+    cut((long)p.prefix_tiles * nkv, prefix_len, 12L * sms, 64, 16, 4 * kMaxParts, p.prefix_parts, p.prefix_chunk);
+  }
+  // lengths are spread below max_len: two ranges a warp (12 an SM) even that out
+  cut((long)p.suffix_tiles * nkv * n_requests, max_len, 24L * p.stream_sms, 64, 16, kMaxParts, p.suffix_parts,
+      p.suffix_chunk);
+
+  // the other way, for requests that bring about a tile of rows: each by itself, prefix and own positions
+  if (most_rows > 16) {
+    const int mt = terms > 1 || most_rows <= kTcRows ? 1 : 2;
+    const int tiles = cdiv(prefix_len, kTcKeys) + cdiv(max_len, kTcKeys);
+    const double units = (double)n_requests * nkv * cdiv(mean_rows, kTcRows * mt);
+    for (int parts = 1; parts <= std::min(tiles, kMaxParts); ++parts) {
+      const int each = cdiv(tiles, parts);
+      const double ctas = units * cdiv(tiles, each);
+      const double by_itself = (kAround + tc_tile_cycles(hd, terms, mt) * each) * std::ceil(ctas / sms) +
+                               (parts > 1 ? kJoinAround : 0);
+      if (by_itself < cycles) {
+        cycles = by_itself;
+        p.own = true;
+        p.tc_tiles = mt;
+        p.prefix_tiles = cdiv(most_rows, kTcRows * mt);
+        p.prefix_chunk = each * kTcKeys;
+        p.prefix_parts = cdiv(tiles, each);
+        p.suffix_parts = 0;
+      }
+      if (ctas > 2.0 * sms) break;
     }
-    // lengths are spread below max_len: two ranges a warp (12 an SM) even that out
-    cut((long)p.suffix_tiles * nkv * n_requests, max_len, 24L * p.stream_sms, 64, 16, p.suffix_parts, p.suffix_chunk);
   }
   const bool direct = p.own && p.prefix_parts <= 1;   // whole results, no parts to keep
   const size_t part_rows = direct ? 0 : (size_t)(p.prefix_parts + p.suffix_parts) * n_tokens * nh;
@@ -274,23 +304,22 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
   return p;
 }
 
-template <int HD, typename C, int MT>
+template <int HD, typename Q, typename C, int TERMS, int MT>
 void launch_tc(const PrefixAttnArgs& a, cudaStream_t stream) {
-  const size_t smem = TcLayout<HD, MT>::kSmem;
-  allow_smem<prefix_tc_kernel<HD, C, MT>>(smem);
+  using L = TcLayout<HD, TERMS, MT>;
+  allow_smem<prefix_tc_kernel<HD, Q, C, TERMS, MT>>(L::kSmem);
   // the register hand-over inside the kernel waits for good if the launch holds less than it shares out
   static const int regs = [] {
     cudaFuncAttributes attr = {};
-    CK(cudaFuncGetAttributes(&attr, prefix_tc_kernel<HD, C, MT>));
+    CK(cudaFuncGetAttributes(&attr, prefix_tc_kernel<HD, Q, C, TERMS, MT>));
     return attr.numRegs;
   }();
-  constexpr int kNeed = TcLayout<HD, MT>::kLaunchRegs;
-  REQUIRE(regs >= kNeed, LS_ECUDA,
+  REQUIRE(regs >= L::kLaunchRegs, LS_ECUDA,
           "prefix attention: built with " + std::to_string(regs) + " registers a thread, fewer than it shares out");
   const long units = (long)a.prefix_tiles * a.nkv * std::max(1, a.prefix_parts) * (a.own ? a.n_requests : 1);
   REQUIRE(units <= INT32_MAX, LS_EINVAL, "prefix attention: too many units for one launch");
-  launch(prefix_tc_kernel<HD, C, MT>, dim3((unsigned)units),
-         dim3(TcLayout<HD, MT>::kThreads), smem, stream, false, a);
+  launch(prefix_tc_kernel<HD, Q, C, TERMS, MT>, dim3((unsigned)units), dim3(L::kThreads), (size_t)L::kSmem, stream,
+         false, a);
 }
 
 // The stream kernel over the prefix, the requests' own positions or both.
@@ -316,9 +345,9 @@ void launch_stream(const PrefixAttnArgs& a, int rt, bool prefix, bool suffix, bo
 
 template <int HD, typename Q, typename C, int TERMS>
 void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& plan, cudaStream_t stream) {
+  if (plan.tc_tiles == 1) launch_tc<HD, Q, C, TERMS, 1>(a, stream);
   if constexpr (TERMS == 1) {
-    if (plan.tc_tiles == 1) launch_tc<HD, C, 1>(a, stream);
-    if (plan.tc_tiles == 2) launch_tc<HD, C, 2>(a, stream);
+    if (plan.tc_tiles == 2) launch_tc<HD, Q, C, TERMS, 2>(a, stream);
   }
   if (a.direct) return;
   const bool prefix = plan.tc_tiles == 0 && a.prefix_parts > 0, suffix = a.suffix_parts > 0 && a.suffix_tiles > 0;
@@ -381,7 +410,7 @@ void run_prefix_attention(const ls_prefix_attention_args& p, cudaStream_t stream
               p.q_stride * eb % 16 == 0 && p.out_stride * eb % 16 == 0 && p.slot_stride * 2 % 16 == 0,
           LS_EINVAL, "prefix attention: pointers and row strides must be 16-byte aligned");
   const PrefixPlan plan = make_plan(p.n_tokens, p.n_requests, p.n_heads, p.n_kv_heads, p.head_dim, p.prefix_len,
-                                    p.max_new, p.max_len, p.q_type == LS_F32, sm_count());
+                                    p.max_new, p.max_len, p.q_type != LS_F32 ? 1 : p.cache_type == LS_BF16 ? 3 : 2, sm_count());
   REQUIRE((reinterpret_cast<uintptr_t>(p.workspace) & 255) == 0, LS_EINVAL,
           "prefix attention: workspace must be 256-byte aligned");
   REQUIRE(p.workspace_bytes >= plan.total, LS_EINVAL,
@@ -481,9 +510,9 @@ size_t ls_prefix_attention_workspace_bytes(int n_tokens, int n_requests, int n_h
   size_t bytes = 0;
   guarded([&] {
     check_prefix_sizes(n_tokens, n_requests, n_heads, n_kv_heads, head_dim, prefix_len, max_new, max_len);
-    for (const bool split_q : {false, true})   // enough for either type of q
+    for (const int terms : {1, 2, 3})   // enough for any type of q
       bytes = std::max({(size_t)256, bytes, make_plan(n_tokens, n_requests, n_heads, n_kv_heads, head_dim, prefix_len,
-                                                      max_new, max_len, split_q, sm_count()).total});
+                                                      max_new, max_len, terms, sm_count()).total});
   });
   return bytes;   // 0: refused, see ls_last_error(NULL)
 }

@@ -190,12 +190,23 @@ def test_tokens_that_see_nothing_and_padding_get_zeros():
     ([300, 1, 40], [300, 1, 129], 513, 9, 3),     # requests of one and of several tiles
     ([130, 140], [128, 100], 0, 4, 4),            # more new tokens than positions: the first see nothing
     ([256, 257], [256, 513], 127, 1, 1),
+    ([200], [1500], 200, 8, 2),                   # own positions in several key ranges
 ])
 def test_prompts_behind_a_prefix(counts, lens, prefix, nh, nkv, hd, kind, cache):
     c = make(counts, lens, prefix, 16, nh, nkv, hd, kind, cache, seed=sum(counts) + prefix, pad=3, fill=float("nan"))
     out = call(c, 16)
     near(out, c, 16, kind, cache)
     assert not bool(out[-3:].any())
+
+
+@pytest.mark.parametrize("kind,cache", ALL)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("requests,nh,nkv", [(20, 32, 32), (40, 128, 32)])
+def test_many_key_tiles_in_one_unit(requests, nh, nkv, hd, kind, cache):
+    """Enough kv heads that a unit walks many key tiles: every stage of its ring is used several times."""
+    prefix = 2600 if requests == 20 else 1400
+    c = make([1] * requests, [1 + i % 3 for i in range(requests)], prefix, 16, nh, nkv, hd, kind, cache, seed=hd)
+    near(call(c, 16), c, 16, kind, cache)
 
 
 @pytest.mark.parametrize("kind,cache", [("bf16", "bf16"), ("f16", "f16")])
