@@ -74,6 +74,7 @@ struct PrefixAttnArgs {
   int suffix_parts, suffix_chunk;    // ... of max_len own positions
   int prefix_tiles, suffix_tiles;    // row tiles, of their kernels' rows
   bool prefix_units, suffix_units;   // what a launch of the stream kernel does
+  bool behind;                       // it runs beside a kernel of the same call
   bool own, direct;                  // tcgen05 kernel: rows of one request and its own positions; whole results
   int* status;
 };
@@ -249,6 +250,10 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
   const int gid = lane >> 2, tig = lane & 3;
   const int G = a.nh / a.nkv;
   const int mask = (1 << a.page_shift) - 1;
+  // A call's first kernel is launched early: it waits for what came before, and
+  // only then lets the next one start. Behind another kernel of the call its
+  // inputs are there; it waits at the end, so that it is not done before that one.
+  if (!a.behind) pdl_wait();
   pdl_launch_dependents();
   unsigned char* ring = s_ring + (size_t)warp * ST * unit_stage_bytes<HD>();
   const int W = gridDim.x * kUnitWarps, w = warp * gridDim.x + blockIdx.x;
@@ -570,8 +575,7 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
     }
     cp_async_wait<0>();
   }
-  // a prefix kernel ahead of this one runs on beside it; this grid is not done before that one is
-  pdl_wait();
+  if (a.behind) pdl_wait();
 }
 
 __device__ __forceinline__ void store4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
@@ -598,7 +602,9 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
   __shared__ float2 s_ml[GROUPS];
   __shared__ int s_len;
   const int t = blockIdx.x;
-  // whether a valid request holds the token: written by nobody ahead of this kernel
+  if (!a.behind) pdl_wait();
+  pdl_launch_dependents();   // the next call's first kernel, which waits for this one
+  // whether a valid request holds the token: written by no kernel of the call
   bool mine = false;
   for (int i = threadIdx.x; i < a.n_requests; i += kJoinThreads) {
     const int start = a.token_start[i], end = a.token_start[i + 1], len = a.lens[i];
@@ -609,7 +615,7 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
     }
   }
   const bool ok = __syncthreads_or(mine);
-  pdl_wait();
+  if (a.behind) pdl_wait();
   const int group = threadIdx.x / TPR, c = (threadIdx.x % TPR) * 4;
   const int h = SPLIT ? blockIdx.y : blockIdx.y * GROUPS + group;
   if (!SPLIT && h >= a.nh) return;

@@ -301,6 +301,9 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
   const uint32_t full0 = bars, empty0 = full0 + 8 * ST, s_full = empty0 + 8 * ST, p_full = s_full + 16,
                  pv_done = p_full + 16, q_full = pv_done + 16, noted = q_full + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // the first kernel of a call: launched early, it waits for what came before,
+  // and only then lets the next one start
+  pdl_wait();
   pdl_launch_dependents();
 
   // the unit: its rows, and its keys as prefix positions [ka0, ka1) and own positions [kb0, kb1)
@@ -342,9 +345,9 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
   const int n_shared = (a.prefix_len + kTcKeys - 1) / kTcKeys;
   const int ka0 = min(a.prefix_len, j0 * kTcKeys), ka1 = min(a.prefix_len, j1 * kTcKeys);
   const int last_row = min(rows, row0 + MT * kTcRows) - 1;
-  const int see_first = seen0 + row0 / G;          // own positions every row sees, and some row sees
+  const int see_first = seen0 + div_by(row0, G, a.g_magic);          // own positions every row sees, and some row sees
   const int kb0 = max(0, j0 - n_shared) * kTcKeys;
-  const int kb1 = a.own ? min(max(0, j1 - n_shared) * kTcKeys, min(len, seen0 + last_row / G)) : 0;
+  const int kb1 = a.own ? min(max(0, j1 - n_shared) * kTcKeys, min(len, seen0 + div_by(last_row, G, a.g_magic))) : 0;
   const int na = (ka1 - ka0 + kTcKeys - 1) / kTcKeys;
   const int n = na + (max(0, kb1 - kb0) + kTcKeys - 1) / kTcKeys;    // key tiles
   const int* own_table = a.block_table + req * a.table_stride;
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         const int i = (threadIdx.x & 255) + 256 * k, r = i / CH, c = i % CH, rr = row0 + t * kTcRows + r;
         v[k] = Raw8<Q>();
         if (rr < rows) {
-          const int tok = rr / G, h = g * G + rr - tok * G;
+          const int tok = div_by(rr, G, a.g_magic), h = g * G + rr - tok * G;
           v[k].load(q + (long)(start + tok) * a.q_stride + (long)h * HD + c * 8);
         }
       }
@@ -422,7 +425,8 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
       const uint32_t out = lanes + L::kOut + t * 128 + half * (HD / 2);
       // own positions this row sees, within the unit's
-      const int see = rr < rows ? min(kb1, seen0 + rr / G) : kb1;
+      const int row_tok = div_by(rr, G, a.g_magic);
+      const int see = rr < rows ? min(kb1, seen0 + row_tok) : kb1;
       const int see_least = __reduce_min_sync(0xffffffffu, see);
       float m = -INFINITY, l = 0.f;
       bool ok = true;
@@ -523,7 +527,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       row_sum[half * kTcRows] = l;
       asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
       l = row_sum[0] + row_sum[kTcRows];
-      const int tok = start + rr / G, h = g * G + rr % G;
+      const int tok = start + row_tok, h = g * G + rr - row_tok * G;
       const float inv = !have ? 0.f : !a.direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
       const long at = ((long)part * a.n_tokens + tok) * a.nh + h;
       if (!a.direct && rr < rows && half == 0)

@@ -210,7 +210,7 @@ double tc_tile_cycles(int hd, int terms, int tc_tiles) {
 }
 
 // ... and this a tile of 16 keys by 8 or 16 rows
-double stream_tile_cycles(int terms, int rt) { return (terms == 1 ? 300 : 450) * rt; }
+double stream_tile_cycles(int terms, int rt) { return terms == 1 ? (rt == 1 ? 300 : 560) : (rt == 1 ? 450 : 1000); }
 
 // How many key ranges the tcgen05 kernel cuts the shared prefix into, and the
 // SMs left to the stream kernel, which does the requests' own positions beside
@@ -227,7 +227,7 @@ double share(PrefixPlan& p, int prefix_len, double tile_cycles, double stream_cy
     const int ctas = units * cdiv(tiles, cdiv(tiles, parts));
     const double after = ranged(parts) * cdiv(ctas, sms) + stream_cycles / sms;
     // lengths are only bounded: never stretch the prefix far for the sake of the rest
-    const double beside = ctas < sms && ranged(parts) <= 1.6 * ranged(most)
+    const double beside = ctas < sms && ranged(parts) <= 2 * ranged(most)
                               ? std::max(ranged(parts), stream_cycles / (sms - ctas)) : after;
     const double cycles = std::min(after, beside);
     if (best == 0 || cycles < best) {
@@ -319,7 +319,7 @@ void launch_tc(const PrefixAttnArgs& a, cudaStream_t stream) {
   const long units = (long)a.prefix_tiles * a.nkv * std::max(1, a.prefix_parts) * (a.own ? a.n_requests : 1);
   REQUIRE(units <= INT32_MAX, LS_EINVAL, "prefix attention: too many units for one launch");
   launch(prefix_tc_kernel<HD, Q, C, TERMS, MT>, dim3((unsigned)units), dim3(L::kThreads), (size_t)L::kSmem, stream,
-         false, a);
+         true, a);
 }
 
 // The stream kernel over the prefix, the requests' own positions or both.
@@ -331,10 +331,11 @@ void launch_stream(PrefixAttnArgs a, bool prefix, bool suffix, bool behind, int 
   REQUIRE(units <= INT32_MAX / 2, LS_EINVAL, "prefix attention: too many units for one launch");   // and a stride past the last
   a.prefix_units = prefix;
   a.suffix_units = suffix;
+  a.behind = behind;
   const size_t smem = unit_smem_bytes<HD, TERMS, RT>();
   allow_smem<prefix_stream_kernel<HD, Q, C, TERMS, RT>>(smem);
   const long ctas = std::min<long>((long)unit_ctas<HD, TERMS, RT>() * sms, cdiv(units, kUnitWarps));
-  launch(prefix_stream_kernel<HD, Q, C, TERMS, RT>, dim3((unsigned)ctas), dim3(kUnitThreads), smem, stream, behind, a);
+  launch(prefix_stream_kernel<HD, Q, C, TERMS, RT>, dim3((unsigned)ctas), dim3(kUnitThreads), smem, stream, true, a);
 }
 
 template <int HD, typename Q, typename C, int TERMS>
@@ -344,7 +345,7 @@ void launch_stream(const PrefixAttnArgs& a, int rt, bool prefix, bool suffix, bo
 }
 
 template <int HD, typename Q, typename C, int TERMS>
-void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& plan, cudaStream_t stream) {
+void launch_prefix(PrefixAttnArgs a, const PrefixPlan& plan, cudaStream_t stream) {
   if (plan.tc_tiles == 1) launch_tc<HD, Q, C, TERMS, 1>(a, stream);
   if constexpr (TERMS == 1) {
     if (plan.tc_tiles == 2) launch_tc<HD, Q, C, TERMS, 2>(a, stream);
@@ -361,13 +362,13 @@ void launch_prefix(const PrefixAttnArgs& a, const PrefixPlan& plan, cudaStream_t
     if (suffix) launch_stream<HD, Q, C, TERMS>(a, plan.suffix_rt, false, true, behind, plan.stream_sms, stream);
     behind = behind || suffix;
   }
-  // early only behind kernels of this call: it reads the lengths before it waits
+  a.behind = behind;
   constexpr int kGroups = kJoinThreads / (HD / 4);
   const dim3 rows((unsigned)a.n_tokens, (unsigned)a.nh), groups((unsigned)a.n_tokens, (unsigned)cdiv(a.nh, kGroups));
   // a row's parts are shared out where there are too few rows to keep the GPU busy
   if (a.prefix_parts + a.suffix_parts > kJoinBatch && (long)groups.x * groups.y < 16L * sm_count())
-    launch(prefix_join_kernel<HD, Q, true>, rows, dim3(kJoinThreads), 0, stream, behind, a);
-  else launch(prefix_join_kernel<HD, Q, false>, groups, dim3(kJoinThreads), 0, stream, behind, a);
+    launch(prefix_join_kernel<HD, Q, true>, rows, dim3(kJoinThreads), 0, stream, true, a);
+  else launch(prefix_join_kernel<HD, Q, false>, groups, dim3(kJoinThreads), 0, stream, true, a);
 }
 
 template <typename Q, typename C, int TERMS>
