@@ -61,7 +61,7 @@ struct TcLayout {
   static constexpr int kSoftRegs = 104, kRestRegs = 64;
   static constexpr int kLaunchRegs = MT == 2 ? (512 * kSoftRegs + 128 * kRestRegs) / kThreads : 0;
   static constexpr int kMaxBuffers = MT == 1 ? 2 : 1;      // see the softmax warps
-  static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 1 + 1;
+  static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 2 + 1 + 1;
   static constexpr int kQTiles = MT * TERMS;
   static constexpr int kSmem = kQTiles * kTile + kStages * kTile + kMaxBuffers * MT * 2 * kTcRows * 4 + kBars * 8 + 8 * 4 + 16;
   static constexpr int kPoly = TERMS == 1 ? 2 : 0;         // eighths of the exponentials on the FMA units
@@ -155,6 +155,15 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+
+// Wait for this thread's loads into r. The registers pass through the wait, so
+// that no arithmetic on them is moved ahead of it.
+template <int N>
+__device__ __forceinline__ void tmem_ld_done(uint32_t (&r)[N]) {
+  tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i])::"memory");
 }
 
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -299,7 +308,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
   uint32_t* s_bad = reinterpret_cast<uint32_t*>(s_max + L::kMaxBuffers * MT * 2 * kTcRows) + 2 * L::kBars;   // [8] bits
   uint32_t* s_tmem = s_bad + 8;
   const uint32_t full0 = bars, empty0 = full0 + 8 * ST, s_full = empty0 + 8 * ST, p_full = s_full + 16,
-                 pv_done = p_full + 16, q_full = pv_done + 16, noted = q_full + 8;
+                 pv_done = p_full + 16, o_done = pv_done + 16, q_full = o_done + 16, noted = q_full + 8;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // the first kernel of a call: launched early, it waits for what came before,
   // and only then lets the next one start
@@ -364,6 +373,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       // with MT = 2 a buffer belongs to a row tile; one without rows is never used
       mbar_init(p_full + 8 * b, max(1, 2 * live_warps(MT == 2 ? b : 0)));
       mbar_init(pv_done + 8 * b, 1);
+      mbar_init(o_done + 8 * b, 1);
     }
     mbar_init(q_full, 8 * MT);
     mbar_init(noted, L::kProducers);
@@ -442,7 +452,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         uint32_t s[64];
         tmem_ld_x32(sc + half * 64, s);
         tmem_ld_x32(sc + half * 64 + 32, s + 32);
-        tmem_ld_wait();
+        tmem_ld_done(s);
         if (cut) {
 #pragma unroll
           for (int i = 0; i < 64; ++i)
@@ -476,7 +486,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
             for (int c = 0; c < HD / 2; c += 16) {
               uint32_t v[16];
               tmem_ld_x16(out + c, v);
-              tmem_ld_wait();
+              tmem_ld_done(v);
 #pragma unroll
               for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * keep);
               tmem_st_x16(out + c, v);
@@ -519,7 +529,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         if (lane == 0) mbar_arrive(p_full + 8 * b);
       }
       // join the two halves' sums; a wait that timed out leaves zeros
-      if (n > 0) wait_on(ok, pv_done + 8 * t, (n - 1) & 1, a.status, kDevTimeoutAcc);
+      if (n > 0) wait_on(ok, o_done + 8 * t, 0, a.status, kDevTimeoutAcc);
       if (a.own) wait_on(ok, noted, 0, a.status, kDevTimeoutAcc);
       const bool have = n > 0 && ok;
       tc_fence_after();
@@ -545,7 +555,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       for (int c = 0; c < HD / 2; c += 16) {
         uint32_t v[16];
         tmem_ld_x16(out + c, v);
-        tmem_ld_wait();
+        tmem_ld_done(v);
         float f[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[i] = have ? __uint_as_float(v[i]) * inv : 0.f;
@@ -697,7 +707,11 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         for (int i = 0; i < kTcKeys / 16; ++i)
           tc_mma_ts(leader, tmem + L::kOut + t * 128, tmem + L::kScores + b * L::kBuffer + x * 64 + i * 8,
                     v + (i * 2048 >> 4), kUmmaHi, idesc_o, i != 0 || x != TERMS - 1 ? 1u : (uint32_t)(j != 0));
+      // A softmax warp at tile j may wait for product j - 1: it knows of j - 2, so
+      // the turn is plain. For the last product, which it could be two turns
+      // ahead of, there is a barrier of its own.
       tc_commit_if(leader, pv_done + 8 * t);
+      if (j == n - 1) tc_commit_if(leader, o_done + 8 * t);
     };
     if (n > 0) {
       wait_on(ok, q_full, 0, a.status, kDevTimeoutFull);
