@@ -64,7 +64,11 @@ struct TcLayout {
   static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 2 + 1 + 1;
   static constexpr int kQTiles = MT * TERMS;
   static constexpr int kSmem = kQTiles * kTile + kStages * kTile + kMaxBuffers * MT * 2 * kTcRows * 4 + kBars * 8 + 8 * 4 + 16;
-  static constexpr int kPoly = TERMS == 1 ? 2 : 0;         // eighths of the exponentials on the FMA units
+  // Eighths of the exponentials on the FMA units. The softmax is bound by issue
+  // slots: with heads of 128 the tensor cores take longer and none is best
+  // (0, 1, 2, 3 eighths: 289, 296, 308, 326 us for 2100 tokens behind 8192
+  // positions), with heads of 64 one (740, 633, 664, 663 us for 3050 behind 16384).
+  static constexpr int kPoly = TERMS == 1 && HD == 64 ? 1 : 0;
   // tensor memory columns: two buffers of scores, each with room for P's terms (64 each) over them, then O
   static constexpr uint32_t kScores = 0, kBuffer = TERMS == 3 ? 192 : 128, kOut = 2 * kBuffer;
   static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");

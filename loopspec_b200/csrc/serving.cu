@@ -198,6 +198,10 @@ void cut(long units, int len, long resident, int least, int grain, int most, int
   parts = cdiv(len, chunk);
 }
 
+// Fewest keys of a stream unit: 64, or 32 where that leaves most SMs idle (4
+// requests behind 333 positions: 10.3 -> 8.3 us; 16 behind 2048: 23.0 -> 24.5).
+int least_keys(long units, int len, int sms) { return units * cdiv(len, 64) <= 2L * sms ? 32 : 64; }
+
 // Measured costs, in cycles of an SM. A CTA of the tcgen05 kernel fills one and
 // spends kAround besides its key tiles (lookups, first copies, results out).
 // The stream kernel spends kStreamAround on every SM.
@@ -268,10 +272,13 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
     // one launch for both if it reads the prefix no more than twice (from L2)
     p.prefix_rt = p.suffix_rt;
     p.prefix_tiles = cdiv(rows, 8 * p.prefix_rt);
-    cut((long)p.prefix_tiles * nkv, prefix_len, 12L * sms, 64, 16, 4 * kMaxParts, p.prefix_parts, p.prefix_chunk);
+    const long units = (long)p.prefix_tiles * nkv;
+    cut(units, prefix_len, 12L * sms, least_keys(units, prefix_len, sms), 16, 4 * kMaxParts, p.prefix_parts,
+        p.prefix_chunk);
   }
   // lengths are spread below max_len: two ranges a warp (12 an SM) even that out
-  cut((long)p.suffix_tiles * nkv * n_requests, max_len, 24L * p.stream_sms, 64, 16, kMaxParts, p.suffix_parts,
+  const long own_units = (long)p.suffix_tiles * nkv * n_requests;
+  cut(own_units, max_len, 24L * p.stream_sms, least_keys(own_units, max_len, sms), 16, kMaxParts, p.suffix_parts,
       p.suffix_chunk);
 
   // the other way, for requests that bring about a tile of rows: each by itself, prefix and own positions
