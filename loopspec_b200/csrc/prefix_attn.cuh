@@ -603,7 +603,9 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
   __shared__ int s_len;
   const int t = blockIdx.x;
   if (!a.behind) pdl_wait();
-  pdl_launch_dependents();   // the next call's first kernel, which waits for this one
+  // no early launch of what follows: CTAs of the next call that wait here took
+  // the places of this call's last ones (16 requests behind 2048 positions with
+  // fp32 queries, call after call: 31.6 us with it, 22.6 without)
   // whether a valid request holds the token: written by no kernel of the call
   bool mine = false;
   for (int i = threadIdx.x; i < a.n_requests; i += kJoinThreads) {
