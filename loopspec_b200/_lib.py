@@ -192,6 +192,25 @@ def lib():
     return _LIB
 
 
+_FACTS = None
+
+
+def tensor_facts():
+    """facts and pointers of csrc/tensor_facts.cpp: tensor arguments looked over
+    in one call each, for the operators whose whole call takes microseconds."""
+    global _FACTS
+    if _FACTS is None:
+        try:
+            from . import _tensor_facts
+        except ImportError as e:
+            raise ImportError(f"{e}: build it with `python -c 'import loopspec_b200.build as b; b.build()'`") from e
+        _FACTS = _tensor_facts.facts, _tensor_facts.pointers
+    return _FACTS
+
+
+BF16, F16, F32, I32, BYTE = range(5)   # type codes: LS_BF16, LS_F16, LS_F32, and those of index and scratch tensors
+
+
 class EngineError(RuntimeError):
     def __init__(self, code, message):
         super().__init__(f"[{code}] {message}")

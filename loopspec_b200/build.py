@@ -1,4 +1,5 @@
-"""Build libloopspec_engine.so in-tree for sm_100a with nvcc.
+"""Build libloopspec_engine.so in-tree for sm_100a with nvcc, and beside it the
+CPython module _tensor_facts.so (host code that reads torch tensors).
 
     python -m loopspec_b200.build            # rebuild if any source is newer
     python -m loopspec_b200.build --force
@@ -11,12 +12,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 # translation units compiled in parallel, then linked into one library
 SRCS = [os.path.join(HERE, "csrc", name) for name in ("engine.cu", "serving.cu")]
 OUT = os.path.join(HERE, "libloopspec_engine.so")
+FACTS_SRC = os.path.join(HERE, "csrc", "tensor_facts.cpp")
+FACTS_OUT = os.path.join(HERE, "_tensor_facts.so")
 OBJ_DIR = os.path.join(HERE, "_build")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -24,7 +28,7 @@ NVCC_FLAGS = [*ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-
 
 
 def _sources():
-    return glob.glob(os.path.join(HERE, "csrc", "*")) + glob.glob(os.path.join(ROOT, "include", "*.h"))
+    return glob.glob(os.path.join(HERE, "csrc", "*.cu*")) + glob.glob(os.path.join(ROOT, "include", "*.h"))
 
 
 def _nvcc():
@@ -35,6 +39,37 @@ def _nvcc():
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
+    facts = build_facts(force)
+    try:
+        return build_engine(force, verbose)
+    finally:
+        finish_facts(facts)
+
+
+def build_facts(force):
+    """Start the compiler on the tensor module; None if it is newer than its source."""
+    if not force and os.path.exists(FACTS_OUT) and os.path.getmtime(FACTS_OUT) >= os.path.getmtime(FACTS_SRC):
+        return None
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{path}" for path in includes), "-o", FACTS_OUT + ".tmp",
+           FACTS_SRC, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+
+
+def finish_facts(proc):
+    if proc is None:
+        return
+    text, _ = proc.communicate()
+    if proc.returncode != 0:
+        raise RuntimeError("g++ failed:\n" + text)
+    os.replace(FACTS_OUT + ".tmp", FACTS_OUT)
+
+
+def build_engine(force: bool, verbose: bool) -> str:
     if not force and os.path.exists(OUT):
         newest = max(os.path.getmtime(p) for p in _sources())
         if os.path.getmtime(OUT) >= newest:

@@ -12,11 +12,10 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .qk_norm import TYPE_CODES, check_pools
+from .qk_norm import FLOATS, check_pools
 from .status import enqueue, on_stream
 
 _pack = _lib.packer(_lib.PrefixAttentionArgs)
-_i32 = torch.int32
 
 
 def workspace_bytes(n_tokens, n_heads, n_kv_heads, head_dim, *, n_requests, prefix_len, max_new, max_len):
@@ -42,45 +41,50 @@ def prefix_attention(q, k_pool, v_pool, prefix_table, prefix_len, block_table, l
     workspace    uint8 CUDA tensor of workspace_bytes(...) bytes, kept by the caller or made here;
                  calls that share one must be on one stream
     """
-    n_slots, n_kv, hd, slot_stride = check_pools(k_pool, v_pool, "prefix attention")
-    shape, row, dtype = q.shape, q.stride(), q.dtype
-    n, nh, width = shape
-    if not (width == hd and q.is_cuda and row[2] == 1 and row[1] == hd and dtype in TYPE_CODES):
+    facts, pointers = _lib.tensor_facts()
+    k_ptr, v_ptr, gpu, cache, n_slots, n_kv, hd, slot_stride = check_pools(k_pool, v_pool, "prefix attention")
+    x = facts(q)
+    if not (x and len(x) == 9 and x[1] == gpu and x[2] in FLOATS and x[5] == hd and x[8] == 1 and x[7] == hd):
         raise ValueError("prefix attention: q must be a CUDA tensor [T, n_heads, head_dim] with contiguous rows")
-    n_req, blocks = block_table.shape
-    columns = block_table.stride()
-    if not (block_table.dtype is _i32 and block_table.is_cuda and (blocks <= 1 or columns[1] == 1)):
+    x_ptr, _, code, n, nh, _, row = x[:7]
+    table = facts(block_table)
+    if not (table and len(table) == 7 and table[1] == gpu and table[2] == _lib.I32
+            and (table[4] <= 1 or table[6] == 1)):
         raise ValueError("prefix attention: block_table must be an int32 CUDA tensor with contiguous rows")
-    if not (lens.dtype is _i32 and token_start.dtype is _i32 and lens.is_cuda and token_start.is_cuda
-            and lens.is_contiguous() and token_start.is_contiguous() and lens.numel() == n_req
-            and token_start.numel() == n_req + 1):
+    table_ptr, _, _, n_req, blocks, columns, _ = table
+    ptrs = pointers(gpu, _lib.I32, lens, n_req, token_start, n_req + 1)
+    if ptrs is None:
         raise ValueError("prefix attention: lens [n_requests] and token_start [n_requests + 1] must be int32 "
                          "contiguous CUDA tensors")
     if max_len is None:
         max_len = blocks * page_size
     if not (page_size >= 1 and max_len <= blocks * page_size):
         raise ValueError("prefix attention: max_len exceeds the block table")
-    if prefix_len and not (prefix_table is not None and prefix_table.dtype is _i32 and prefix_table.is_cuda
-                           and prefix_table.is_contiguous() and prefix_table.numel() * page_size >= prefix_len > 0):
-        raise ValueError("prefix attention: prefix_table must be an int32 contiguous CUDA tensor that covers prefix_len")
+    shared = (0,)
+    if prefix_len:
+        shared = pointers(gpu, _lib.I32, prefix_table, -1)
+        if not (shared and prefix_table is not None and prefix_table.numel() * page_size >= prefix_len > 0):
+            raise ValueError("prefix attention: prefix_table must be an int32 contiguous CUDA tensor that covers "
+                             "prefix_len")
     if scale is None:
         scale = hd ** -0.5
     if out is None or workspace is None:
         with on_stream(q.device, stream):
             if out is None:
-                out = torch.empty(n, nh, hd, dtype=dtype, device=q.device)
+                out = torch.empty(n, nh, hd, dtype=q.dtype, device=q.device)
             if workspace is None:
                 need = workspace_bytes(n, nh, n_kv, hd, n_requests=n_req, prefix_len=prefix_len, max_new=max_new,
                                        max_len=max_len)
                 workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    to = out.stride()
-    if not (out.shape == shape and out.dtype is dtype and out.is_cuda and to[2] == 1 and to[1] == hd):
+    to = facts(out)
+    if not (to and to[1:6] == x[1:6] and to[8] == 1 and to[7] == hd):
         raise ValueError("prefix attention: out must be a CUDA tensor of q's shape and type with contiguous rows")
-    before = (q.data_ptr(), row[0] if n > 1 else nh * hd, k_pool.data_ptr(), v_pool.data_ptr(), slot_stride,
-              prefix_table.data_ptr() if prefix_len else 0, block_table.data_ptr(),
-              columns[0] if n_req > 1 else blocks, lens.data_ptr(), token_start.data_ptr(),
-              out.data_ptr(), to[0] if n > 1 else nh * hd, workspace.data_ptr(), workspace.numel())
-    after = (TYPE_CODES[dtype], TYPE_CODES[k_pool.dtype], n, n_req, nh, n_kv, hd, prefix_len, max_new, max_len,
-             page_size, n_slots, scale)
+    scratch = pointers(gpu, _lib.BYTE, workspace, -1)
+    if scratch is None:
+        raise ValueError("prefix attention: workspace must be a contiguous uint8 CUDA tensor")
+    before = (x_ptr, row if n > 1 else nh * hd, k_ptr, v_ptr, slot_stride, *shared, table_ptr,
+              columns if n_req > 1 else blocks, *ptrs, to[0], to[6] if n > 1 else nh * hd, *scratch,
+              workspace.numel())
+    after = (code, cache, n, n_req, nh, n_kv, hd, prefix_len, max_new, max_len, page_size, n_slots, scale)
     enqueue(_lib.lib().ls_prefix_attention, _pack, before, after, q.device, status, stream)
     return out

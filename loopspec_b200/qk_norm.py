@@ -9,20 +9,19 @@ from . import _lib
 from .status import enqueue, on_stream
 
 _pack = _lib.packer(_lib.QkNormArgs)
-_i32, _f32 = torch.int32, torch.float32
-TYPE_CODES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}    # LS_BF16, LS_F16, LS_F32
+TYPE_CODES = {torch.bfloat16: _lib.BF16, torch.float16: _lib.F16, torch.float32: _lib.F32}
+FLOATS = (_lib.BF16, _lib.F16, _lib.F32)
 
 
 def check_pools(k_pool, v_pool, what):
-    """(n_slots, n_kv_heads, head_dim, slot stride) of a pair of K/V pools."""
-    shape, stride = k_pool.shape, k_pool.stride()
-    if not (len(shape) == 3 and v_pool.shape == shape and v_pool.dtype is k_pool.dtype and v_pool.stride() == stride
-            and stride[2] == 1 and stride[1] == shape[2] and k_pool.is_cuda and v_pool.is_cuda
-            and k_pool.dtype in TYPE_CODES):
+    """(k pointer, v pointer, GPU, type code, n_slots, n_kv_heads, head_dim, slot stride) of a pair of K/V pools."""
+    facts, _ = _lib.tensor_facts()
+    k, v = facts(k_pool), facts(v_pool)
+    if not (k and v and len(k) == 9 and k[1:] == v[1:] and k[2] in FLOATS and k[8] == 1 and k[7] == k[5] > 0):
         raise ValueError(f"{what}: k_pool and v_pool must be CUDA tensors [n_slots, n_kv_heads, head_dim] of one type "
                          "and layout, with contiguous slots")
-    n_slots, n_kv, hd = shape
-    return n_slots, n_kv, hd, stride[0] if n_slots > 1 else n_kv * hd
+    k_ptr, gpu, code, n_slots, n_kv, hd, stride = k[:7]
+    return k_ptr, v[0], gpu, code, n_slots, n_kv, hd, stride if n_slots > 1 else n_kv * hd
 
 
 def rope_table(max_positions, rot, theta=10000.0, device="cuda"):
@@ -44,34 +43,35 @@ def qk_norm_rope(qkv, q_weight, k_weight, rope, positions, k_pool, v_pool, slots
     k_pool, v_pool       [n_slots, n_kv_heads, head_dim], bf16 or f16
     out        q's destination [T, n_heads, head_dim] of qkv's type (may be the q part of qkv)
     """
-    n_slots, n_kv, hd, slot_stride = check_pools(k_pool, v_pool, "qk norm")
-    n, width = qkv.shape
-    nh = width // hd - 2 * n_kv
-    row, dtype = qkv.stride(), qkv.dtype
-    if not (width % hd == 0 and nh > 0 and qkv.is_cuda and row[1] == 1 and dtype in TYPE_CODES):
+    facts, pointers = _lib.tensor_facts()
+    k_ptr, v_ptr, gpu, cache, n_slots, n_kv, hd, slot_stride = check_pools(k_pool, v_pool, "qk norm")
+    x = facts(qkv)
+    if not (x and len(x) == 7 and x[1] == gpu and x[2] in FLOATS and x[6] == 1 and x[4] % hd == 0
+            and x[4] // hd > 2 * n_kv):
         raise ValueError("qk norm: qkv must be a CUDA tensor whose contiguous rows hold q, k and v heads")
-    if not (q_weight.numel() == hd == k_weight.numel() and q_weight.dtype is k_weight.dtype
-            and q_weight.dtype in TYPE_CODES and q_weight.is_cuda and k_weight.is_cuda
-            and q_weight.is_contiguous() and k_weight.is_contiguous()):
+    x_ptr, _, code, n, width, row, _ = x
+    nh = width // hd - 2 * n_kv
+    weight_code = TYPE_CODES.get(q_weight.dtype, -1)
+    weights = pointers(gpu, weight_code, q_weight, hd, k_weight, hd) if weight_code >= 0 else None
+    if weights is None:
         raise ValueError("qk norm: q_weight and k_weight must be contiguous CUDA tensors [head_dim] of one type")
     limit, two, half = rope.shape
-    if not (two == 2 and rope.dtype is _f32 and rope.is_cuda and rope.is_contiguous()):
+    table = pointers(gpu, _lib.F32, rope, -1)
+    if table is None or two != 2:
         raise ValueError("qk norm: rope must be a contiguous fp32 CUDA tensor [max_positions, 2, rot / 2]")
-    for t in (positions, slots):
-        if t is not None and not (t.dtype is _i32 and t.is_cuda and t.is_contiguous() and t.numel() == n):
-            raise ValueError("qk norm: positions and slots must be int32 contiguous CUDA tensors, one entry a token")
+    where = pointers(gpu, _lib.I32, positions, n, slots, n)
+    if where is None:
+        raise ValueError("qk norm: positions and slots must be int32 contiguous CUDA tensors, one entry a token")
     if slots is None and n > n_slots:
         raise ValueError("qk norm: without slots the pools need a row for each token")
     if out is None:
         with on_stream(qkv.device, stream):
-            out = torch.empty(n, nh, hd, dtype=dtype, device=qkv.device)
-    to = out.stride()
-    if not (out.shape == (n, nh, hd) and out.dtype is dtype and out.is_cuda and to[2] == 1 and to[1] == hd):
+            out = torch.empty(n, nh, hd, dtype=qkv.dtype, device=qkv.device)
+    to = facts(out)
+    if not (to and to[1:6] == (gpu, code, n, nh, hd) and to[8] == 1 and to[7] == hd):
         raise ValueError("qk norm: out must be a CUDA tensor [T, n_heads, head_dim] of qkv's type with contiguous rows")
-    before = (qkv.data_ptr(), row[0] if n > 1 else width, q_weight.data_ptr(), k_weight.data_ptr(), rope.data_ptr(),
-              positions.data_ptr(), 0 if slots is None else slots.data_ptr(), k_pool.data_ptr(),
-              v_pool.data_ptr(), slot_stride, out.data_ptr(), to[0] if n > 1 else nh * hd)
-    after = (TYPE_CODES[dtype], TYPE_CODES[q_weight.dtype], TYPE_CODES[k_pool.dtype], n, nh, n_kv, hd, limit, 2 * half,
-             int(interleaved), n_slots, eps)
+    before = (x_ptr, row if n > 1 else width, *weights, *table, *where, k_ptr, v_ptr, slot_stride, to[0],
+              to[6] if n > 1 else nh * hd)
+    after = (code, weight_code, cache, n, nh, n_kv, hd, limit, 2 * half, int(interleaved), n_slots, eps)
     enqueue(_lib.lib().ls_qk_norm_rope, _pack, before, after, qkv.device, status, stream)
     return out

@@ -16,7 +16,6 @@ from . import _lib
 from .status import enqueue
 
 _pack = _lib.packer(_lib.SlotsArgs)
-_i32 = torch.int32
 
 
 class SlotMap:
@@ -48,19 +47,18 @@ def build_slots(lens, delta, block_table, free_blocks, free_count, *, page_size,
     All or nothing: on a bad length, too few free blocks or more new tokens
     than out.slots holds, nothing changes and the status says why.
     """
-    for t in (lens, delta, free_blocks, free_count, out.lens, out.free_count):
-        if not (t.dtype is _i32 and t.is_cuda and t.is_contiguous()):
-            raise ValueError("slot maps: int32 contiguous CUDA tensors expected")
-    n, width = block_table.shape
-    row = block_table.stride()
-    if not (block_table.dtype is _i32 and block_table.is_cuda and row[1] == 1):
-        raise ValueError("slot maps: block_table must be an int32 CUDA tensor with contiguous rows")
-    if not (lens.numel() == n == delta.numel() == out.lens.numel() and out.token_start.numel() == n + 1
-            and free_count.numel() == 1 == out.free_count.numel()):
-        raise ValueError("slot maps: lens, delta, block_table and out must describe the same requests")
-    before = (lens.data_ptr(), delta.data_ptr(), block_table.data_ptr(), row[0] if n > 1 else width,
-              free_blocks.data_ptr(), free_count.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(),
-              out.requests.data_ptr(), out.token_start.data_ptr(), out.lens.data_ptr(), out.free_count.data_ptr())
-    after = (n, width, free_blocks.numel(), n_blocks, page_size, base, out.slots.numel())
+    facts, pointers = _lib.tensor_facts()
+    table = facts(block_table)
+    if not (table and len(table) == 7 and table[2] == _lib.I32 and table[6] == 1):
+        raise ValueError("slot maps: block_table must be an int32 CUDA tensor [n_requests, width] with contiguous rows")
+    table_ptr, gpu, _, n, width, row, _ = table
+    most = out.slots.numel()
+    ptrs = pointers(gpu, _lib.I32, lens, n, delta, n, free_blocks, -1, free_count, 1, out.slots, most, out.positions,
+                    most, out.requests, most, out.token_start, n + 1, out.lens, n, out.free_count, 1)
+    if ptrs is None:
+        raise ValueError("slot maps: lens, delta, free_blocks, free_count and out must be int32 contiguous CUDA tensors "
+                         "that describe the block table's requests")
+    before = (*ptrs[:2], table_ptr, row if n > 1 else width, *ptrs[2:])
+    after = (n, width, free_blocks.numel(), n_blocks, page_size, base, most)
     enqueue(_lib.lib().ls_build_slots, _pack, before, after, lens.device, status, stream)
     return out

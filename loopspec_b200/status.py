@@ -10,6 +10,8 @@ without one waits for its kernels and raises at once.
 
 from __future__ import annotations
 
+from contextlib import nullcontext
+
 import torch
 
 from . import _lib
@@ -59,5 +61,4 @@ def enqueue(call, pack, before, after, device, status, stream):
 
 def on_stream(device, stream):
     """A context whose allocations belong to `stream` (a handle, or None for the current one)."""
-    return torch.cuda.stream(torch.cuda.current_stream(device) if stream is None
-                             else torch.cuda.ExternalStream(stream, device))
+    return nullcontext() if stream is None else torch.cuda.stream(torch.cuda.ExternalStream(stream, device))
