@@ -86,5 +86,5 @@ def prefix_attention(q, k_pool, v_pool, prefix_table, prefix_len, block_table, l
               columns if n_req > 1 else blocks, *ptrs, to[0], to[6] if n > 1 else nh * hd, *scratch,
               workspace.numel())
     after = (code, cache, n, n_req, nh, n_kv, hd, prefix_len, max_new, max_len, page_size, n_slots, scale)
-    enqueue(_lib.lib().ls_prefix_attention, _pack, before, after, q.device, status, stream)
+    enqueue(_lib.lib().ls_prefix_attention, _pack, before, after, gpu, status, stream)
     return out

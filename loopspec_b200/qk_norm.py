@@ -73,5 +73,5 @@ def qk_norm_rope(qkv, q_weight, k_weight, rope, positions, k_pool, v_pool, slots
     before = (x_ptr, row if n > 1 else width, *weights, *table, *where, k_ptr, v_ptr, slot_stride, to[0],
               to[6] if n > 1 else nh * hd)
     after = (code, weight_code, cache, n, nh, n_kv, hd, limit, 2 * half, int(interleaved), n_slots, eps)
-    enqueue(_lib.lib().ls_qk_norm_rope, _pack, before, after, qkv.device, status, stream)
+    enqueue(_lib.lib().ls_qk_norm_rope, _pack, before, after, gpu, status, stream)
     return out

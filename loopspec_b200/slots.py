@@ -60,5 +60,5 @@ def build_slots(lens, delta, block_table, free_blocks, free_count, *, page_size,
                          "that describe the block table's requests")
     before = (*ptrs[:2], table_ptr, row if n > 1 else width, *ptrs[2:])
     after = (n, width, free_blocks.numel(), n_blocks, page_size, base, most)
-    enqueue(_lib.lib().ls_build_slots, _pack, before, after, lens.device, status, stream)
+    enqueue(_lib.lib().ls_build_slots, _pack, before, after, gpu, status, stream)
     return out

@@ -34,26 +34,28 @@ class DeviceStatus:
 
 
 # The current stream's handle without the Stream object around it, which costs
-# 2 of the ~8 microseconds that a small call takes on the host.
+# 2 of the ~8 microseconds that a small call takes on the host; the current
+# device without the initialisation check, as there are tensors on one.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def enqueue(call, pack, before, after, device, status, stream):
-    """Run `call(struct, stream)` on the tensors' device, where the struct is
-    pack(*before, status word, *after); with no status, wait and raise."""
+def enqueue(call, pack, before, after, gpu, status, stream):
+    """Run `call(struct, stream)` on the tensors' GPU (its index), where the struct
+    is pack(*before, status word, *after); with no status, wait and raise."""
     if stream is None:
-        stream = _raw_stream(device.index)
+        stream = _raw_stream(gpu)
     if status is None:
-        with torch.cuda.device(device), torch.cuda.stream(torch.cuda.ExternalStream(stream, device)):
-            own = DeviceStatus(device)
+        with torch.cuda.device(gpu), torch.cuda.stream(torch.cuda.ExternalStream(stream, gpu)):
+            own = DeviceStatus(torch.device("cuda", gpu))
             _lib.check(call(pack(*before, own.ptr, *after), stream))
             own.check(stream)
         return
-    if device.index == torch.cuda.current_device():
+    if gpu == _current_device():
         code = call(pack(*before, status.ptr, *after), stream)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(gpu):
             code = call(pack(*before, status.ptr, *after), stream)
     if code:
         _lib.check(code)
