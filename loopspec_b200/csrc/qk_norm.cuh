@@ -105,6 +105,8 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(QkNormArgs a) 
   const int t = blockIdx.x;
   const int j = threadIdx.x % L;
   const int heads = a.nh + 2 * a.nkv;
+  pdl_wait();                // launched early: inputs may be on their way
+  pdl_launch_dependents();   // what follows waits for this kernel in the same way
   const int pos = a.positions[t];
   const int slot = a.slots ? a.slots[t] : t;
   const T* src = static_cast<const T*>(a.qkv) + (long)t * a.qkv_stride;

@@ -102,13 +102,16 @@ void run_build_slots(const ls_slots_args& p, cudaStream_t stream) {
   const int work = std::max({p.max_tokens, p.n_requests, 1});
   int ctas = std::min(cdiv(work, kSlotThreads), sm_count());
   cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   if (a.in_place) {
     ctas = std::min(ctas, kSlotMaxCluster);
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim = {(unsigned)ctas, 1, 1};
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)ctas, 1, 1};
+    cfg.numAttrs = 2;
   }
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kSlotThreads);
@@ -121,8 +124,8 @@ void run_build_slots(const ls_slots_args& p, cudaStream_t stream) {
 template <typename T, typename C, int HD, int U>
 void launch_qk(const QkNormArgs& a, bool interleaved, cudaStream_t stream) {
   const dim3 grid(a.n_tokens, cdiv(a.nh + 2 * a.nkv, kQkThreads * 16 / HD * U));
-  if (interleaved) launch(qk_norm_rope_kernel<T, C, HD, true, U>, grid, dim3(kQkThreads), 0, stream, false, a);
-  else launch(qk_norm_rope_kernel<T, C, HD, false, U>, grid, dim3(kQkThreads), 0, stream, false, a);
+  if (interleaved) launch(qk_norm_rope_kernel<T, C, HD, true, U>, grid, dim3(kQkThreads), 0, stream, true, a);
+  else launch(qk_norm_rope_kernel<T, C, HD, false, U>, grid, dim3(kQkThreads), 0, stream, true, a);
 }
 
 // One pass a CTA while the passes fit the GPU at once (about 8 CTAs an SM);

@@ -82,6 +82,8 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int page = 1 << a.page_shift;
   const long capacity = (long)a.table_width << a.page_shift;
+  pdl_wait();                // launched early: inputs may be on their way
+  pdl_launch_dependents();   // what follows waits for this kernel in the same way
 
   // running sums: each thread adds a run of consecutive requests, the block
   // scans the runs (64-bit: lengths may be garbage), the thread lays them out
