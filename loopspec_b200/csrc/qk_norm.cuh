@@ -13,7 +13,9 @@
 // log2(HD/16) shuffles. A warp covers 32*16/HD heads at a time.
 //
 // Bound: HBM for prompts (each row is read once, q, k and v written once),
-// launch latency for decode batches.
+// launch latency for decode batches. 8191 tokens of 16 + 32 heads of 128 in f16
+// (203 MB): 38.5 us, 5.3 TB/s, four fifths of a plain copy; up to 61 tokens 2.5
+// us, call after call in a graph.
 #pragma once
 
 #include <cuda_fp16.h>
