@@ -14,7 +14,7 @@
 //
 // Bound: HBM for prompts (each row is read once, q, k and v written once),
 // launch latency for decode batches. 8191 tokens of 16 + 32 heads of 128 in f16
-// (203 MB): 38.5 us, 5.3 TB/s, four fifths of a plain copy; up to 61 tokens 2.5
+// (203 MB): 37.7 us, 5.4 TB/s, four fifths of a plain copy; up to 61 tokens 2.1
 // us, call after call in a graph.
 #pragma once
 
@@ -45,6 +45,7 @@ struct QkNormArgs {
   void* q_out;
   long q_out_stride;     // elements
   int* status;
+  int parts;   // warps that share a token
 };
 
 __device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
@@ -98,14 +99,16 @@ struct Raw8 {
   __device__ __forceinline__ void get(float (&f)[8]) const { load8(reinterpret_cast<const T*>(v), f); }
 };
 
-// grid (n_tokens, parts): part p of a token's heads, U passes of kQkThreads*16/HD
-// heads at a time, whose loads are all issued before the first is used.
+// A warp takes one of `parts` parts of a token's heads: U passes of 512/HD heads,
+// whose loads are all issued before the first is used.
 template <typename T, typename C, int HD, bool INTERLEAVED, int U>
 __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(QkNormArgs a) {
   constexpr int L = HD / 16;                 // lanes of one head
-  constexpr int HEADS = kQkThreads / L;      // heads of a CTA at a time
-  const int t = blockIdx.x;
-  const int j = threadIdx.x % L;
+  constexpr int HEADS = 32 / L;              // heads of a pass
+  const unsigned unit = blockIdx.x * (kQkThreads / 32) + threadIdx.x / 32;
+  const int t = (int)(unit / (unsigned)a.parts), part = (int)(unit % (unsigned)a.parts);
+  if (t >= a.n_tokens) return;
+  const int lane = threadIdx.x & 31, j = lane % L;
   const int heads = a.nh + 2 * a.nkv;
   pdl_wait();                // launched early: inputs may be on their way
   pdl_launch_dependents();   // what follows waits for this kernel in the same way
@@ -128,22 +131,20 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(QkNormArgs a) 
     ca = turn_a ? j : rc + 2 * (j - rc / 2);
     cb = turn_a ? j + rc / 2 : ca + 1;
   }
-  // the first heads are on their way while the position is looked up
+  // the heads are on their way while the position is looked up
+  const int first = part * (HEADS * U) + lane / L;
   Raw8<T> xs[U], ys[U];
-  auto load = [&](int h0) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = min(h0 + u * HEADS + (int)threadIdx.x / L, heads - 1);   // past the last: read it again, store nothing
-      xs[u].load(src + (long)h * HD + 8 * ca);
-      ys[u].load(src + (long)h * HD + 8 * cb);
-    }
-  };
-  load(blockIdx.y * (HEADS * U));
+  for (int u = 0; u < U; ++u) {
+    const int h = min(first + u * HEADS, heads - 1);   // past the last: read it again, store nothing
+    xs[u].load(src + (long)h * HD + 8 * ca);
+    ys[u].load(src + (long)h * HD + 8 * cb);
+  }
 
   const bool pos_ok = pos >= 0 && pos < a.max_positions;
   const bool slot_ok = pos_ok && slot >= 0 && slot < a.n_slots;
   // a slot of -1 marks padding, whose K/V go nowhere
-  if (threadIdx.x == 0 && (!pos_ok || slot < -1 || slot >= a.n_slots)) atomicCAS(a.status, kDevOk, kDevBadIndex);
+  if (lane == 0 && (!pos_ok || slot < -1 || slot >= a.n_slots)) atomicCAS(a.status, kDevOk, kDevBadIndex);
 
   // cosines and sines: 8 pairs (i, i + rot/2), or 4 pairs of each chunk
   float cs[8], sn[8];
@@ -173,68 +174,65 @@ __global__ void __launch_bounds__(kQkThreads) qk_norm_rope_kernel(QkNormArgs a) 
   T* q_row = static_cast<T*>(a.q_out) + (long)t * a.q_out_stride;
   C* k_row = static_cast<C*>(a.k_pool) + (long)(slot_ok ? slot : 0) * a.slot_stride;
   C* v_row = static_cast<C*>(a.v_pool) + (long)(slot_ok ? slot : 0) * a.slot_stride;
-  // whole warps loop together: the norm's shuffles need every lane
-  for (int h0 = blockIdx.y * (HEADS * U); h0 < heads; h0 += gridDim.y * (HEADS * U)) {
+  // the whole warp stays in the loop: the norm's shuffles need every lane
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[8], y[8];
-      xs[u].get(x);
-      ys[u].get(y);
-      const int h = h0 + u * HEADS + threadIdx.x / L;
-      float ss = 0.f;
+  for (int u = 0; u < U; ++u) {
+    float x[8], y[8];
+    xs[u].get(x);
+    ys[u].get(y);
+    const int h = first + u * HEADS;
+    float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
+    for (int i = 0; i < 8; ++i) ss += x[i] * x[i] + y[i] * y[i];
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (h >= heads) continue;
-      if (h >= a.nh + a.nkv) {
-        if (slot_ok) {
-          store8(v_row + (long)(h - a.nh - a.nkv) * HD + 8 * ca, x);
-          store8(v_row + (long)(h - a.nh - a.nkv) * HD + 8 * cb, y);
-        }
-        continue;
+    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (h >= heads) continue;
+    if (h >= a.nh + a.nkv) {
+      if (slot_ok) {
+        store8(v_row + (long)(h - a.nh - a.nkv) * HD + 8 * ca, x);
+        store8(v_row + (long)(h - a.nh - a.nkv) * HD + 8 * cb, y);
       }
-      float wx[8], wy[8];
-      const void* w = h < a.nh ? a.q_weight : a.k_weight;
-      load8_as(w, a.weight_type, 8 * ca, wx);
-      load8_as(w, a.weight_type, 8 * cb, wy);
-      const float inv = rsqrtf(ss / HD + a.eps);
+      continue;
+    }
+    float wx[8], wy[8];
+    const void* w = h < a.nh ? a.q_weight : a.k_weight;
+    load8_as(w, a.weight_type, 8 * ca, wx);
+    load8_as(w, a.weight_type, 8 * cb, wy);
+    const float inv = rsqrtf(ss / HD + a.eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = x[i] * inv * wx[i];
+      y[i] = y[i] * inv * wy[i];
+    }
+    // unrotated chunks stay out of the products: 0 * inf would spoil them
+    if (INTERLEAVED) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x1 = x[2 * i], x2 = x[2 * i + 1], y1 = y[2 * i], y2 = y[2 * i + 1];
+        if (turn_a) {
+          x[2 * i] = x1 * cs[i] - x2 * sn[i];
+          x[2 * i + 1] = x2 * cs[i] + x1 * sn[i];
+        }
+        if (turn_b) {
+          y[2 * i] = y1 * cs[4 + i] - y2 * sn[4 + i];
+          y[2 * i + 1] = y2 * cs[4 + i] + y1 * sn[4 + i];
+        }
+      }
+    } else if (turn_a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        x[i] = x[i] * inv * wx[i];
-        y[i] = y[i] * inv * wy[i];
-      }
-      // unrotated chunks stay out of the products: 0 * inf would spoil them
-      if (INTERLEAVED) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x1 = x[2 * i], x2 = x[2 * i + 1], y1 = y[2 * i], y2 = y[2 * i + 1];
-          if (turn_a) {
-            x[2 * i] = x1 * cs[i] - x2 * sn[i];
-            x[2 * i + 1] = x2 * cs[i] + x1 * sn[i];
-          }
-          if (turn_b) {
-            y[2 * i] = y1 * cs[4 + i] - y2 * sn[4 + i];
-            y[2 * i + 1] = y2 * cs[4 + i] + y1 * sn[4 + i];
-          }
-        }
-      } else if (turn_a) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float x1 = x[i], x2 = y[i];
-          x[i] = x1 * cs[i] - x2 * sn[i];
-          y[i] = x2 * cs[i] + x1 * sn[i];
-        }
-      }
-      if (h < a.nh) {
-        store8(q_row + (long)h * HD + 8 * ca, x);
-        store8(q_row + (long)h * HD + 8 * cb, y);
-      } else if (slot_ok) {
-        store8(k_row + (long)(h - a.nh) * HD + 8 * ca, x);
-        store8(k_row + (long)(h - a.nh) * HD + 8 * cb, y);
+        const float x1 = x[i], x2 = y[i];
+        x[i] = x1 * cs[i] - x2 * sn[i];
+        y[i] = x2 * cs[i] + x1 * sn[i];
       }
     }
-    if (h0 + gridDim.y * (HEADS * U) < heads) load(h0 + gridDim.y * (HEADS * U));
+    if (h < a.nh) {
+      store8(q_row + (long)h * HD + 8 * ca, x);
+      store8(q_row + (long)h * HD + 8 * cb, y);
+    } else if (slot_ok) {
+      store8(k_row + (long)(h - a.nh) * HD + 8 * ca, x);
+      store8(k_row + (long)(h - a.nh) * HD + 8 * cb, y);
+    }
   }
 }
 

@@ -124,18 +124,23 @@ void run_build_slots(const ls_slots_args& p, cudaStream_t stream) {
 // ----------------------------------------------------------- norm and rotation
 template <typename T, typename C, int HD, int U>
 void launch_qk(const QkNormArgs& a, bool interleaved, cudaStream_t stream) {
-  const dim3 grid(a.n_tokens, cdiv(a.nh + 2 * a.nkv, kQkThreads * 16 / HD * U));
+  const long warps = (long)a.n_tokens * a.parts;
+  REQUIRE(warps <= INT32_MAX, LS_EINVAL, "qk norm: too many tokens and heads for one launch");
+  const dim3 grid((unsigned)cdiv(warps, kQkThreads / 32));
   if (interleaved) launch(qk_norm_rope_kernel<T, C, HD, true, U>, grid, dim3(kQkThreads), 0, stream, true, a);
   else launch(qk_norm_rope_kernel<T, C, HD, false, U>, grid, dim3(kQkThreads), 0, stream, true, a);
 }
 
-// One pass a CTA while the passes fit the GPU at once (about 8 CTAs an SM);
-// three for prompts, where loads in flight decide (61 tokens: 2.5 us with one,
-// 3.3 with three; 8191 tokens: 46.0 and 38.5).
+// One pass a warp while the passes fit the GPU at once; up to three for prompts,
+// where loads in flight decide, as evenly as the heads go (61 tokens: 2.1 us with
+// one, 2.9 with three; 8191 tokens of 48 heads: 44.0 and 37.7).
 template <typename T, typename C, int HD>
-void launch_qk(const QkNormArgs& a, bool interleaved, cudaStream_t stream) {
-  const long passes = (long)a.n_tokens * cdiv(a.nh + 2 * a.nkv, kQkThreads * 16 / HD);
-  if (passes <= 8L * sm_count()) launch_qk<T, C, HD, 1>(a, interleaved, stream);
+void launch_qk(QkNormArgs a, bool interleaved, cudaStream_t stream) {
+  const int passes = cdiv(a.nh + 2 * a.nkv, 512 / HD);
+  a.parts = (long)a.n_tokens * passes <= 32L * sm_count() ? passes : cdiv(passes, 3);
+  const int each = cdiv(passes, a.parts);
+  if (each == 1) launch_qk<T, C, HD, 1>(a, interleaved, stream);
+  else if (each == 2) launch_qk<T, C, HD, 2>(a, interleaved, stream);
   else launch_qk<T, C, HD, 3>(a, interleaved, stream);
 }
 
@@ -169,7 +174,7 @@ void run_qk_norm_rope(const ls_qk_norm_args& p, cudaStream_t stream) {
           LS_EINVAL, "qk norm: pointers and row strides must be 16-byte aligned");
   QkNormArgs a{p.qkv, (long)p.qkv_stride, p.n_tokens, p.n_heads, p.n_kv_heads, p.q_weight, p.k_weight,
                p.weight_type, p.eps, p.rope, p.max_positions, p.rot, p.positions, p.slots, p.k_pool, p.v_pool,
-               (long)p.slot_stride, p.n_slots, p.q_out, (long)p.q_out_stride, p.status};
+               (long)p.slot_stride, p.n_slots, p.q_out, (long)p.q_out_stride, p.status, 1};
   const bool il = p.interleaved != 0;
   if (p.qkv_type == LS_BF16) launch_qk<bf16, bf16>(a, p.head_dim, il, stream);
   else if (p.qkv_type == LS_F16) launch_qk<__half, __half>(a, p.head_dim, il, stream);
