@@ -120,9 +120,14 @@ def main():
             raise AssertionError("an output is not finite")
         return start.elapsed_time(end) / a.layers * 1e3
 
-    print(f"prefix of {a.prefix}: {step([a.prefix] + [0] * (R - 1)):.0f} us a layer")
+    def again(delta):                         # the first time loads the kernels: taken back, and once more
+        step(delta)
+        batch.begin(-torch.tensor(delta, dtype=torch.int32, device=dev), 0, 0)
+        return step(delta)
+
+    print(f"prefix of {a.prefix}: {again([a.prefix] + [0] * (R - 1)):.0f} us a layer")
     batch.share(0, a.prefix)
-    print(f"{R} prompts of up to {a.prompt}: {step([a.prompt - i * a.prompt // (2 * R) for i in range(R)]):.0f} us a layer")
+    print(f"{R} prompts of up to {a.prompt}: {again([a.prompt - i * a.prompt // (2 * R) for i in range(R)]):.0f} us a layer")
     times = []
     for _ in range(a.steps):
         times.append(step([a.drafts] * R))
