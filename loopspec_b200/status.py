@@ -18,8 +18,14 @@ from . import _lib
 
 
 class DeviceStatus:
+    """A status word on one GPU, for calls on tensors of that GPU: kernels write it by its address."""
+
     def __init__(self, device="cuda"):
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"the status word must be on a GPU, not on {device}")
         self.word = torch.zeros(1, dtype=torch.int32, device=device)
+        self.gpu = self.word.get_device()
         self.ptr = self.word.data_ptr()
 
     def check(self, stream=None):
@@ -52,6 +58,8 @@ def enqueue(call, pack, before, after, gpu, status, stream):
             _lib.check(call(pack(*before, own.ptr, *after), stream))
             own.check(stream)
         return
+    if status.gpu != gpu:
+        raise ValueError(f"the status word is on GPU {status.gpu}, the tensors on GPU {gpu}")
     if gpu == _current_device():
         code = call(pack(*before, status.ptr, *after), stream)
     else:
