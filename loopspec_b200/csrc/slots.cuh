@@ -151,17 +151,19 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
   else if (total_grow > count + total_back) code = kDevNoBlocks;
   else if (count + total_back - total_grow > a.free_capacity) code = kDevBadLength;
 
-  const int at = (int)blockIdx.x * kSlotThreads + tid, step = (int)gridDim.x * kSlotThreads;
+  // unsigned: the loops' counters go past their ends, which may be 2^31 - 1, by up to a step
+  const unsigned at = blockIdx.x * kSlotThreads + tid, step = gridDim.x * kSlotThreads;
+  const unsigned n_buffer = (unsigned)a.max_tokens, n_req = (unsigned)R;
   if (code != kDevOk) {   // all or nothing
     if (at == 0) atomicCAS(a.status, kDevOk, code);
-    for (int k = at; k < a.max_tokens; k += step) {
+    for (unsigned k = at; k < n_buffer; k += step) {
       a.slots[k] = -1;
       a.positions[k] = 0;
       a.requests[k] = -1;
     }
-    for (int i = at; i <= R; i += step) a.token_start[i] = 0;
+    for (unsigned i = at; i <= n_req; i += step) a.token_start[i] = 0;
     if (a.lens_out != a.lens)
-      for (int i = at; i < R; i += step) a.lens_out[i] = a.lens[i];
+      for (unsigned i = at; i < n_req; i += step) a.lens_out[i] = a.lens[i];
     if (a.free_count_out != a.free_count && at == 0) a.free_count_out[0] = (int)count;
     return;
   }
@@ -197,12 +199,12 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
     return p < count ? a.free_blocks[p] : given((int)(p - count));
   };
 
-  for (int k = at; k < a.max_tokens; k += step) {
+  for (unsigned k = at; k < n_buffer; k += step) {
     int slot = -1, position = 0, request = -1;
-    if (k < n_tok) {
-      request = owner_of(s_tok, R, k);
+    if (k < (unsigned)n_tok) {
+      request = owner_of(s_tok, R, (int)k);
       const int len = a.lens[request];
-      const int pos = len + (k - s_tok[request]);
+      const int pos = len + ((int)k - s_tok[request]);
       const int have = (len + page - 1) >> a.page_shift, blk = pos >> a.page_shift;
       const int block = blk < have ? a.table[request * a.table_stride + blk]
                                    : taken(s_grow[request] + blk - have);
@@ -214,15 +216,15 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
     a.positions[k] = position;
     a.requests[k] = request;
   }
-  for (int k = at; k < n_take; k += step) {
-    const int i = owner_of(s_grow, R, k);
+  for (unsigned k = at; k < (unsigned)n_take; k += step) {
+    const int i = owner_of(s_grow, R, (int)k);
     const int have = (a.lens[i] + page - 1) >> a.page_shift;
-    a.table[i * a.table_stride + have + (k - s_grow[i])] = taken(k);
+    a.table[i * a.table_stride + have + ((int)k - s_grow[i])] = taken((int)k);
   }
   for (long p = count + at; p < count + n_give - n_take; p += step) a.free_blocks[p] = given((int)(p - count));
-  for (int i = at; i <= R; i += step) a.token_start[i] = s_tok[i];
+  for (unsigned i = at; i <= n_req; i += step) a.token_start[i] = s_tok[i];
   if (a.in_place) cg::this_cluster().sync();   // every CTA has read lens and the count
-  for (int i = at; i < R; i += step) a.lens_out[i] = a.lens[i] + a.delta[i];
+  for (unsigned i = at; i < n_req; i += step) a.lens_out[i] = a.lens[i] + a.delta[i];
   if (at == 0) a.free_count_out[0] = (int)(count + n_give - n_take);
 }
 
