@@ -334,8 +334,9 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       auto clear = [&](int t0, int t1) {
         t0 = max(0, t0);
         t1 = min(a.n_tokens, t1);
-        for (int i = threadIdx.x; i < (t1 - t0) * G * (HD / 4); i += blockDim.x) {
-          const int t = t0 + i / (G * (HD / 4)), c = i % (G * (HD / 4));
+        const int per = G * (HD / 4);                // 4-element pieces of a token
+        for (long i = threadIdx.x; i < (long)(t1 - t0) * per; i += blockDim.x) {
+          const int t = t0 + (int)(i / per), c = (int)(i % per);
           store4(static_cast<Q*>(a.out) + (long)t * a.out_stride + (long)g * G * HD + c * 4, make_float4(0.f, 0.f, 0.f, 0.f));
         }
       };
