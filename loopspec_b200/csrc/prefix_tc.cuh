@@ -745,6 +745,10 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         }
       }
     }
+    // No product is under way when the tensor memory is given back: the softmax
+    // warps have seen the last ones end, unless a wait of theirs timed out.
+    bool ended = n > 0;
+    for (int t = 0; t < tiles_here; ++t) wait_on(ended, o_done + 8 * t, 0, a.status, kDevTimeoutAcc);
   }
   tc_fence_before();
   __syncthreads();
