@@ -95,7 +95,7 @@ void run_build_slots(const ls_slots_args& p, cudaStream_t stream) {
              p.free_blocks, p.free_capacity, p.free_count, p.n_blocks, shift, p.base, p.max_tokens,
              p.slots, p.positions, p.requests, p.token_start, p.lens_out, p.free_count_out, p.status, false};
   const size_t smem = slot_smem_bytes(p.n_requests);
-  if (smem > 48 * 1024) allow_smem<build_slots_kernel>(slot_smem_bytes(kSlotMaxRequests));
+  allow_smem<build_slots_kernel>(slot_smem_bytes(kSlotMaxRequests));   // 48 KB without it, the static part included
   a.in_place = p.lens_out == p.lens || p.free_count_out == p.free_count;
   // a token a thread, on as many SMs as that takes: each CTA repeats the sums,
   // but the token loop's dependent loads (length, block) are what takes time

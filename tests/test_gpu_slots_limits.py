@@ -1,9 +1,34 @@
 """Slot maps at the edges of their ranges."""
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+ONE_CALL = """
+import sys
+import torch
+from loopspec_b200.slots import SlotMap, build_slots
+n = int(sys.argv[1])
+i32 = dict(dtype=torch.int32, device="cuda")
+lens, count = torch.zeros(n, **i32), torch.tensor([n], **i32)
+table, stack = torch.full((n, 1), -1, **i32), torch.arange(n - 1, -1, -1, **i32)
+m = build_slots(lens, torch.ones(n, **i32), table, stack, count, page_size=4, n_blocks=n, out=SlotMap(n, n))
+assert m.slots.tolist() == [4 * i for i in range(n)] and m.free_count.tolist() == [0]
+"""
+
+
+@pytest.mark.parametrize("n", [1, 3988, 3989, 4073, 4074, 4095, 4096, 16384])
+def test_any_number_of_requests_in_a_process_that_made_no_call_before(n):
+    """Around 48 KB of shared memory, which a kernel gets only if it is asked for: the first call of a process."""
+    run = subprocess.run([sys.executable, "-c", ONE_CALL, str(n)], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
 
 
 def test_token_buffers_of_2_31_entries():
