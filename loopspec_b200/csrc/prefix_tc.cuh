@@ -327,27 +327,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
   const unsigned n_parts = max(1, a.prefix_parts);
   const int part = (int)(u % n_parts), req = (int)(u / n_parts);
   int start = 0, n_new = a.n_tokens, len = 0;
-  if (a.own) {
-    const bool ok = request_range(a, req, start, n_new, len);
-    if (tile == 0 && part == 0) {
-      // tokens of no request, and those of one that is out of bounds, get zeros
-      auto clear = [&](int t0, int t1) {
-        t0 = max(0, t0);
-        t1 = min(a.n_tokens, t1);
-        const int per = G * (HD / 4);                // 4-element pieces of a token
-        for (long i = threadIdx.x; i < (long)(t1 - t0) * per; i += blockDim.x) {
-          const int t = t0 + (int)(i / per), c = (int)(i % per);
-          store4(static_cast<Q*>(a.out) + (long)t * a.out_stride + (long)g * G * HD + c * 4, make_float4(0.f, 0.f, 0.f, 0.f));
-        }
-      };
-      if (a.direct) {
-        if (req == 0) clear(0, a.token_start[0]);
-        if (req == a.n_requests - 1) clear(a.token_start[a.n_requests], a.n_tokens);
-        if (!ok) clear(a.token_start[req], a.token_start[req + 1]);
-      }
-    }
-    if (!ok) return;
-  }
+  if (a.own && !request_range(a, req, start, n_new, len)) return;
   const int rows = n_new * G;                      // rows of the kv head
   const int row0 = tile * (MT * kTcRows);
   if (row0 >= rows) return;

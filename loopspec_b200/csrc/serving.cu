@@ -367,7 +367,10 @@ void launch_prefix(PrefixAttnArgs a, const PrefixPlan& plan, cudaStream_t stream
   if constexpr (TERMS == 1) {
     if (plan.tc_tiles == 2) launch_tc<HD, Q, C, TERMS, 2>(a, stream);
   }
-  if (a.direct) return;
+  if (a.direct) {
+    launch(prefix_clear_kernel<HD, Q>, dim3((unsigned)std::min(a.n_tokens, sm_count())), dim3(kJoinThreads), 0, stream, true, a);
+    return;
+  }
   const bool prefix = plan.tc_tiles == 0 && a.prefix_parts > 0, suffix = a.suffix_parts > 0 && a.suffix_tiles > 0;
   bool behind = plan.tc_tiles != 0;
   if (prefix && suffix && plan.prefix_rt == plan.suffix_rt) {
