@@ -213,7 +213,8 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // cubic that minimises the largest relative error there (Remez exchange: 7.5e-5,
 // a fiftieth of bf16's half unit, a seventh of f16's), times 2^n put together
 // from its exponent bits: 0 from n = -127 on down, so a masked score weighs
-// nothing. NaN is not passed on; the caller's row maximum does that.
+// nothing. NaN is not passed on: a row with a NaN score has a NaN reference, whose
+// other exponentials are NaN, and a reference of +inf makes the row's sum NaN.
 __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
   constexpr float kMagic = 12582912.f;
   const float2 v = unpair(x);
@@ -461,7 +462,8 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         if (__any_sync(0xffffffffu, move)) {
           const float keep = move && m > -INFINITY ? exp2_fast((m - top) * a.scale_log2) : 1.f;
           if (move) m = top;
-          l *= keep;
+          // inf - inf: the row is NaN, whichever way its weights are computed
+          l = m == INFINITY ? NAN : l * keep;
           if (j > 0) {
             wait_on(ok, pv_done + 8 * t, (j - 1) & 1, a.status, kDevTimeoutAcc);
             tc_fence_after();
