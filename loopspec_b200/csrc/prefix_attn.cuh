@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
   constexpr int TPR = HD / 4, GROUPS = kJoinThreads / TPR;
   __shared__ float4 s_acc[SPLIT ? GROUPS : 1][TPR];
   __shared__ float2 s_ml[GROUPS];
-  __shared__ int s_len;
+  __shared__ int s_len, s_seen;   // own positions of the token's request, and those that the token sees
   const int t = blockIdx.x;
   if (!a.behind) pdl_wait();
   // no early launch of what follows: CTAs of the next call that wait here took
@@ -618,6 +618,7 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
         len <= a.max_len) {
       mine = true;
       s_len = len;
+      s_seen = len - (end - start) + 1 + (t - start);
     }
   }
   const bool ok = __syncthreads_or(mine);
@@ -685,7 +686,8 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
       acc.w += v.w * w;
     }
   }
-  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  // zeros for a row that sees nothing; one whose scores are all -inf is 0 / 0
+  const float inv = !ok || (a.prefix_len == 0 && s_seen <= 0) ? 0.f : 1.f / ll;
   acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
   store4(static_cast<Q*>(a.out) + (long)t * a.out_stride + (long)h * HD + c, acc);
 }

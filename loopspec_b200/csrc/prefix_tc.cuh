@@ -523,7 +523,9 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
       l = row_sum[0] + row_sum[kTcRows];
       const int tok = start + row_tok, h = g * G + rr - row_tok * G;
-      const float inv = !have ? 0.f : !a.direct ? 1.f : l == 0.f ? 0.f : 1.f / l;
+      // zeros for a row that sees nothing; one whose scores are all -inf is 0 / 0
+      const bool nothing = a.prefix_len == 0 && see <= 0;
+      const float inv = !have ? 0.f : !a.direct ? 1.f : nothing ? 0.f : 1.f / l;
       const long at = ((long)part * a.n_tokens + tok) * a.nh + h;
       if (!a.direct && rr < rows && half == 0)
         a.part_ml[at] = have ? make_float2(m * a.scale_log2, l) : make_float2(-INFINITY, 0.f);

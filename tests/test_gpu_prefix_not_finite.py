@@ -111,3 +111,25 @@ def infinite_key(way, first, hd, kind, cache):
 @pytest.mark.parametrize("way,first", INFINITE_KEY, ids=KEY_IDS)
 def test_an_infinite_key(way, first, hd, kind, cache):
     infinite_key(way, first, hd, kind, cache)
+
+
+def only_minus_infinity(way, hd, kind, cache):
+    """0 / 0, as the formula says: not the zeros of a row that sees nothing."""
+    page = 16
+    clean = built(way, page, hd, kind, cache, seed=hd)
+    clean[0][:, :, 0] = -1
+    bad = [clean[0], clean[1].clone(), *clean[2:]]
+    bad[1][slots_of(clean, page, 0), :, 0] = INF
+    ref = check(call(tuple(bad), page), bad, clean, page, kind, cache)
+    assert bool(torch.isnan(ref[0]).all())
+
+
+ONLY = [dict(PROMPT, lens=[130]), dict(STREAM, prefix=0, lens=[1, 2]), dict(STREAM, prefix=3)]
+ONLY_IDS = ["prompt", "own", "prefix"]
+
+
+@pytest.mark.parametrize("kind,cache", HALVES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("way", ONLY, ids=ONLY_IDS)
+def test_rows_whose_every_score_is_minus_infinity(way, hd, kind, cache):
+    only_minus_infinity(way, hd, kind, cache)
