@@ -225,6 +225,60 @@ __device__ __forceinline__ void add_by_weight(float (&o)[RT][HD / 16][4], const 
   }
 }
 
+// The pools' rows of one kv head.
+template <typename C>
+struct PoolView {
+  const C* k;
+  const C* v;
+  long stride;
+  int n_slots, page_shift;
+  __device__ __forceinline__ PoolView(const PrefixAttnArgs& a, int g, int hd)
+      : k(static_cast<const C*>(a.k_pool) + (long)g * hd), v(static_cast<const C*>(a.v_pool) + (long)g * hd),
+        stride(a.slot_stride), n_slots(a.n_slots), page_shift(a.page_shift) {}
+};
+
+// The weight of a key for a row by the formula; `base`: the row's reference in
+// powers of two, less the weights' bias.
+template <int HD, typename Q, typename C>
+__device__ __noinline__ float weight_of(const Q* q, const C* k, float base, float scale_log2) {
+  float s = 0.f;
+  for (int i = 0; i < HD; ++i) s += (float)q[i] * (float)k[i];
+  return exp2_fast(s * scale_log2 - base);
+}
+
+// Whether the terms of P can lose an infinite value: a term of 0, or of the other
+// sign than the one before it, times infinity is NaN. An f16 term is 0 for weights
+// below 2^-32 of the reference's even where it is the only one.
+template <typename C, int TERMS>
+constexpr bool kTermsLose = TERMS > 1 || std::is_same<C, __half>::value;
+
+// Dimensions first + i step, i < count, of an output row that met values which are
+// not finite, at positions [p0, p1) of a table: their sum once more, by the formula.
+// What is finite in them no longer counts. `done`: a bit for each dimension begun.
+template <int HD, typename Q, typename C, typename D>
+__device__ __noinline__ uint64_t redo_infinite(PoolView<C> pools, const int* table, int p0, int p1, const Q* q,
+                                               float base, float scale_log2, float factor, D* dst, int first, int step,
+                                               int count, uint64_t done) {
+  for (int pos = p0; pos < p1; ++pos) {
+    const int block = table[pos >> pools.page_shift];
+    const long slot = ((long)block << pools.page_shift) + (pos & ((1 << pools.page_shift) - 1));
+    if (block < 0 || slot >= pools.n_slots) continue;
+    const C* v = pools.v + slot * pools.stride;
+    float w = 0.f;
+    bool weighed = false;
+    for (int i = 0; i < count; ++i) {
+      const float x = (float)v[first + i * step];
+      if (fabsf(x) < INFINITY) continue;
+      if (!weighed) w = weight_of<HD>(q, pools.k + slot * pools.stride, base, scale_log2) * factor;
+      weighed = true;
+      D* to = dst + first + i * step;
+      *to = (D)((done >> i & 1 ? (float)*to : 0.f) + w * x);
+      done |= 1ull << i;
+    }
+  }
+  return done;
+}
+
 constexpr int kBatchRequests = 256;    // looked up at a time; 32 x 8 for the search
 
 // Units of a batch of requests: their lengths, and where each one's units begin.
@@ -574,6 +628,17 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
           for (int i = 0; i < MT; ++i) {
             dst[i * 16] = o[rt][i][e];
             dst[i * 16 + 8] = o[rt][i][2 + e];
+          }
+          if constexpr (kTermsLose<C, TERMS>) {
+            bool redo = false;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) redo |= !(fabsf(o[rt][i][e]) < INFINITY) || !(fabsf(o[rt][i][2 + e]) < INFINITY);
+            if (redo && sum > 0.f) {
+              const Q* q = static_cast<const Q*>(a.q) + (long)(start + j) * a.q_stride + (long)(g * G + r - j * G) * HD;
+              const float ref = (m[rt][e] == -INFINITY ? 0.f : m[rt][e]) - weight_bias(C());
+              redo_infinite<HD>(PoolView<C>(a, g, HD), suffix ? a.block_table + x.req * a.table_stride : a.prefix_table, k0,
+                                min(k1, see[rt][e]), q, ref, a.scale_log2, 1.f, a.part_o + row * HD, gid, 8, HD / 8, 0);
+            }
           }
         }
     }

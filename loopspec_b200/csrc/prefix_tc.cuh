@@ -276,15 +276,6 @@ __device__ __forceinline__ void cp_async16_to(uint32_t dst, const void* src, boo
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
 
-// The weight of own position `pos` for a row whose reference is m, by the formula.
-template <int HD, typename Q, typename C>
-__device__ __noinline__ float weight_of(const Q* q, const C* k, float m, float scale_log2) {
-  float s = 0.f;
-  for (int i = 0; i < HD; ++i) s += (float)q[i] * (float)k[i];
-  const float base = (m == -INFINITY ? 0.f : m * scale_log2) - weight_bias(C());
-  return exp2_fast(s * scale_log2 - base);
-}
-
 // Whether 8 packed 16-bit values hold a NaN or infinity (exponent bits all set).
 template <typename C>
 __device__ __forceinline__ bool not_finite8(const uint4& v) {
@@ -526,7 +517,9 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       // zeros for a row that sees nothing; one whose scores are all -inf is 0 / 0
       const bool nothing = a.prefix_len == 0 && see <= 0;
       const float inv = !have ? 0.f : !a.direct ? 1.f : nothing ? 0.f : 1.f / l;
+      const float base = (m == -INFINITY ? 0.f : m * a.scale_log2) - weight_bias(C());
       const long at = ((long)part * a.n_tokens + tok) * a.nh + h;
+      bool redo = false;                             // some output is not finite
       if (!a.direct && rr < rows && half == 0)
         a.part_ml[at] = have ? make_float2(m * a.scale_log2, l) : make_float2(-INFINITY, 0.f);
       // Parts leave by a patch of the row tile's queries, which are done with:
@@ -555,11 +548,15 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
               const long slot = ((long)own_table[pos >> a.page_shift] << a.page_shift) + (pos & ((1 << a.page_shift) - 1));
               const C* k = static_cast<const C*>(a.k_pool) + slot * a.slot_stride + (long)g * HD;
               const C* v = static_cast<const C*>(a.v_pool) + slot * a.slot_stride + (long)g * HD + d;
-              const float p = weight_of<HD, Q, C>(static_cast<const Q*>(a.q) + (long)tok * a.q_stride + (long)h * HD, k, m,
-                                                  a.scale_log2) * inv;
+              const float p = weight_of<HD>(static_cast<const Q*>(a.q) + (long)tok * a.q_stride + (long)h * HD, k, base,
+                                            a.scale_log2) * inv;
 #pragma unroll
               for (int i = 0; i < 16; ++i) f[i] += p * (float)v[i];
             }
+        }
+        if constexpr (kTermsLose<C, TERMS>) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) redo |= !(fabsf(f[i]) < INFINITY);
         }
         if (a.direct) {
           if (rr < rows) {
@@ -581,6 +578,19 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
             store4(a.part_o + to * HD + half * (HD / 2) + c + 16 - CW + chunk * 4, *place(row, chunk));
         }
         __syncwarp();
+      }
+      if constexpr (kTermsLose<C, TERMS>) {
+        if (redo && have && rr < rows && l > 0.f) {
+          const Q* q = static_cast<const Q*>(a.q) + (long)tok * a.q_stride + (long)h * HD;
+          const PoolView<C> pools(a, g, HD);
+          auto again = [&](auto* dst) {
+            uint64_t done = 0;
+            done = redo_infinite<HD>(pools, a.prefix_table, ka0, ka1, q, base, a.scale_log2, inv, dst, half * (HD / 2), 1, HD / 2, done);
+            redo_infinite<HD>(pools, own_table, kb0, see, q, base, a.scale_log2, inv, dst, half * (HD / 2), 1, HD / 2, done);
+          };
+          if (a.direct) again(static_cast<Q*>(a.out) + (long)tok * a.out_stride + (long)h * HD);
+          else again(a.part_o + at * HD);
+        }
       }
       tc_fence_before();
     }

@@ -133,3 +133,39 @@ ONLY_IDS = ["prompt", "own", "prefix"]
 @pytest.mark.parametrize("way", ONLY, ids=ONLY_IDS)
 def test_rows_whose_every_score_is_minus_infinity(way, hd, kind, cache):
     only_minus_infinity(way, hd, kind, cache)
+
+
+@pytest.mark.parametrize("kind,cache", ALL)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("way,positions", [(PROMPT, (0, 37, 70)), (RANGES, (1, 700, 2499, 2500)), (SHARED, (0, 333, 699)),
+                                           (STREAM, (0, 89, 90))], ids=["prompt", "ranges", "shared", "stream"])
+def test_an_infinite_value(way, positions, hd, kind, cache):
+    """Infinite in its own dimension, with its sign; two of opposite sign are NaN there."""
+    page = 16
+    clean = built(way, page, hd, kind, cache, seed=hd, spread=1.0)
+    slots = slots_of(clean, page, 0)
+    bad = [clean[0], clean[1], clean[2].clone(), *clean[3:]]
+    for pos in positions:
+        bad[2][slots[pos], 0, 5] = INF
+        bad[2][slots[pos], -1, hd - 1] = -INF
+    bad[2][slots[positions[0]], 0, 9] = INF
+    bad[2][slots[positions[1]], 0, 9] = -INF
+    ref = check(call(tuple(bad), page), bad, clean, page, kind, cache)
+    assert bool(torch.isposinf(ref[0, 0, 5])) and bool(torch.isneginf(ref[0, -1, -1])) and bool(torch.isnan(ref[0, 0, 9]))
+
+
+@pytest.mark.parametrize("kind,cache", ALL)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("way", [PROMPT, RANGES, SHARED, STREAM], ids=["prompt", "ranges", "shared", "stream"])
+def test_an_infinite_value_of_small_weight(way, hd, kind, cache):
+    """A weight of e^-25, below what 16-bit floats with 5 exponent bits hold, still counts."""
+    page = 16
+    clean = built(way, page, hd, kind, cache, seed=hd)
+    clean[0][:] = 1
+    clean[1][:] = 25 * hd ** -0.5
+    slots = slots_of(clean, page, 0)
+    clean[1][slots[20]] = 0
+    bad = [clean[0], clean[1], clean[2].clone(), *clean[3:]]
+    bad[2][slots[20], :, 3] = INF
+    ref = check(call(tuple(bad), page), bad, clean, page, kind, cache)
+    assert bool(torch.isposinf(ref[0, :, 3]).all())
