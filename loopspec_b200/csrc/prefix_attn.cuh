@@ -237,46 +237,74 @@ struct PoolView {
         stride(a.slot_stride), n_slots(a.n_slots), page_shift(a.page_shift) {}
 };
 
+template <int HD, typename Q, typename C>
+__device__ __forceinline__ float score_of(const Q* q, const C* k) {
+  float s = 0.f;
+  for (int i = 0; i < HD; ++i) s += (float)q[i] * (float)k[i];
+  return s;
+}
+
 // The weight of a key for a row by the formula; `base`: the row's reference in
 // powers of two, less the weights' bias.
 template <int HD, typename Q, typename C>
 __device__ __noinline__ float weight_of(const Q* q, const C* k, float base, float scale_log2) {
-  float s = 0.f;
-  for (int i = 0; i < HD; ++i) s += (float)q[i] * (float)k[i];
-  return exp2_fast(s * scale_log2 - base);
+  return exp2_fast(score_of<HD>(q, k) * scale_log2 - base);
 }
 
-// Whether the terms of P can lose an infinite value: a term of 0, or of the other
-// sign than the one before it, times infinity is NaN. An f16 term is 0 for weights
-// below 2^-32 of the reference's even where it is the only one.
+// Whether terms of q and P can make NaN of what is infinite: a term of 0, or of the
+// other sign than the one before it, times infinity is NaN, and the whole of it
+// infinite. An f16 weight is 0 below 2^-32 of the largest even as the only term.
 template <typename C, int TERMS>
 constexpr bool kTermsLose = TERMS > 1 || std::is_same<C, __half>::value;
 
-// Dimensions first + i step, i < count, of an output row that met values which are
-// not finite, at positions [p0, p1) of a table: their sum once more, by the formula.
-// What is finite in them no longer counts. `done`: a bit for each dimension begun.
+// Keys of a unit: positions [p0, p1) of a table, then [p2, p3) of another.
+struct KeyRanges {
+  const int* table;
+  int p0, p1;
+  const int* then;
+  int p2, p3;
+};
+
+// Outputs first + i step, i < count, of a unit's part of one row over again, by the
+// formula in fp32, where they are not finite; divided by the sum if `whole`. m: the
+// part's reference, which the outputs that stay refer to, or NaN where the sum is
+// not finite either. Returns (m, l).
 template <int HD, typename Q, typename C, typename D>
-__device__ __noinline__ uint64_t redo_infinite(PoolView<C> pools, const int* table, int p0, int p1, const Q* q,
-                                               float base, float scale_log2, float factor, D* dst, int first, int step,
-                                               int count, uint64_t done) {
-  for (int pos = p0; pos < p1; ++pos) {
-    const int block = table[pos >> pools.page_shift];
+__device__ __noinline__ float2 redo_row(PoolView<C> pools, KeyRanges keys, const Q* q, float scale_log2, float m, D* dst,
+                                        int first, int step, int count, bool whole) {
+  const int n = max(0, keys.p1 - keys.p0), all = n + max(0, keys.p3 - keys.p2);
+  auto slot_of = [&](int i) {                       // -1: a block that is not there, its K and V zeros
+    const int pos = i < n ? keys.p0 + i : keys.p2 + i - n;
+    const int block = (i < n ? keys.table : keys.then)[pos >> pools.page_shift];
     const long slot = ((long)block << pools.page_shift) + (pos & ((1 << pools.page_shift) - 1));
-    if (block < 0 || slot >= pools.n_slots) continue;
-    const C* v = pools.v + slot * pools.stride;
-    float w = 0.f;
-    bool weighed = false;
-    for (int i = 0; i < count; ++i) {
-      const float x = (float)v[first + i * step];
-      if (fabsf(x) < INFINITY) continue;
-      if (!weighed) w = weight_of<HD>(q, pools.k + slot * pools.stride, base, scale_log2) * factor;
-      weighed = true;
-      D* to = dst + first + i * step;
-      *to = (D)((done >> i & 1 ? (float)*to : 0.f) + w * x);
-      done |= 1ull << i;
+    return block < 0 || slot >= pools.n_slots ? -1L : slot;
+  };
+  auto score = [&](long slot) { return slot < 0 ? 0.f : score_of<HD>(q, pools.k + slot * pools.stride) * scale_log2; };
+  float l = 0.f, acc[HD / 2];
+  for (int i = 0; i < count; ++i) acc[i] = 0.f;
+  if (m != m) {
+    m = -INFINITY;
+    for (int i = 0; i < all && m == m; ++i) {
+      const float s = score(slot_of(i));
+      m = s == s ? fmaxf(m, s) : s;
     }
   }
-  return done;
+  const float base = (m == -INFINITY ? 0.f : m) - weight_bias(C());
+  if (m != m) {                                     // NaN, as all of the row
+    l = m;
+    for (int i = 0; i < count; ++i) acc[i] = m;
+  } else {
+    for (int i = 0; i < all; ++i) {
+      const long slot = slot_of(i);
+      const float w = exp2_fast(score(slot) - base);
+      l += w;
+      if (slot < 0) continue;
+      const C* v = pools.v + slot * pools.stride + first;
+      for (int d = 0; d < count; ++d) acc[d] += w * (float)v[d * step];
+    }
+  }
+  for (int i = 0; i < count; ++i) dst[first + i * step] = (D)(whole ? acc[i] * (1.f / l) : acc[i]);
+  return make_float2(m, l);
 }
 
 constexpr int kBatchRequests = 256;    // looked up at a time; 32 x 8 for the search
@@ -610,6 +638,8 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
 
       // the unit's part; the eight lanes of a row store 32 bytes side by side
       const long base = (long)(suffix ? a.prefix_parts + part : part) * a.n_tokens * a.nh;
+      int redo = 0;                                // rows whose part is not finite, by bits
+      float ref[4] = {};
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -630,17 +660,27 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
             dst[i * 16 + 8] = o[rt][i][2 + e];
           }
           if constexpr (kTermsLose<C, TERMS>) {
-            bool redo = false;
+            bool bad = TERMS > 1 && !(sum < INFINITY);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) redo |= !(fabsf(o[rt][i][e]) < INFINITY) || !(fabsf(o[rt][i][2 + e]) < INFINITY);
-            if (redo && sum > 0.f) {
-              const Q* q = static_cast<const Q*>(a.q) + (long)(start + j) * a.q_stride + (long)(g * G + r - j * G) * HD;
-              const float ref = (m[rt][e] == -INFINITY ? 0.f : m[rt][e]) - weight_bias(C());
-              redo_infinite<HD>(PoolView<C>(a, g, HD), suffix ? a.block_table + x.req * a.table_stride : a.prefix_table, k0,
-                                min(k1, see[rt][e]), q, ref, a.scale_log2, 1.f, a.part_o + row * HD, gid, 8, HD / 8, 0);
-            }
+            for (int i = 0; i < MT; ++i) bad |= !(fabsf(o[rt][i][e]) < INFINITY) || !(fabsf(o[rt][i][2 + e]) < INFINITY);
+            if (bad && (TERMS > 1 || sum < INFINITY)) redo |= 1 << (rt * 2 + e);
+            ref[rt * 2 + e] = sum < INFINITY ? m[rt][e] : NAN;
           }
         }
+      if constexpr (kTermsLose<C, TERMS>) {
+#pragma unroll 1
+        for (; redo; redo &= redo - 1) {
+          const int b = __ffs(redo) - 1, r = tile * ROWS + (b >> 1) * 8 + tig * 2 + (b & 1), j = div_by(r, G, a.g_magic);
+          const long h = (long)g * G + r - j * G, row = base + (long)(start + j) * a.nh + h;
+          const KeyRanges keys{suffix ? a.block_table + x.req * a.table_stride : a.prefix_table, k0,
+                               min(k1, suffix ? seen0 + j : len), nullptr, 0, 0};
+          const float2 ml = redo_row<HD>(PoolView<C>(a, g, HD), keys,
+                                         static_cast<const Q*>(a.q) + (long)(start + j) * a.q_stride + h * HD, a.scale_log2,
+                                         b == 0 ? ref[0] : b == 1 ? ref[1] : b == 2 ? ref[2] : ref[3], a.part_o + row * HD, gid, 8,
+                                         HD / 8, false);
+          if (gid == 0) a.part_ml[row] = ml;
+        }
+      }
     }
     cp_async_wait<0>();
   }

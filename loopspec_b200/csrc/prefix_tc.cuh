@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       const float inv = !have ? 0.f : !a.direct ? 1.f : nothing ? 0.f : 1.f / l;
       const float base = (m == -INFINITY ? 0.f : m * a.scale_log2) - weight_bias(C());
       const long at = ((long)part * a.n_tokens + tok) * a.nh + h;
-      bool redo = false;                             // some output is not finite
+      bool redo = TERMS > 1 && !(l < INFINITY);      // the sum or some output is not finite
       if (!a.direct && rr < rows && half == 0)
         a.part_ml[at] = have ? make_float2(m * a.scale_log2, l) : make_float2(-INFINITY, 0.f);
       // Parts leave by a patch of the row tile's queries, which are done with:
@@ -580,16 +580,18 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         __syncwarp();
       }
       if constexpr (kTermsLose<C, TERMS>) {
-        if (redo && have && rr < rows && l > 0.f) {
+        if (redo && have && rr < rows && (TERMS > 1 || l < INFINITY)) {
           const Q* q = static_cast<const Q*>(a.q) + (long)tok * a.q_stride + (long)h * HD;
-          const PoolView<C> pools(a, g, HD);
-          auto again = [&](auto* dst) {
-            uint64_t done = 0;
-            done = redo_infinite<HD>(pools, a.prefix_table, ka0, ka1, q, base, a.scale_log2, inv, dst, half * (HD / 2), 1, HD / 2, done);
-            redo_infinite<HD>(pools, own_table, kb0, see, q, base, a.scale_log2, inv, dst, half * (HD / 2), 1, HD / 2, done);
-          };
-          if (a.direct) again(static_cast<Q*>(a.out) + (long)tok * a.out_stride + (long)h * HD);
-          else again(a.part_o + at * HD);
+          const KeyRanges keys{a.prefix_table, ka0, ka1, own_table, kb0, see};
+          const float ref = l < INFINITY ? m * a.scale_log2 : NAN;
+          if (a.direct) {
+            redo_row<HD>(PoolView<C>(a, g, HD), keys, q, a.scale_log2, ref, static_cast<Q*>(a.out) + (long)tok * a.out_stride + (long)h * HD,
+                         half * (HD / 2), 1, HD / 2, true);
+          } else {
+            const float2 ml = redo_row<HD>(PoolView<C>(a, g, HD), keys, q, a.scale_log2, ref, a.part_o + at * HD, half * (HD / 2),
+                                           1, HD / 2, false);
+            if (half == 0) a.part_ml[at] = ml;
+          }
         }
       }
       tc_fence_before();

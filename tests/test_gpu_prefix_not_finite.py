@@ -113,6 +113,13 @@ def test_an_infinite_key(way, first, hd, kind, cache):
     infinite_key(way, first, hd, kind, cache)
 
 
+@pytest.mark.parametrize("kind,cache", SINGLE)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("way,first", INFINITE_KEY, ids=KEY_IDS)
+def test_an_infinite_key_with_fp32_queries(way, first, hd, kind, cache):
+    infinite_key(way, first, hd, kind, cache)
+
+
 def only_minus_infinity(way, hd, kind, cache):
     """0 / 0, as the formula says: not the zeros of a row that sees nothing."""
     page = 16
@@ -132,6 +139,13 @@ ONLY_IDS = ["prompt", "own", "prefix"]
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("way", ONLY, ids=ONLY_IDS)
 def test_rows_whose_every_score_is_minus_infinity(way, hd, kind, cache):
+    only_minus_infinity(way, hd, kind, cache)
+
+
+@pytest.mark.parametrize("kind,cache", SINGLE)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("way", ONLY, ids=ONLY_IDS)
+def test_rows_whose_every_score_is_minus_infinity_with_fp32_queries(way, hd, kind, cache):
     only_minus_infinity(way, hd, kind, cache)
 
 
