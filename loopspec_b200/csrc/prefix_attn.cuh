@@ -34,12 +34,17 @@
 //
 // Types: bf16 or f16 K/V. q of the cache's type enters the product exactly.
 // fp32 q enters as a sum of TERMS values of the cache's type, each the
-// rounding of what the ones before leave (bf16: 3 x 8 bits, f16: 2 x 11),
-// S = sum of the terms' products, and P likewise, so nothing of fp32's 24 bits
-// is lost to the 16-bit operands. With 16-bit q and output P is rounded once
-// to the cache's type, as fine as the output's own rounding. An f16 P is
-// scaled by 2^7 (and the sum with it), which keeps small weights and low
-// terms out of the subnormals. Scores, running max, sums and outputs are fp32.
+// rounding of what the ones before leave, S = sum of the terms' products, and P
+// likewise: bf16 3 x 8 bits, all that fp32 has; f16 2 x 11 bits, 22 of its 24 (a
+// third term would cost a half more products for errors below those of the sums).
+// For f16 each row of q is first multiplied by the power of two that brings its
+// largest element to [2^14, 2^15), and its scores' scale divided by it, so that q
+// may have any size and low terms stay out of the subnormals. With 16-bit q and
+// output P is rounded once to the cache's type, as fine as the output's own
+// rounding (errors against 64 bits, relative to the outputs' size: bf16 0.0022, 0.0017
+// without; f16 0.00027, 0.00021). An f16 P is scaled by 2^7 (and the sum with it),
+// which keeps small weights and low terms out of the subnormals. Scores, running
+// max, sums and outputs are fp32.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -177,6 +182,16 @@ __device__ __forceinline__ bool request_range(const PrefixAttnArgs& a, int i, in
   return true;
 }
 
+// The exponent shift that brings a largest |q| of `most` to [2^14, 2^15): 0 for rows of zeros and those that are not
+// finite. What it is for: f16 terms of an fp32 q.
+template <int TERMS, typename C>
+constexpr bool kScaledRows = TERMS > 1 && std::is_same<C, __half>::value;
+__device__ __forceinline__ int row_shift(float most) {
+  const int e = (int)(__float_as_uint(most) >> 23);       // biased; most >= 0
+  return e == 0xff || most == 0.f ? 0 : min(126, 127 + 14 - e);
+}
+__device__ __forceinline__ float power2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
 // Two consecutive values of a query row as fp32.
 __device__ __forceinline__ float2 load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
 __device__ __forceinline__ float2 load2(const __nv_bfloat16* p) {
@@ -237,18 +252,13 @@ struct PoolView {
         stride(a.slot_stride), n_slots(a.n_slots), page_shift(a.page_shift) {}
 };
 
-template <int HD, typename Q, typename C>
-__device__ __forceinline__ float score_of(const Q* q, const C* k) {
-  float s = 0.f;
-  for (int i = 0; i < HD; ++i) s += (float)q[i] * (float)k[i];
-  return s;
-}
-
 // The weight of a key for a row by the formula; `base`: the row's reference in
 // powers of two, less the weights' bias.
 template <int HD, typename Q, typename C>
 __device__ __noinline__ float weight_of(const Q* q, const C* k, float base, float scale_log2) {
-  return exp2_fast(score_of<HD>(q, k) * scale_log2 - base);
+  float s = 0.f;
+  for (int i = 0; i < HD; ++i) s += (float)q[i] * (float)k[i];
+  return exp2_fast(s * scale_log2 - base);
 }
 
 // Whether terms of q and P can make NaN of what is infinite: a term of 0, or of the
@@ -279,9 +289,15 @@ __device__ __noinline__ float2 redo_row(PoolView<C> pools, KeyRanges keys, const
     const long slot = ((long)block << pools.page_shift) + (pos & ((1 << pools.page_shift) - 1));
     return block < 0 || slot >= pools.n_slots ? -1L : slot;
   };
-  auto score = [&](long slot) { return slot < 0 ? 0.f : score_of<HD>(q, pools.k + slot * pools.stride) * scale_log2; };
-  float l = 0.f, acc[HD / 2];
-  for (int i = 0; i < count; ++i) acc[i] = 0.f;
+  auto score = [&](long slot) {
+    float s = 0.f;
+    if (slot >= 0) {
+      const C* k = pools.k + slot * pools.stride;
+#pragma unroll 4
+      for (int d = 0; d < HD; ++d) s += (float)q[d] * (float)k[d];
+    }
+    return s * scale_log2;
+  };
   if (m != m) {
     m = -INFINITY;
     for (int i = 0; i < all && m == m; ++i) {
@@ -290,20 +306,24 @@ __device__ __noinline__ float2 redo_row(PoolView<C> pools, KeyRanges keys, const
     }
   }
   const float base = (m == -INFINITY ? 0.f : m) - weight_bias(C());
-  if (m != m) {                                     // NaN, as all of the row
-    l = m;
-    for (int i = 0; i < count; ++i) acc[i] = m;
-  } else {
-    for (int i = 0; i < all; ++i) {
+  float l = 0.f;
+#pragma unroll 1
+  for (int d0 = 0; d0 < count; d0 += 8) {           // a few at a time: an array by itself would be in memory
+    float acc[8] = {};
+    l = 0.f;
+    for (int i = 0; i < all && m == m; ++i) {
       const long slot = slot_of(i);
       const float w = exp2_fast(score(slot) - base);
       l += w;
       if (slot < 0) continue;
-      const C* v = pools.v + slot * pools.stride + first;
-      for (int d = 0; d < count; ++d) acc[d] += w * (float)v[d * step];
+      const C* v = pools.v + slot * pools.stride + first + d0 * step;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) acc[d] += w * (float)v[d * step];
     }
+    if (m != m) l = m;                              // NaN, as all of the row
+#pragma unroll
+    for (int d = 0; d < 8; ++d) dst[first + (d0 + d) * step] = (D)(whole ? acc[d] / l : m == m ? acc[d] : m);
   }
-  for (int i = 0; i < count; ++i) dst[first + i * step] = (D)(whole ? acc[i] * (1.f / l) : acc[i]);
   return make_float2(m, l);
 }
 
@@ -485,6 +505,7 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
 
       // q of row gid of each eight as the second operand
       uint32_t qf[TERMS][RT][KS][2];
+      float row_scale[RT][2];                    // of the scores of rows 2 tig and 2 tig + 1, where rows have one of their own
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         const int r = tile * ROWS + rt * 8 + gid;
@@ -493,20 +514,41 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
           const int j = div_by(r, G, a.g_magic);
           src = static_cast<const Q*>(a.q) + (long)(start + j) * a.q_stride + (long)(g * G + r - j * G) * HD + tig * 2;
         }
+        if constexpr (TERMS == 1) {              // q is of the cache's type: as it is
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
+          for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if constexpr (TERMS == 1) {          // q is of the cache's type: as it is
+            for (int x = 0; x < 2; ++x)
               qf[0][rt][ks][x] = src ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 * x) : 0;
-            } else {
-              const float2 v = src ? load2(src + ks * 16 + 8 * x) : make_float2(0.f, 0.f);
+        } else {
+          float2 v[KS][2];
+          float most = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              v[ks][x] = src ? load2(src + ks * 16 + 8 * x) : make_float2(0.f, 0.f);
+              most = fmaxf(most, fmaxf(fabsf(v[ks][x].x), fabsf(v[ks][x].y)));
+            }
+          float up = 1.f;
+          if constexpr (kScaledRows<TERMS, C>) {
+            most = fmaxf(most, __shfl_xor_sync(kAll, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(kAll, most, 2));
+            const int shift = row_shift(most);
+            up = power2(shift);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) row_scale[rt][e] = a.scale_log2 * power2(-__shfl_sync(kAll, shift, (tig * 2 + e) * 4));
+          }
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
               uint32_t term[TERMS];
-              split2<TERMS, C>(v.x, v.y, term);
+              split2<TERMS, C>(v[ks][x].x * up, v[ks][x].y * up, term);
 #pragma unroll
               for (int i = 0; i < TERMS; ++i) qf[i][rt][ks][x] = term[i];
             }
-          }
+        }
       }
       // the scores and outputs of this thread belong to rows 2 tig and 2 tig + 1
       // of each eight: the number of positions they see
@@ -565,7 +607,7 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
             float v = acc[CHAINS - 1][rt][e];    // smallest terms first
 #pragma unroll
             for (int i = CHAINS - 2; i >= 0; --i) v += acc[i][rt][e];
-            sc[rt][e] = v * a.scale_log2;
+            sc[rt][e] = v * (kScaledRows<TERMS, C> ? row_scale[rt][e & 1] : a.scale_log2);
             if (cut) {
               const int pos = key + gid + (e >> 1) * 8;
               if (pos >= k1 || pos >= see[rt][e & 1]) sc[rt][e] = -INFINITY;

@@ -72,7 +72,9 @@ struct TcLayout {
   static constexpr int kMaxBuffers = MT == 1 ? 2 : 1;      // see the softmax warps
   static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 2 + 1 + 1;
   static constexpr int kQTiles = MT * TERMS;
-  static constexpr int kSmem = kQTiles * kTile + kStages * kTile + kMaxBuffers * MT * 2 * kTcRows * 4 + kBars * 8 + 8 * 4 + 16;
+  static constexpr int kRowScales = TERMS == 2 ? kTcRows : 0;   // see kScaledRows
+  static constexpr int kSmem = kQTiles * kTile + kStages * kTile + (kMaxBuffers * MT * 2 * kTcRows + kRowScales) * 4 + kBars * 8 +
+                               8 * 4 + 16;
   // Eighths of the exponentials on the FMA units. The softmax is bound by issue
   // slots: with heads of 128 the tensor cores take longer and none is best
   // (0, 1, 2, 3 eighths: 289, 296, 308, 326 us for 2100 tokens behind 8192
@@ -298,8 +300,9 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
   unsigned char* s_q = smem;
   unsigned char* s_ring = smem + L::kQTiles * L::kTile;
   float* s_max = reinterpret_cast<float*>(s_ring + ST * L::kTile);   // [kMaxBuffers][MT][half][row]
-  const uint32_t bars = smem_u32(s_max + L::kMaxBuffers * MT * 2 * kTcRows);
-  uint32_t* s_bad = reinterpret_cast<uint32_t*>(s_max + L::kMaxBuffers * MT * 2 * kTcRows) + 2 * L::kBars;   // [8] bits
+  float* s_scale = s_max + L::kMaxBuffers * MT * 2 * kTcRows;        // [kRowScales]
+  const uint32_t bars = smem_u32(s_scale + L::kRowScales);
+  uint32_t* s_bad = reinterpret_cast<uint32_t*>(s_scale + L::kRowScales) + 2 * L::kBars;   // [8] bits
   uint32_t* s_tmem = s_bad + 8;
   const uint32_t full0 = bars, empty0 = full0 + 8 * ST, s_full = empty0 + 8 * ST, p_full = s_full + 16,
                  pv_done = p_full + 16, o_done = pv_done + 16, q_full = o_done + 16, noted = q_full + 8;
@@ -392,6 +395,18 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         } else {
           float f[8];
           v[k].get(f);
+          if constexpr (kScaledRows<TERMS, C>) {
+            float most = 0.f;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) most = fmaxf(most, fabsf(f[x]));
+#pragma unroll
+            for (int x = 1; x < CH; x <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, x));   // CH lanes a row
+            const int shift = row_shift(most);
+            const float up = power2(shift);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) f[x] *= up;
+            if (c == 0) s_scale[r] = a.scale_log2 * power2(-shift);
+          }
           uint32_t term[4][TERMS];
 #pragma unroll
           for (int x = 0; x < 4; ++x) split2<TERMS, C>(f[2 * x], f[2 * x + 1], term[x]);
@@ -403,6 +418,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
+      if constexpr (kScaledRows<TERMS, C>) asm volatile("bar.sync 9, 256;" ::: "memory");   // the row tile's scales are there
     }
     const int r = quarter * 32 + lane, rr = row0 + t * kTcRows + r;
     if (quarter < live_warps(t)) {
@@ -413,6 +429,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       const int row_tok = div_by(rr, G, a.g_magic);
       const int see = rr < rows ? min(kb1, seen0 + row_tok) : kb1;
       const int see_least = __reduce_min_sync(0xffffffffu, see);
+      const float scale_log2 = kScaledRows<TERMS, C> ? s_scale[r] : a.scale_log2;
       float m = -INFINITY, l = 0.f;
       bool ok = true;
       for (int j = 0; j < n; ++j) {
@@ -449,9 +466,9 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         top = max2_nan(top, row_max[(half ^ 1) * kTcRows]);
         // m and top are raw scores; their distance counts after the scale. A NaN
         // score makes the reference NaN, and with it the whole row
-        const bool move = m == -INFINITY ? top != -INFINITY : !((top - m) * a.scale_log2 <= kGrow);
+        const bool move = m == -INFINITY ? top != -INFINITY : !((top - m) * scale_log2 <= kGrow);
         if (__any_sync(0xffffffffu, move)) {
-          const float keep = move && m > -INFINITY ? exp2_fast((m - top) * a.scale_log2) : 1.f;
+          const float keep = move && m > -INFINITY ? exp2_fast((m - top) * scale_log2) : 1.f;
           if (move) m = top;
           // inf - inf: the row is NaN, whichever way its weights are computed
           l = m == INFINITY ? NAN : l * keep;
@@ -469,10 +486,10 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
             }
           }
         }
-        const float base = (m == -INFINITY ? 0.f : m * a.scale_log2) - weight_bias(C());
+        const float base = (m == -INFINITY ? 0.f : m * scale_log2) - weight_bias(C());
         // Of eight pairs kPoly go to the FMA units, the others to the special
         // function units, which do 4 of these a cycle and SM quarter
-        const uint64_t scale = pair(a.scale_log2, a.scale_log2), minus = pair(-base, -base);
+        const uint64_t scale = pair(scale_log2, scale_log2), minus = pair(-base, -base);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int i0 = 0; i0 < 32; i0 += 16) {
@@ -517,11 +534,11 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       // zeros for a row that sees nothing; one whose scores are all -inf is 0 / 0
       const bool nothing = a.prefix_len == 0 && see <= 0;
       const float inv = !have ? 0.f : !a.direct ? 1.f : nothing ? 0.f : 1.f / l;
-      const float base = (m == -INFINITY ? 0.f : m * a.scale_log2) - weight_bias(C());
+      const float base = (m == -INFINITY ? 0.f : m * scale_log2) - weight_bias(C());
       const long at = ((long)part * a.n_tokens + tok) * a.nh + h;
       bool redo = TERMS > 1 && !(l < INFINITY);      // the sum or some output is not finite
       if (!a.direct && rr < rows && half == 0)
-        a.part_ml[at] = have ? make_float2(m * a.scale_log2, l) : make_float2(-INFINITY, 0.f);
+        a.part_ml[at] = have ? make_float2(m * scale_log2, l) : make_float2(-INFINITY, 0.f);
       // Parts leave by a patch of the row tile's queries, which are done with:
       // a warp's rows by CW columns, 16-byte chunks swizzled, so that it stores
       // whole rows of 4 CW bytes (a thread storing its own row by itself
@@ -583,7 +600,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         if (redo && have && rr < rows && (TERMS > 1 || l < INFINITY)) {
           const Q* q = static_cast<const Q*>(a.q) + (long)tok * a.q_stride + (long)h * HD;
           const KeyRanges keys{a.prefix_table, ka0, ka1, own_table, kb0, see};
-          const float ref = l < INFINITY ? m * a.scale_log2 : NAN;
+          const float ref = l < INFINITY ? m * scale_log2 : NAN;
           if (a.direct) {
             redo_row<HD>(PoolView<C>(a, g, HD), keys, q, a.scale_log2, ref, static_cast<Q*>(a.out) + (long)tok * a.out_stride + (long)h * HD,
                          half * (HD / 2), 1, HD / 2, true);
