@@ -757,15 +757,16 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
   // no early launch of what follows: CTAs of the next call that wait here took
   // the places of this call's last ones (16 requests behind 2048 positions with
   // fp32 queries, call after call: 31.6 us with it, 22.6 without)
-  // whether a valid request holds the token: written by no kernel of the call
+  // Whether a valid request holds the token: written by no kernel of the call. This
+  // also tells of ranges that are out of bounds where no kernel ran for the requests'
+  // own positions (max_new or max_len is 0).
   bool mine = false;
   for (int i = threadIdx.x; i < a.n_requests; i += kJoinThreads) {
-    const int start = a.token_start[i], end = a.token_start[i + 1], len = a.lens[i];
-    if (t >= start && t < end && start >= 0 && end - start <= a.max_new && end <= a.n_tokens && len >= 0 &&
-        len <= a.max_len) {
+    int start, n, len;
+    if (request_range(a, i, start, n, len) && t >= start && t - start < n) {
       mine = true;
       s_len = len;
-      s_seen = len - (end - start) + 1 + (t - start);
+      s_seen = len - n + 1 + (t - start);
     }
   }
   const bool ok = __syncthreads_or(mine);

@@ -32,6 +32,27 @@ def test_a_token_range_out_of_bounds_among_prompts_leaves_valid_requests_whole(p
     assert not bool(out[~held].any())
 
 
+@pytest.mark.parametrize("counts,nh", [([1, 1], 4), ([1] * 30, 2)])
+@pytest.mark.parametrize("fault", ["max_new 0", "max_len 0", "both 0"])
+def test_bounds_of_zero_are_bounds(counts, nh, fault):
+    """No kernel of the requests' own positions runs then; tokens or lengths past the bound are told all the same."""
+    from loopspec_b200 import _lib
+    from loopspec_b200.status import DeviceStatus
+    c = make(counts, [3] * len(counts), 50, 16, nh, 2, 64, "bf16", "bf16", seed=2)
+    bounds = dict(max_new=0 if fault != "max_len 0" else 1, max_len=0 if fault != "max_new 0" else 16)
+    status = DeviceStatus("cuda")
+    out = call(c, 16, status=status, **bounds)
+    assert not bool(out.any())
+    with pytest.raises(_lib.EngineError) as err:
+        status.check()
+    assert err.value.code == _lib.LS_EDEVICE
+    # and within the bounds nothing is told
+    ok = make([0 if bounds["max_new"] == 0 else n for n in counts], [0 if bounds["max_len"] == 0 else 3] * len(counts), 50,
+              16, nh, 2, 64, "bf16", "bf16", seed=2, pad=2)
+    call(ok, 16, status=status, **bounds)
+    status.check()
+
+
 def test_padding_of_more_than_32_bits_of_elements():
     """A prompt of 130 tokens and 2^27 rows of padding: 2^31 pieces of four elements to clear, and one token's more."""
     from loopspec_b200.prefix_attention import prefix_attention
