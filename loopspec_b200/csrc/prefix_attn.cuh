@@ -201,6 +201,13 @@ __device__ __forceinline__ float2 load2(const __half* p) {
   return unpack2(*reinterpret_cast<const uint32_t*>(p), __half());
 }
 
+// A maximum that is NaN when an operand is.
+__device__ __forceinline__ float max2_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 constexpr float kGrow = 8.f;   // log2 growth of a row's maximum that moves its reference
 
 // Whether a warp's 16 V rows in shared memory hold a NaN or infinity (exponent bits all set).
@@ -263,9 +270,11 @@ __device__ __noinline__ float weight_of(const Q* q, const C* k, float base, floa
 
 // Whether terms of q and P can make NaN of what is infinite: a term of 0, or of the
 // other sign than the one before it, times infinity is NaN, and the whole of it
-// infinite. An f16 weight is 0 below 2^-32 of the largest even as the only term.
-template <typename C, int TERMS>
-constexpr bool kTermsLose = TERMS > 1 || std::is_same<C, __half>::value;
+// infinite. An f16 weight is 0 below 2^-32 of the largest even as the only term. So
+// rows that come out not finite are computed once more by the formula, where they
+// are whole: in the joining pass, or at the end of a unit that is all of its rows.
+template <typename Q, typename C>
+constexpr bool kTermsLose = !std::is_same<Q, C>::value || std::is_same<C, __half>::value;
 
 // Keys of a unit: positions [p0, p1) of a table, then [p2, p3) of another.
 struct KeyRanges {
@@ -275,56 +284,60 @@ struct KeyRanges {
   int p2, p3;
 };
 
-// Outputs first + i step, i < count, of a unit's part of one row over again, by the
-// formula in fp32, where they are not finite; divided by the sum if `whole`. m: the
-// part's reference, which the outputs that stay refer to, or NaN where the sum is
-// not finite either. Returns (m, l).
-template <int HD, typename Q, typename C, typename D>
-__device__ __noinline__ float2 redo_row(PoolView<C> pools, KeyRanges keys, const Q* q, float scale_log2, float m, D* dst,
-                                        int first, int step, int count, bool whole) {
-  const int n = max(0, keys.p1 - keys.p0), all = n + max(0, keys.p3 - keys.p2);
-  auto slot_of = [&](int i) {                       // -1: a block that is not there, its K and V zeros
-    const int pos = i < n ? keys.p0 + i : keys.p2 + i - n;
-    const int block = (i < n ? keys.table : keys.then)[pos >> pools.page_shift];
-    const long slot = ((long)block << pools.page_shift) + (pos & ((1 << pools.page_shift) - 1));
-    return block < 0 || slot >= pools.n_slots ? -1L : slot;
-  };
-  auto score = [&](long slot) {
-    float s = 0.f;
-    if (slot >= 0) {
-      const C* k = pools.k + slot * pools.stride;
+// slot of key i of the ranges; -1: a block that is not there, its K and V are zeros
+template <typename C>
+__device__ __forceinline__ long slot_of(const PoolView<C>& pools, const KeyRanges& keys, int i) {
+  const int n = max(0, keys.p1 - keys.p0), pos = i < n ? keys.p0 + i : keys.p2 + i - n;
+  const int block = (i < n ? keys.table : keys.then)[pos >> pools.page_shift];
+  const long slot = ((long)block << pools.page_shift) + (pos & ((1 << pools.page_shift) - 1));
+  return block < 0 || slot >= pools.n_slots ? -1L : slot;
+}
+__device__ __forceinline__ int keys_in(const KeyRanges& keys) { return max(0, keys.p1 - keys.p0) + max(0, keys.p3 - keys.p2); }
+
+// score in powers of two
+template <int HD, typename Q, typename C>
+__device__ __forceinline__ float score_of(const PoolView<C>& pools, long slot, const Q* q, float scale_log2) {
+  float s = 0.f;
+  if (slot >= 0) {
+    const C* k = pools.k + slot * pools.stride;
 #pragma unroll 4
-      for (int d = 0; d < HD; ++d) s += (float)q[d] * (float)k[d];
-    }
-    return s * scale_log2;
-  };
-  if (m != m) {
-    m = -INFINITY;
-    for (int i = 0; i < all && m == m; ++i) {
-      const float s = score(slot_of(i));
-      m = s == s ? fmaxf(m, s) : s;
-    }
+    for (int d = 0; d < HD; ++d) s += (float)q[d] * (float)k[d];
   }
-  const float base = (m == -INFINITY ? 0.f : m) - weight_bias(C());
+  return s * scale_log2;
+}
+
+// A row's whole result by the formula in fp32, columns c .. c + 3, by the HD / 4
+// lanes of its group: each weighs a key, all add its value. Inlined: a kernel with
+// a call in it took 0.6 us more with 256 CTAs, 3 with 1024, though none called.
+template <int HD, typename Q, typename C>
+__device__ __forceinline__ float4 row_by_formula(PoolView<C> pools, KeyRanges keys, const Q* q, float scale_log2, int c,
+                                              unsigned group) {
+  constexpr int L = HD / 4;
+  const int lane = threadIdx.x % L, all = keys_in(keys);
+  float m = -INFINITY;
+  for (int i = lane; i < all; i += L) m = max2_nan(m, score_of<HD>(pools, slot_of(pools, keys, i), q, scale_log2));
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) m = max2_nan(m, __shfl_xor_sync(group, m, o));
+  if (m != m) return make_float4(m, m, m, m);
+  const float base = m == -INFINITY ? 0.f : m;
   float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < all; i0 += L) {
+    const int slot = i0 + lane < all ? (int)slot_of(pools, keys, i0 + lane) : -1;
+    const float w = i0 + lane < all ? exp2_fast(score_of<HD>(pools, slot, q, scale_log2) - base) : 0.f;
+    l += w;
 #pragma unroll 1
-  for (int d0 = 0; d0 < count; d0 += 8) {           // a few at a time: an array by itself would be in memory
-    float acc[8] = {};
-    l = 0.f;
-    for (int i = 0; i < all && m == m; ++i) {
-      const long slot = slot_of(i);
-      const float w = exp2_fast(score(slot) - base);
-      l += w;
-      if (slot < 0) continue;
-      const C* v = pools.v + slot * pools.stride + first + d0 * step;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) acc[d] += w * (float)v[d * step];
+    for (int k = 0; k < L; ++k) {
+      const float wk = __shfl_sync(group, w, k, L);
+      const int sk = __shfl_sync(group, slot, k, L);
+      if (sk < 0) continue;
+      const C* v = pools.v + sk * pools.stride + c;
+      acc = make_float4(acc.x + wk * (float)v[0], acc.y + wk * (float)v[1], acc.z + wk * (float)v[2], acc.w + wk * (float)v[3]);
     }
-    if (m != m) l = m;                              // NaN, as all of the row
-#pragma unroll
-    for (int d = 0; d < 8; ++d) dst[first + (d0 + d) * step] = (D)(whole ? acc[d] / l : m == m ? acc[d] : m);
   }
-  return make_float2(m, l);
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) l += __shfl_xor_sync(group, l, o);
+  return make_float4(acc.x / l, acc.y / l, acc.z / l, acc.w / l);
 }
 
 constexpr int kBatchRequests = 256;    // looked up at a time; 32 x 8 for the search
@@ -521,17 +534,16 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
             for (int x = 0; x < 2; ++x)
               qf[0][rt][ks][x] = src ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 * x) : 0;
         } else {
-          float2 v[KS][2];
-          float most = 0.f;
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              v[ks][x] = src ? load2(src + ks * 16 + 8 * x) : make_float2(0.f, 0.f);
-              most = fmaxf(most, fmaxf(fabsf(v[ks][x].x), fabsf(v[ks][x].y)));
-            }
           float up = 1.f;
           if constexpr (kScaledRows<TERMS, C>) {
+            float most = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                const float2 v = src ? load2(src + ks * 16 + 8 * x) : make_float2(0.f, 0.f);
+                most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
+              }
             most = fmaxf(most, __shfl_xor_sync(kAll, most, 1));
             most = fmaxf(most, __shfl_xor_sync(kAll, most, 2));
             const int shift = row_shift(most);
@@ -543,8 +555,9 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
           for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
+              const float2 v = src ? load2(src + ks * 16 + 8 * x) : make_float2(0.f, 0.f);
               uint32_t term[TERMS];
-              split2<TERMS, C>(v[ks][x].x * up, v[ks][x].y * up, term);
+              split2<TERMS, C>(v.x * up, v.y * up, term);
 #pragma unroll
               for (int i = 0; i < TERMS; ++i) qf[i][rt][ks][x] = term[i];
             }
@@ -680,8 +693,6 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
 
       // the unit's part; the eight lanes of a row store 32 bytes side by side
       const long base = (long)(suffix ? a.prefix_parts + part : part) * a.n_tokens * a.nh;
-      int redo = 0;                                // rows whose part is not finite, by bits
-      float ref[4] = {};
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -701,28 +712,7 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
             dst[i * 16] = o[rt][i][e];
             dst[i * 16 + 8] = o[rt][i][2 + e];
           }
-          if constexpr (kTermsLose<C, TERMS>) {
-            bool bad = TERMS > 1 && !(sum < INFINITY);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) bad |= !(fabsf(o[rt][i][e]) < INFINITY) || !(fabsf(o[rt][i][2 + e]) < INFINITY);
-            if (bad && (TERMS > 1 || sum < INFINITY)) redo |= 1 << (rt * 2 + e);
-            ref[rt * 2 + e] = sum < INFINITY ? m[rt][e] : NAN;
-          }
         }
-      if constexpr (kTermsLose<C, TERMS>) {
-#pragma unroll 1
-        for (; redo; redo &= redo - 1) {
-          const int b = __ffs(redo) - 1, r = tile * ROWS + (b >> 1) * 8 + tig * 2 + (b & 1), j = div_by(r, G, a.g_magic);
-          const long h = (long)g * G + r - j * G, row = base + (long)(start + j) * a.nh + h;
-          const KeyRanges keys{suffix ? a.block_table + x.req * a.table_stride : a.prefix_table, k0,
-                               min(k1, suffix ? seen0 + j : len), nullptr, 0, 0};
-          const float2 ml = redo_row<HD>(PoolView<C>(a, g, HD), keys,
-                                         static_cast<const Q*>(a.q) + (long)(start + j) * a.q_stride + h * HD, a.scale_log2,
-                                         b == 0 ? ref[0] : b == 1 ? ref[1] : b == 2 ? ref[2] : ref[3], a.part_o + row * HD, gid, 8,
-                                         HD / 8, false);
-          if (gid == 0) a.part_ml[row] = ml;
-        }
-      }
     }
     cp_async_wait<0>();
   }
@@ -745,13 +735,15 @@ constexpr int kJoinBatch = 4;
 // each has a row of its own. grid: (token, heads over the rows of a CTA).
 // Tokens past token_start[R] and those of a request that was skipped get zeros,
 // as do rows that see nothing. Bound: the latency of two loads (lengths; parts,
-// all at once) after the parts are there.
-template <int HD, typename Q, bool SPLIT>
-__global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArgs a) {
+// all at once) after the parts are there; told that one CTA an SM will do, the
+// compiler takes the registers that this needs (48; 40 otherwise: 23.7 us a call
+// with 16 requests behind 2048 positions and fp32 queries, 23.3 so).
+template <int HD, typename Q, typename C, bool SPLIT>
+__global__ void __launch_bounds__(kJoinThreads, 1) prefix_join_kernel(PrefixAttnArgs a) {
   constexpr int TPR = HD / 4, GROUPS = kJoinThreads / TPR;
   __shared__ float4 s_acc[SPLIT ? GROUPS : 1][TPR];
   __shared__ float2 s_ml[GROUPS];
-  __shared__ int s_len, s_seen;   // own positions of the token's request, and those that the token sees
+  __shared__ int s_req, s_len, s_seen;   // the token's request, its own positions, and those that the token sees
   const int t = blockIdx.x;
   if (!a.behind) pdl_wait();
   // no early launch of what follows: CTAs of the next call that wait here took
@@ -765,6 +757,7 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
     int start, n, len;
     if (request_range(a, i, start, n, len) && t >= start && t - start < n) {
       mine = true;
+      s_req = i;
       s_len = len;
       s_seen = len - n + 1 + (t - start);
     }
@@ -835,8 +828,18 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(PrefixAttnArg
     }
   }
   // zeros for a row that sees nothing; one whose scores are all -inf is 0 / 0
-  const float inv = !ok || (a.prefix_len == 0 && s_seen <= 0) ? 0.f : 1.f / ll;
+  const bool sees = ok && (a.prefix_len > 0 || s_seen > 0);
+  const float inv = sees ? 1.f / ll : 0.f;
   acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  if constexpr (kTermsLose<Q, C>) {                 // a row that is not finite, by the formula
+    const unsigned group_lanes = TPR == 32 ? 0xffffffffu : 0xffffu << (threadIdx.x & 16);
+    const float zero = fmaf(acc.x, 0.f, fmaf(acc.y, 0.f, fmaf(acc.z, 0.f, acc.w * 0.f)));
+    if (__any_sync(group_lanes, sees && zero != 0.f)) {
+      const KeyRanges keys{a.prefix_table, 0, a.prefix_len, a.block_table + s_req * a.table_stride, 0, s_seen};
+      acc = row_by_formula<HD>(PoolView<C>(a, h / (a.nh / a.nkv), HD), keys,
+                               static_cast<const Q*>(a.q) + (long)t * a.q_stride + (long)h * HD, a.scale_log2, c, group_lanes);
+    }
+  }
   store4(static_cast<Q*>(a.out) + (long)t * a.out_stride + (long)h * HD + c, acc);
 }
 

@@ -198,12 +198,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// Maxima that are NaN when an operand is.
-__device__ __forceinline__ float max2_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
+// As max2_nan, of three.
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   float d;
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -276,6 +271,29 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* r) {
 __device__ __forceinline__ void cp_async16_to(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+// Columns first .. first + HD / 2 of a row by the formula in fp32, by one thread.
+template <int HD, typename Q, typename C>
+__device__ __noinline__ void redo_row(PoolView<C> pools, KeyRanges keys, const Q* q, float scale_log2, Q* dst, int first) {
+  const int all = keys_in(keys);
+  float m = -INFINITY;
+  for (int i = 0; i < all; ++i) m = max2_nan(m, score_of<HD>(pools, slot_of(pools, keys, i), q, scale_log2));
+  const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+  for (int d0 = first; d0 < first + HD / 2; d0 += 8) {   // a few at a time: an array by itself would be in memory
+    float l = 0.f, acc[8] = {};
+    for (int i = 0; i < all && m == m; ++i) {
+      const long slot = slot_of(pools, keys, i);
+      const float w = exp2_fast(score_of<HD>(pools, slot, q, scale_log2) - base);
+      l += w;
+      if (slot < 0) continue;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) acc[d] += w * (float)pools.v[slot * pools.stride + d0 + d];
+    }
+#pragma unroll
+    for (int d = 0; d < 8; ++d) dst[d0 + d] = (Q)(m == m ? acc[d] / l : m);
+  }
 }
 
 // Whether 8 packed 16-bit values hold a NaN or infinity (exponent bits all set).
@@ -536,7 +554,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       const float inv = !have ? 0.f : !a.direct ? 1.f : nothing ? 0.f : 1.f / l;
       const float base = (m == -INFINITY ? 0.f : m * scale_log2) - weight_bias(C());
       const long at = ((long)part * a.n_tokens + tok) * a.nh + h;
-      bool redo = TERMS > 1 && !(l < INFINITY);      // the sum or some output is not finite
+      float zero = 0.f;                              // NaN if some output is not finite
       if (!a.direct && rr < rows && half == 0)
         a.part_ml[at] = have ? make_float2(m * scale_log2, l) : make_float2(-INFINITY, 0.f);
       // Parts leave by a patch of the row tile's queries, which are done with:
@@ -571,9 +589,9 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
               for (int i = 0; i < 16; ++i) f[i] += p * (float)v[i];
             }
         }
-        if constexpr (kTermsLose<C, TERMS>) {
+        if constexpr (kTermsLose<Q, C>) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) redo |= !(fabsf(f[i]) < INFINITY);
+          for (int i = 0; i < 16; ++i) zero = fmaf(f[i], 0.f, zero);
         }
         if (a.direct) {
           if (rr < rows) {
@@ -596,20 +614,11 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         }
         __syncwarp();
       }
-      if constexpr (kTermsLose<C, TERMS>) {
-        if (redo && have && rr < rows && (TERMS > 1 || l < INFINITY)) {
-          const Q* q = static_cast<const Q*>(a.q) + (long)tok * a.q_stride + (long)h * HD;
-          const KeyRanges keys{a.prefix_table, ka0, ka1, own_table, kb0, see};
-          const float ref = l < INFINITY ? m * scale_log2 : NAN;
-          if (a.direct) {
-            redo_row<HD>(PoolView<C>(a, g, HD), keys, q, a.scale_log2, ref, static_cast<Q*>(a.out) + (long)tok * a.out_stride + (long)h * HD,
-                         half * (HD / 2), 1, HD / 2, true);
-          } else {
-            const float2 ml = redo_row<HD>(PoolView<C>(a, g, HD), keys, q, a.scale_log2, ref, a.part_o + at * HD, half * (HD / 2),
-                                           1, HD / 2, false);
-            if (half == 0) a.part_ml[at] = ml;
-          }
-        }
+      if constexpr (kTermsLose<Q, C>) {
+        if (a.direct && zero != 0.f && have && rr < rows)
+          redo_row<HD>(PoolView<C>(a, g, HD), KeyRanges{a.prefix_table, ka0, ka1, own_table, kb0, see},
+                       static_cast<const Q*>(a.q) + (long)tok * a.q_stride + (long)h * HD, a.scale_log2,
+                       static_cast<Q*>(a.out) + (long)tok * a.out_stride + (long)h * HD, half * (HD / 2));
       }
       tc_fence_before();
     }

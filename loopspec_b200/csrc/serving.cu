@@ -388,8 +388,8 @@ void launch_prefix(PrefixAttnArgs a, const PrefixPlan& plan, cudaStream_t stream
   // many parts come with few rows: a row's parts are shared out (4 requests behind
   // 333 positions: 7.0 us, 9.0 with a group a row; 16 behind 2048: 22.4 and 29.6)
   if (a.prefix_parts + a.suffix_parts > kJoinBatch)
-    launch(prefix_join_kernel<HD, Q, true>, rows, dim3(kJoinThreads), 0, stream, true, a);
-  else launch(prefix_join_kernel<HD, Q, false>, groups, dim3(kJoinThreads), 0, stream, true, a);
+    launch(prefix_join_kernel<HD, Q, C, true>, rows, dim3(kJoinThreads), 0, stream, true, a);
+  else launch(prefix_join_kernel<HD, Q, C, false>, groups, dim3(kJoinThreads), 0, stream, true, a);
 }
 
 template <typename Q, typename C, int TERMS>
