@@ -364,8 +364,9 @@ int ls_check_status(int32_t* status, void* stream);
  * the request) and its request; entries past it get -1, 0, -1. All or nothing:
  * when a length is out of range, the blocks do not suffice or the tokens do
  * not fit, lens and the count keep their values, table and stack are left
- * alone, token_start is all 0 and *status tells why. lens_out / free_count_out
- * may be lens / free_count. */
+ * alone, token_start is all 0 and *status tells why. A table entry that is no
+ * block is told too: a token in it gets slot -1, and given back it goes on the
+ * stack as it is. lens_out / free_count_out may be lens / free_count. */
 typedef struct ls_slots_args {
   const int32_t* lens;        /* [R]                                          */
   const int32_t* delta;       /* [R]                                          */

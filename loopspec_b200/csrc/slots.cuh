@@ -221,7 +221,11 @@ __global__ void __launch_bounds__(kSlotThreads) build_slots_kernel(SlotArgs a) {
     const int have = (a.lens[i] + page - 1) >> a.page_shift;
     a.table[i * a.table_stride + have + ((int)k - s_grow[i])] = taken((int)k);
   }
-  for (long p = count + at; p < count + n_give - n_take; p += step) a.free_blocks[p] = given((int)(p - count));
+  for (long p = count + at; p < count + n_give - n_take; p += step) {
+    const int block = given((int)(p - count));
+    if (block < 0 || block >= a.n_blocks) atomicCAS(a.status, kDevOk, kDevBadIndex);   // taken ones are told by their token
+    a.free_blocks[p] = block;
+  }
   for (unsigned i = at; i <= n_req; i += step) a.token_start[i] = s_tok[i];
   if (a.in_place) cg::this_cluster().sync();   // every CTA has read lens and the count
   for (unsigned i = at; i < n_req; i += step) a.lens_out[i] = a.lens[i] + a.delta[i];

@@ -31,6 +31,29 @@ def test_any_number_of_requests_in_a_process_that_made_no_call_before(n):
     assert run.returncode == 0, run.stderr[-2000:]
 
 
+@pytest.mark.parametrize("table,lens,delta", [
+    ([[99, 1]], [2], [-2]),            # released: both blocks go back
+    ([[0, -4]], [2], [-1]),            # cut back: one does
+    ([[0, 3]], [2], [-1]),             # the first block that is not there
+])
+def test_a_bad_block_that_is_given_back_is_reported(table, lens, delta):
+    from loopspec_b200 import _lib
+    from loopspec_b200.slots import SlotMap, build_slots
+    from loopspec_b200.status import DeviceStatus
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for bad in (True, False):
+        tab = i32(table if bad else [[0, 1]])
+        status = DeviceStatus("cuda")
+        build_slots(i32(lens), i32(delta), tab, i32([2, -1, -1]), i32([1]), page_size=1, n_blocks=3, out=SlotMap(1, 4),
+                    status=status)
+        if not bad:
+            status.check()
+            continue
+        with pytest.raises(_lib.EngineError) as err:
+            status.check()
+        assert err.value.code == _lib.LS_EDEVICE
+
+
 def test_token_buffers_of_2_31_entries():
     """The loop over the token buffers passes the last entry without running past 32 bits."""
     from loopspec_b200.slots import SlotMap, build_slots
