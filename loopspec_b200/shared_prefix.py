@@ -69,9 +69,14 @@ class PrefixBatch:
                                 workspace=self.workspace, status=self.status)
 
     def share(self, request, length):
-        """Make the `length` positions of `request` the prefix of all; the request is empty afterwards."""
+        """Make the first `length` positions of `request` the prefix of all, for as long as the batch lives; the
+        request is empty afterwards. Waits for the GPU."""
         if self.prefix_len:
             raise ValueError("the batch has a prefix already")
+        held = self.lens.tolist()
+        cut = torch.zeros(len(held), dtype=torch.int32)
+        cut[request] = length - held[request]
+        self.begin(cut.to(self.lens.device), 0, 0)       # blocks past the prefix go back
         blocks = -(-length // self.page_size)
         self.prefix_table = self.table[request, :blocks].clone()
         self.prefix_len = length
