@@ -74,6 +74,8 @@ class PrefixBatch:
         if self.prefix_len:
             raise ValueError("the batch has a prefix already")
         held = self.lens.tolist()
+        if not (0 <= request < len(held) and 0 < length <= held[request]):
+            raise ValueError(f"request {request} does not hold {length} positions")
         cut = torch.zeros(len(held), dtype=torch.int32)
         cut[request] = length - held[request]
         self.begin(cut.to(self.lens.device), 0, 0)       # blocks past the prefix go back

@@ -37,3 +37,12 @@ def test_every_block_is_the_prefixs_or_free(held, length):
     batch.check()
     assert sorted(sum(blocks(batch), [])) == list(range(N_BLOCKS))
     assert batch.map.positions[:2].tolist() == [length, length + 1]
+
+
+@pytest.mark.parametrize("request_, length", [(1, 34), (1, 0), (1, -3), (0, 1), (3, 5), (-1, 5)])
+def test_a_length_that_the_request_does_not_hold_is_refused(request_, length):
+    batch = batch_of([0, 33, 0])
+    before = blocks(batch)
+    with pytest.raises(ValueError):
+        batch.share(request_, length)
+    assert blocks(batch) == before and batch.prefix_len == 0
