@@ -76,6 +76,8 @@ class PrefixBatch:
         held = self.lens.tolist()
         if not (0 <= request < len(held) and 0 < length <= held[request]):
             raise ValueError(f"request {request} does not hold {length} positions")
+        if sum(held) != held[request]:
+            raise ValueError("the other requests must be empty: their keys are rotated for positions from 0 on")
         cut = torch.zeros(len(held), dtype=torch.int32)
         cut[request] = length - held[request]
         self.begin(cut.to(self.lens.device), 0, 0)       # blocks past the prefix go back

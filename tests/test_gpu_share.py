@@ -46,3 +46,17 @@ def test_a_length_that_the_request_does_not_hold_is_refused(request_, length):
     with pytest.raises(ValueError):
         batch.share(request_, length)
     assert blocks(batch) == before and batch.prefix_len == 0
+
+
+def test_other_requests_with_positions_are_refused():
+    """Their keys were rotated for positions that count from 0; behind the prefix they would count from its end."""
+    batch = batch_of([7, 33, 0])
+    before = blocks(batch)
+    with pytest.raises(ValueError):
+        batch.share(1, 33)
+    assert blocks(batch) == before and batch.prefix_len == 0
+    batch.begin(torch.tensor([-7, 0, 0], dtype=torch.int32, device="cuda"), 0, 0)
+    batch.share(1, 33)
+    with pytest.raises(ValueError):          # one prefix a batch
+        batch.share(2, 1)
+    batch.check()
