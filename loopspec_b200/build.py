@@ -1,5 +1,6 @@
 """Build libloopspec_engine.so in-tree for sm_100a with nvcc, and beside it the
-CPython module _tensor_facts.so (host code that reads torch tensors).
+CPython module _tensor_facts.so (host code that reads torch tensors; where torch
+is installed).
 
     python -m loopspec_b200.build            # rebuild if any source is newer
     python -m loopspec_b200.build --force
@@ -8,6 +9,7 @@ CPython module _tensor_facts.so (host code that reads torch tensors).
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -46,12 +48,20 @@ def build(force: bool = False, verbose: bool = False) -> str:
         finish_facts(facts)
 
 
+def torch_root():
+    """Where torch is installed (it is not imported), or None."""
+    spec = importlib.util.find_spec("torch")
+    return spec and os.path.dirname(spec.origin)
+
+
 def build_facts(force):
-    """Start the compiler on the tensor module; None if it is newer than its source."""
+    """Start the compiler on the tensor module; None if it is newer than its source, or without torch, whose tensors
+    it reads: the library by itself needs none."""
     if not force and os.path.exists(FACTS_OUT) and os.path.getmtime(FACTS_OUT) >= os.path.getmtime(FACTS_SRC):
         return None
-    import torch
-    root = os.path.dirname(torch.__file__)
+    root = torch_root()
+    if root is None:
+        return None
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                 sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
