@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libloopspec_engine.so")
@@ -200,10 +201,15 @@ def tensor_facts():
     in one call each, for the operators whose whole call takes microseconds."""
     global _FACTS
     if _FACTS is None:
+        import torch
+        how = "build it with `python -m loopspec_b200.build`"
         try:
             from . import _tensor_facts
         except ImportError as e:
-            raise ImportError(f"{e}: build it with `python -c 'import loopspec_b200.build as b; b.build()'`") from e
+            raise ImportError(f"{e}: {how}") from e
+        here = (torch.__version__.split("+")[0], *sys.version_info[:2])
+        if _tensor_facts.made_for != here:      # its reading of tensors goes by the layout of that version's objects
+            raise ImportError(f"the tensor module was made for torch and Python {_tensor_facts.made_for}, not {here}: {how}")
         _FACTS = _tensor_facts.facts, _tensor_facts.pointers
     return _FACTS
 

@@ -54,14 +54,30 @@ def torch_root():
     return spec and os.path.dirname(spec.origin)
 
 
+def facts_stamp():
+    return os.path.join(OBJ_DIR, "tensor_facts.made_for")
+
+
+def facts_made_for(root):
+    """What the tensor module depends on besides its source: the interpreter and the torch it is compiled against."""
+    with open(os.path.join(root, "version.py")) as f:
+        return f"{sys.implementation.cache_tag} {root}\n{f.read()}"
+
+
 def build_facts(force):
-    """Start the compiler on the tensor module; None if it is newer than its source, or without torch, whose tensors
-    it reads: the library by itself needs none."""
-    if not force and os.path.exists(FACTS_OUT) and os.path.getmtime(FACTS_OUT) >= os.path.getmtime(FACTS_SRC):
-        return None
+    """Start the compiler on the tensor module; None if it is newer than its source and made for this Python and
+    torch, or without torch, whose tensors it reads: the library by itself needs none."""
     root = torch_root()
     if root is None:
         return None
+    made_for = facts_made_for(root)
+    if not force and os.path.exists(FACTS_OUT) and os.path.getmtime(FACTS_OUT) >= os.path.getmtime(FACTS_SRC):
+        try:
+            with open(facts_stamp()) as f:
+                if f.read() == made_for:
+                    return None
+        except OSError:
+            pass
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     includes = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                 sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
@@ -77,6 +93,9 @@ def finish_facts(proc):
     if proc.returncode != 0:
         raise RuntimeError("g++ failed:\n" + text)
     os.replace(FACTS_OUT + ".tmp", FACTS_OUT)
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    with open(facts_stamp(), "w") as f:
+        f.write(facts_made_for(torch_root()))
 
 
 def build_engine(force: bool, verbose: bool) -> str:

@@ -3,6 +3,7 @@
 // call spent 4-5 of its 8-9 microseconds on them, more than its kernel runs.
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/version.h>
 
 namespace {
 
@@ -95,4 +96,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_facts", nullptr, -1, metho
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__tensor_facts() { return PyModule_Create(&module); }
+// made_for: the torch and the Python that this module was compiled against
+PyMODINIT_FUNC PyInit__tensor_facts() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddObject(m, "made_for", Py_BuildValue("(sii)", TORCH_VERSION, PY_MAJOR_VERSION, PY_MINOR_VERSION)) < 0)
+    Py_CLEAR(m);
+  return m;
+}

@@ -51,3 +51,37 @@ def test_both_are_built_with_torch_and_the_module_once(calls):
     assert calls == ["module", "library", "library"]
     b.build(force=True)
     assert calls[3:] == ["module", "library"]
+
+
+def test_the_module_is_built_again_for_another_torch_or_python(calls, monkeypatch):
+    b.build()
+    for made_for in ("another torch", "another python"):
+        monkeypatch.setattr(b, "facts_made_for", lambda root, made_for=made_for: made_for)
+        del calls[:]
+        b.build()
+        assert calls == ["module", "library"]
+        b.build()
+        assert calls == ["module", "library", "library"]
+
+
+def test_a_module_made_for_another_torch_is_refused(monkeypatch):
+    import sys
+    import types
+
+    from loopspec_b200 import _lib
+    monkeypatch.setattr(_lib, "_FACTS", None)
+    for made_for in (("1.0.0", *sys.version_info[:2]), ("1.0.0", 3, 1)):
+        old = types.ModuleType("loopspec_b200._tensor_facts")
+        old.facts = old.pointers = None
+        old.made_for = made_for
+        monkeypatch.setitem(sys.modules, "loopspec_b200._tensor_facts", old)
+        monkeypatch.setattr(sys.modules["loopspec_b200"], "_tensor_facts", old, raising=False)
+        with pytest.raises(ImportError, match="made for"):
+            _lib.tensor_facts()
+
+
+def test_the_built_module_is_made_for_this_torch():
+    from loopspec_b200 import _lib
+    b.build()
+    facts, pointers = _lib.tensor_facts()
+    assert callable(facts) and callable(pointers)
