@@ -452,6 +452,7 @@ typedef struct ls_prefix_attention_args {
   int32_t prefix_len, max_new, max_len, page_size, n_slots;
   float scale;
 } ls_prefix_attention_args;
+/* Bytes on the current device (they depend on its number of SMs); 0: refused, see ls_last_error(NULL). */
 size_t ls_prefix_attention_workspace_bytes(int n_tokens, int n_requests, int n_heads, int n_kv_heads,
                                            int head_dim, int prefix_len, int max_new, int max_len);
 int ls_prefix_attention(const ls_prefix_attention_args* args, void* stream);

@@ -19,7 +19,7 @@ _pack = _lib.packer(_lib.PrefixAttentionArgs)
 
 
 def workspace_bytes(n_tokens, n_heads, n_kv_heads, head_dim, *, n_requests, prefix_len, max_new, max_len):
-    """Bytes of device scratch of one call (a function of the sizes alone)."""
+    """Bytes of device scratch of one call on the current device: a function of the sizes and of its number of SMs."""
     need = int(_lib.lib().ls_prefix_attention_workspace_bytes(n_tokens, n_requests, n_heads, n_kv_heads, head_dim,
                                                               prefix_len, max_new, max_len))
     if need == 0:
@@ -69,7 +69,7 @@ def prefix_attention(q, k_pool, v_pool, prefix_table, prefix_len, block_table, l
     if scale is None:
         scale = hd ** -0.5
     if out is None or workspace is None:
-        with on_stream(q.device, stream):
+        with torch.cuda.device(gpu), on_stream(q.device, stream):
             if out is None:
                 out = torch.empty(n, nh, hd, dtype=q.dtype, device=q.device)
             if workspace is None:

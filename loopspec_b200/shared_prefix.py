@@ -60,8 +60,9 @@ class PrefixBatch:
         n, k, v = self.n_tokens, self.k[layer], self.v[layer]
         q = qk_norm_rope(qkv, q_weight, k_weight, self.rope, self.map.positions[:n], k, v, self.map.slots[:n], eps=eps,
                          status=self.status)
-        need = workspace_bytes(n, self.n_heads, k.shape[1], k.shape[2], n_requests=self.lens.numel(),
-                               prefix_len=self.prefix_len, max_new=self.max_new, max_len=self.max_len)
+        with torch.cuda.device(k.device):
+            need = workspace_bytes(n, self.n_heads, k.shape[1], k.shape[2], n_requests=self.lens.numel(),
+                                   prefix_len=self.prefix_len, max_new=self.max_new, max_len=self.max_len)
         if self.workspace.numel() < need:
             self.workspace = torch.empty(need, dtype=torch.uint8, device=k.device)
         return prefix_attention(q, k, v, self.prefix_table, self.prefix_len, self.table, self.lens, self.map.token_start,
