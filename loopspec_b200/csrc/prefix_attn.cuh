@@ -95,7 +95,7 @@ constexpr int kUnitWarps = kUnitThreads / 32;
 // stages of a warp's ring that this leaves shared memory for.
 template <int HD, int TERMS, int RT>
 __host__ __device__ constexpr int unit_ctas() {
-  return HD == 128 ? (TERMS * RT <= 3 && RT <= 2 ? 3 : 2) : (TERMS * RT <= 4 && RT <= 2 ? 4 : 3);
+  return HD == 128 ? (TERMS * RT <= 3 ? 3 : 2) : (TERMS * RT <= 4 ? 4 : 3);
 }
 template <int HD, int TERMS, int RT>
 __host__ __device__ constexpr int unit_stages() { return unit_ctas<HD, TERMS, RT>() >= (HD == 128 ? 3 : 4) ? 2 : 3; }
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
         const unsigned char* vb = kb + kUnitKeys * RB;
         // S^T: chains of products that wait for one another cost ~20 cycles a
         // link, so each term (or half of the head) has accumulators of its own
-        constexpr int CHAINS = TERMS == 1 && RT < 4 ? 2 : TERMS;
+        constexpr int CHAINS = TERMS == 1 ? 2 : TERMS;
         float acc[CHAINS][RT][4];
 #pragma unroll
         for (int i = 0; i < CHAINS; ++i)

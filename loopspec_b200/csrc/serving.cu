@@ -188,7 +188,7 @@ struct PrefixPlan {
   int tc_tiles;     // 128-row tiles a CTA of the tcgen05 kernel takes; 0: the stream kernel does everything
   bool own;         // it takes one request's rows and also does that request's own positions
   int prefix_parts, prefix_chunk, suffix_parts, suffix_chunk, prefix_tiles, suffix_tiles;
-  int prefix_rt, suffix_rt;   // eights of rows in a tile of the stream kernel
+  int rt;                     // eights of rows in a tile of the stream kernel
   int stream_sms;             // SMs the stream kernel is launched for
   size_t o_bytes, ml_bytes, total;
 };
@@ -267,11 +267,11 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
   const long most_rows = (long)std::min(max_new, n_tokens) * G, mean_rows = cdiv(rows, n_requests);
 
   // one way: the prefix for all rows together, the requests' own positions by the stream kernel
-  p.suffix_rt = tile_eights(most_rows);
-  p.suffix_tiles = cdiv(most_rows, 8 * p.suffix_rt);
+  p.rt = tile_eights(most_rows);
+  p.suffix_tiles = cdiv(most_rows, 8 * p.rt);
   p.stream_sms = sms;
-  const double own_tiles = (double)n_requests * nkv * cdiv(mean_rows, 8 * p.suffix_rt) * max_len / 16 / 2;
-  const double stream_cycles = max_len ? stream_tile_cycles(terms, p.suffix_rt) * own_tiles + kStreamAround * sms : 0;
+  const double own_tiles = (double)n_requests * nkv * cdiv(mean_rows, 8 * p.rt) * max_len / 16 / 2;
+  const double stream_cycles = max_len ? stream_tile_cycles(terms, p.rt) * own_tiles + kStreamAround * sms : 0;
   double cycles = stream_cycles / sms + kJoinAround;
   if (rows > 16 && prefix_len > 0) {
     p.tc_tiles = terms > 1 || rows <= kTcRows ? 1 : 2;
@@ -280,8 +280,7 @@ PrefixPlan make_plan(int n_tokens, int n_requests, int nh, int nkv, int hd, int 
     cycles = share(p, prefix_len, tc_tile_cycles(hd, terms, p.tc_tiles), stream_cycles, sms, units) + kJoinAround;
   } else {
     // one launch for both if it reads the prefix no more than twice (from L2)
-    p.prefix_rt = p.suffix_rt;
-    p.prefix_tiles = cdiv(rows, 8 * p.prefix_rt);
+    p.prefix_tiles = cdiv(rows, 8 * p.rt);
     const long units = (long)p.prefix_tiles * nkv;
     cut(units, prefix_len, 12L * sms, least_keys(units, prefix_len, sms), 16, 4 * kMaxParts, p.prefix_parts,
         p.prefix_chunk);
@@ -372,17 +371,9 @@ void launch_prefix(PrefixAttnArgs a, const PrefixPlan& plan, cudaStream_t stream
     return;
   }
   const bool prefix = plan.tc_tiles == 0 && a.prefix_parts > 0, suffix = a.suffix_parts > 0 && a.suffix_tiles > 0;
-  bool behind = plan.tc_tiles != 0;
-  if (prefix && suffix && plan.prefix_rt == plan.suffix_rt) {
-    launch_stream<HD, Q, C, TERMS>(a, plan.prefix_rt, true, true, false, plan.stream_sms, stream);
-    behind = true;
-  } else {
-    if (prefix) launch_stream<HD, Q, C, TERMS>(a, plan.prefix_rt, true, false, false, plan.stream_sms, stream);
-    behind = behind || prefix;
-    if (suffix) launch_stream<HD, Q, C, TERMS>(a, plan.suffix_rt, false, true, behind, plan.stream_sms, stream);
-    behind = behind || suffix;
-  }
-  a.behind = behind;
+  const bool behind = plan.tc_tiles != 0;
+  if (prefix || suffix) launch_stream<HD, Q, C, TERMS>(a, plan.rt, prefix, suffix, behind, plan.stream_sms, stream);
+  a.behind = behind || prefix || suffix;
   constexpr int kGroups = kJoinThreads / (HD / 4);
   const dim3 rows((unsigned)a.n_tokens, (unsigned)a.nh), groups((unsigned)a.n_tokens, (unsigned)cdiv(a.nh, kGroups));
   // many parts come with few rows: a row's parts are shared out (4 requests behind
