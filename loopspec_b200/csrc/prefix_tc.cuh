@@ -23,7 +23,8 @@
 //     type (the A operand of the second product comes from tensor memory). O
 //     is rescaled only when a row's maximum has grown by more than 2^8 since
 //     its reference was set: until then the old reference stays, weights reach
-//     2^8, and nothing else changes, as the reference cancels in o / l.
+//     2^8, and nothing else changes, as the reference cancels in o / l. With terms
+//     of an fp32 q they also add up the tiles' products themselves.
 // With MT = 2 the tensor cores work on one row tile while the softmax warps
 // work on the other; with MT = 1 on the next key tile (two score buffers).
 //
@@ -64,11 +65,25 @@ struct TcLayout {
   static constexpr int kProducers = kStages >= 5 ? 3 : 2;
   static_assert(kStages >= kProducers + 2, "a stage's turns would be mistaken for one another");
   static constexpr int kMma = kProducer + kProducers;      // the issuing warp
-  static constexpr int kThreads = 32 * (kMma + 1);
-  // With MT = 2 a thread is launched with 96 registers; the softmax warps draw
-  // on what the last four warps give back: 640 x 96 = 512 x 104 + 128 x 64.
-  static constexpr int kSoftRegs = 104, kRestRegs = 64;
-  static constexpr int kLaunchRegs = MT == 2 ? (512 * kSoftRegs + 128 * kRestRegs) / kThreads : 0;
+  // The tensor cores' sums lose their lower bits towards zero with every addition,
+  // so the error of one sum over a unit's keys grows with their number: with fp32
+  // queries 2.0e-5 of the output behind 8192 positions, 3.9e-5 behind 16384. With
+  // terms of an fp32 q each key tile's product is therefore a sum of its own, and
+  // the softmax warps add them up in registers, rounding to nearest: 7e-7 to 9e-7 at
+  // any length. (With 16-bit q the rounding of P is a hundred times that.)
+  static constexpr bool kOwnSums = TERMS > 1;
+  static constexpr bool kShareRegs = MT == 2 || kOwnSums;
+  static constexpr int kSoftWarps = 8 * MT;
+  // a whole number of warpgroups where registers are handed over
+  static constexpr int kThreads = kShareRegs ? 32 * (kSoftWarps + 4) : 32 * (kMma + 1);
+  static_assert(kThreads >= 32 * (kMma + 1), "a warp for each role");
+  // The softmax warps draw on what the last four warps give back. With MT = 2 a
+  // thread is launched with 96 registers: 640 x 96 = 512 x 104 + 128 x 64; with
+  // sums of their own with 168: 384 x 168 = 256 x 200 + 128 x 104 (with 56 left to
+  // the two or three producers they hold up the rest: 1600 tokens behind 4096, fp32
+  // on bf16, heads of 128: 196 us, 165 with 104, 172 without handing over).
+  static constexpr int kSoftRegs = MT == 2 ? 104 : 200, kRestRegs = MT == 2 ? 64 : 104;
+  static constexpr int kLaunchRegs = kShareRegs ? (32 * kSoftWarps * kSoftRegs + 128 * kRestRegs) / kThreads : 0;
   static constexpr int kMaxBuffers = MT == 1 ? 2 : 1;      // see the softmax warps
   static constexpr int kBars = 2 * kStages + 2 + 2 + 2 + 2 + 1 + 1;
   static constexpr int kQTiles = MT * TERMS;
@@ -388,7 +403,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
 
   if (warp < L::kProducer) {
     // ---------------------------------------------------------------- softmax
-    if (MT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftRegs));
+    if (L::kShareRegs) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L::kSoftRegs));
     const int t = MT == 2 ? warp >> 3 : 0, half = (warp >> 2) & 1, quarter = warp & 3;
     // the row tile's queries, swizzled; rows past the last are zeros
     {
@@ -450,6 +465,15 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       const float scale_log2 = kScaledRows<TERMS, C> ? s_scale[r] : a.scale_log2;
       float m = -INFINITY, l = 0.f;
       bool ok = true;
+      float own_sum[L::kOwnSums ? HD / 2 : 1] = {};
+      auto add_product = [&](float keep) {           // ... and all of it brought to the new one
+        uint32_t v[HD / 2];
+#pragma unroll
+        for (int c = 0; c < HD / 2; c += 32) tmem_ld_x32(out + c, v + c);
+        tmem_ld_done(v);
+#pragma unroll
+        for (int i = 0; i < (L::kOwnSums ? HD / 2 : 0); ++i) own_sum[i] = (own_sum[i] + __uint_as_float(v[i])) * keep;
+      };
       for (int j = 0; j < n; ++j) {
         const int b = MT == 1 ? j & 1 : t;
         const uint32_t ph = (MT == 1 ? j >> 1 : j) & 1;
@@ -485,12 +509,13 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         // m and top are raw scores; their distance counts after the scale. A NaN
         // score makes the reference NaN, and with it the whole row
         const bool move = m == -INFINITY ? top != -INFINITY : !((top - m) * scale_log2 <= kGrow);
+        float keep = 1.f;
         if (__any_sync(0xffffffffu, move)) {
-          const float keep = move && m > -INFINITY ? exp2_fast((m - top) * scale_log2) : 1.f;
+          keep = move && m > -INFINITY ? exp2_fast((m - top) * scale_log2) : 1.f;
           if (move) m = top;
           // inf - inf: the row is NaN, whichever way its weights are computed
           l = m == INFINITY ? NAN : l * keep;
-          if (j > 0) {
+          if (!L::kOwnSums && j > 0) {
             wait_on(ok, pv_done + 8 * t, (j - 1) & 1, a.status, kDevTimeoutAcc);
             tc_fence_after();
 #pragma unroll 1
@@ -534,6 +559,13 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
         }
         const float2 total = unpair(add2(sum[0], sum[1]));
         l += total.x + total.y;
+        if constexpr (L::kOwnSums) {
+          if (j > 0) {                               // the product of the tile before this one, by the old reference
+            wait_on(ok, pv_done + 8 * t, (j - 1) & 1, a.status, kDevTimeoutAcc);
+            tc_fence_after();
+            add_product(keep);
+          }
+        }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -544,6 +576,12 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       if (a.own) wait_on(ok, noted, 0, a.status, kDevTimeoutAcc);
       const bool have = n > 0 && ok;
       tc_fence_after();
+      if constexpr (L::kOwnSums) {                   // the sum takes the last product's place
+        add_product(1.f);
+#pragma unroll
+        for (int c = 0; c < HD / 2; c += 16) tmem_st_x16(out + c, reinterpret_cast<const uint32_t*>(own_sum + c));
+        tmem_st_wait();
+      }
       float* row_sum = s_max + ((MT == 1 ? n & 1 : t) * 2) * kTcRows + r;
       row_sum[half * kTcRows] = l;
       asm volatile("bar.sync %0, 64;" ::"r"(pair_bar) : "memory");
@@ -622,7 +660,7 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
       }
       tc_fence_before();
     }
-  } else if (MT == 2) {
+  } else if (L::kShareRegs) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kRestRegs));
   }
   if (warp >= L::kProducer && warp < L::kMma) {
@@ -731,7 +769,8 @@ __global__ void __launch_bounds__(TcLayout<HD, TERMS, MT>::kThreads, 1) prefix_t
 #pragma unroll
         for (int i = 0; i < kTcKeys / 16; ++i)
           tc_mma_ts(leader, tmem + L::kOut + t * 128, tmem + L::kScores + b * L::kBuffer + x * 64 + i * 8,
-                    v + (i * 2048 >> 4), kUmmaHi, idesc_o, i != 0 || x != TERMS - 1 ? 1u : (uint32_t)(j != 0));
+                    v + (i * 2048 >> 4), kUmmaHi, idesc_o,
+                    i != 0 || x != TERMS - 1 ? 1u : L::kOwnSums ? 0u : (uint32_t)(j != 0));
       // A softmax warp at tile j may wait for product j - 1: it knows of j - 2, so
       // the turn is plain. For the last product, which it could be two turns
       // ahead of, there is a barrier of its own.
