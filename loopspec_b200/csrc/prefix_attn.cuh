@@ -658,13 +658,19 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
           for (int e = 0; e < 4; ++e) {
             const float base = (m[rt][e & 1] == -INFINITY ? 0.f : m[rt][e & 1]) - weight_bias(C());
             sc[rt][e] = exp2_fast(sc[rt][e] - base);
-            l[rt][e & 1] += sc[rt][e];
+            if (TERMS > 1) l[rt][e & 1] += sc[rt][e];
           }
         // A weight of 0 times a NaN or infinity is NaN: where some rows of the
         // tile must not see a position that others see, a value that is not
         // finite is kept out of the product, and added one weight at a time
         if (key + kUnitKeys > seen_by_all && any_not_finite<HD, C>(vb, lane)) {
           add_by_weight<HD, C, RT>(o, sc, vb, key, k1, see, lane);
+          if constexpr (TERMS == 1) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) l[rt][e & 1] += sc[rt][e];
+          }
         } else {
           uint32_t pf[TERMS][RT][2];             // P^T as the second operand: rows become columns
 #pragma unroll
@@ -673,6 +679,11 @@ __global__ void __launch_bounds__(kUnitThreads, unit_ctas<HD, TERMS, RT>()) pref
             for (int x = 0; x < 2; ++x) {
               uint32_t term[TERMS];
               split2<TERMS, C>(sc[rt][2 * x], sc[rt][2 * x + 1], term);
+              if constexpr (TERMS == 1) {        // the weights that the product gets: the rounding of a large one cancels
+                const float2 w = unpack2(term[0], C());
+                l[rt][0] += w.x;
+                l[rt][1] += w.y;
+              }
 #pragma unroll
               for (int i = 0; i < TERMS; ++i) pf[i][rt][x] = transpose8x8(term[i]);
             }

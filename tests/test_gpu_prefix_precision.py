@@ -35,3 +35,23 @@ def test_the_error_does_not_grow_with_the_prefix(counts, prefix, nh, nkv, hd, ca
     ref, _, _ = reference(list(c), 16)
     error = float((call(c, 16).double() - ref).norm() / ref.norm())
     assert error <= BOUND, error
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_weights_add_up_to_one(kind, hd):
+    """Where all values are 1 the output is 1, whatever 16-bit weights are rounded to: numerator and sum share it. One
+    key has nearly all the weight here, 2^6.1 to 2^7.9 of the reference, the score of a key 16 before it, so nothing averages out."""
+    rows = 64
+    c = list(make([1] * rows, [40] * rows, 0, 16, 4, 2, hd, kind, kind, seed=3))
+    q, k, table = c[0], c[1], c[5]
+    q[:] = 0
+    q[:, :, 0] = hd ** 0.5
+    for i in range(rows):
+        slots = table[i].long().repeat_interleave(16) * 16 + torch.arange(16).repeat(table.shape[1])
+        k[slots[:40]] = 0
+        k[slots[:40], :, 0] = -30.0
+        k[slots[4], :, 0] = 0.0
+        k[slots[20], :, 0] = (6.1 + 1.8 * i / rows) * 0.6931
+    c[2][:] = 1
+    assert bool((call(c, 16) == 1).all())
