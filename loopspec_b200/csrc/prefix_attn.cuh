@@ -29,8 +29,8 @@
 // its reference was set (the reference cancels in o / l).
 // Bound: the latency of short reads at the lengths of a decode step (a cold read
 // of this size ramps up for some 13 us), then HBM. 16 requests of up to 700
-// positions behind 2048, 16 heads, fp32 q: 63 MB in 22.4 us with the joining
-// pass, 2.8 TB/s; 4 requests behind 333: 7.0 us, call after call in a graph.
+// positions behind 2048, 16 heads, fp32 q: 63 MB in 21.4 us with the joining
+// pass, 2.9 TB/s; 4 requests behind 333: 6.7 us, call after call in a graph.
 //
 // Types: bf16 or f16 K/V. q of the cache's type enters the product exactly.
 // fp32 q enters as a sum of TERMS values of the cache's type, each the

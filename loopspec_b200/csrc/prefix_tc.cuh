@@ -31,9 +31,11 @@
 // Bound: for prompts the softmax warps' issue slots (58 % used, the
 // exponentials' unit 60 %, with the waits on tensor memory between) beside the
 // tensor cores: 4 prompts of up to 700 tokens behind 8192 positions, 32 heads of
-// 128, 290-305 us, 1.0 PFLOP/s, six tenths of a library product's rate; 8 of up
-// to 509 behind 16384, 32 heads of 64, 633 us, 0.66 PFLOP/s, as half as many
-// dimensions come with each exponential. For decode batches the gathering of K
+// 128, 293-326 us by the clock under load, 1.0-0.9 PFLOP/s, six tenths of a library
+// product's rate; 8 of up to 509 behind 16384, 32 heads of 64, 648 us, 0.65 PFLOP/s,
+// as half as many dimensions come with each exponential. fp32 q: 4 prompts of up to
+// 400 behind 4096, 16 heads of 128, 165 us (bf16 cache, three terms), 134 (f16, two).
+// For decode batches the gathering of K
 // and V: 64 requests behind 32768 positions 61 us with their own positions and
 // the joining pass, 203 MB, 3.3 TB/s.
 //
@@ -93,7 +95,8 @@ struct TcLayout {
   // Eighths of the exponentials on the FMA units. The softmax is bound by issue
   // slots: with heads of 128 the tensor cores take longer and none is best
   // (0, 1, 2, 3 eighths: 289, 296, 308, 326 us for 2100 tokens behind 8192
-  // positions), with heads of 64 one (740, 633, 664, 663 us for 3050 behind 16384).
+  // positions), with heads of 64 one (740, 648, 672, 672 us for 3050 behind 16384;
+  // with one it also depends on how the compiler orders the loop: 645 to 760 us).
   static constexpr int kPoly = TERMS == 1 && HD == 64 ? 1 : 0;
   // tensor memory columns: two buffers of scores, each with room for P's terms (64 each) over them, then O
   static constexpr uint32_t kScores = 0, kBuffer = TERMS == 3 ? 192 : 128, kOut = 2 * kBuffer;

@@ -377,7 +377,7 @@ void launch_prefix(PrefixAttnArgs a, const PrefixPlan& plan, cudaStream_t stream
   constexpr int kGroups = kJoinThreads / (HD / 4);
   const dim3 rows((unsigned)a.n_tokens, (unsigned)a.nh), groups((unsigned)a.n_tokens, (unsigned)cdiv(a.nh, kGroups));
   // many parts come with few rows: a row's parts are shared out (4 requests behind
-  // 333 positions: 7.0 us, 9.0 with a group a row; 16 behind 2048: 22.4 and 29.6)
+  // 333 positions: 6.7 us, 9.0 with a group a row; 16 behind 2048: 21.4 and 29.6)
   if (a.prefix_parts + a.suffix_parts > kJoinBatch)
     launch(prefix_join_kernel<HD, Q, C, true>, rows, dim3(kJoinThreads), 0, stream, true, a);
   else launch(prefix_join_kernel<HD, Q, C, false>, groups, dim3(kJoinThreads), 0, stream, true, a);
